@@ -258,6 +258,116 @@ typedef struct SsdStepArgs {
 } SsdStepArgs;
 int ssd_b200_step_strided(const SsdStepArgs* args, void* stream);
 
+/* ---- Pieces of a recurrent block beside the core.  The reference has no counterparts but those named. ---- */
+
+/* Per-channel gated linear recurrence over a sequence: with
+ *   log a[t] = -rate * softplus(decay[c]) * sigmoid(decay_gate[t]),  b[t] = sqrt(1 - a[t]^2),
+ *   h[t] = a[t] * h[t-1] + b[t] * sigmoid(input_gate[t]) * x[t],     y[t] = h[t]
+ * (the carry of model_ref.py:152-157 with a state of one number per channel).  Strides in elements (batch, sequence; reset's
+ * in bytes); channels contiguous.  A token whose reset byte is not 0 starts anew: h[t-1] is left out, whatever it is.
+ * The states entering every 64th token go to `pieces` when given: what ssd_b200_gated_scan_backward() starts from.
+ * Results do not vary from run to run. */
+typedef struct SsdGatedScanArgs {
+  const void* x;                /* [b,s,d]  dtype */
+  const void* input_gate;       /* [b,s,d]  dtype, before the sigmoid */
+  const void* decay_gate;       /* [b,s,d]  dtype, before the sigmoid */
+  const float* decay;           /* [d]      fp32 */
+  const float* initial_state;   /* [b,d]    fp32 contiguous, or NULL for zeros */
+  const uint8_t* reset;         /* [b,s]    bytes, or NULL */
+  void* y;                      /* [b,s,d]  dtype */
+  float* final_state;           /* [b,d]    fp32 contiguous, or NULL */
+  float* pieces;                /* [b,ceil(s/64),d] fp32 contiguous: written by the forward unless NULL, read by the backward */
+  /* the backward alone; every result is written whole */
+  const void* dy;               /* [b,s,d]  dtype */
+  const float* dfinal_state;    /* [b,d]    fp32 contiguous, or NULL for zeros */
+  void* dx;                     /* [b,s,d]  dtype */
+  void* dinput_gate;            /* [b,s,d]  dtype */
+  void* ddecay_gate;            /* [b,s,d]  dtype */
+  float* ddecay;                /* [d]      fp32 */
+  float* dinitial_state;        /* [b,d]    fp32 contiguous, or NULL */
+  void* workspace;              /* ssd_b200_gated_scan_workspace_bytes() bytes, 256-byte aligned; this call's alone while it runs */
+  size_t workspace_bytes;
+  int32_t* status;              /* device int32, or NULL: 8 where a wait between tiles ran out */
+  float rate;                   /* > 0 */
+  int32_t batch, seqlen, channels, dtype;
+  int32_t wait_limit_ms;        /* 0: about one second */
+  int64_t x_stride[2], input_gate_stride[2], decay_gate_stride[2], reset_stride[2], y_stride[2];
+  int64_t dy_stride[2], dx_stride[2], dinput_gate_stride[2], ddecay_gate_stride[2];
+} SsdGatedScanArgs;
+size_t ssd_b200_gated_scan_workspace_bytes(const SsdGatedScanArgs* args, int32_t backward);
+int ssd_b200_gated_scan(const SsdGatedScanArgs* args, void* stream);
+int ssd_b200_gated_scan_backward(const SsdGatedScanArgs* args, void* stream);
+
+/* One token of it, [b,d] operands (stride: batch); state_out may be state. */
+typedef struct SsdGatedStepArgs {
+  const void* x;
+  const void* input_gate;
+  const void* decay_gate;
+  const float* decay;           /* [d]   fp32 */
+  const float* state;           /* [b,d] fp32 contiguous */
+  float* state_out;             /* [b,d] fp32 contiguous */
+  void* y;
+  float rate;                   /* > 0 */
+  int32_t batch, channels, dtype;
+  int64_t x_stride, input_gate_stride, decay_gate_stride, y_stride;
+} SsdGatedStepArgs;
+int ssd_b200_gated_step(const SsdGatedStepArgs* args, void* stream);
+
+/* RMS norms between blocks: the nn.RMSNorm of model_ref.py:49-66, 199, with the residual sum of the block before (:165-204).
+ * ssd_b200_rms_norm, over rows of d numbers:
+ *   o = x, or with post_weight x * rms(x) * post_weight;  o *= scale when given;
+ *   r = residual + o in residual_dtype (residual NULL: r = o, kept in fp32),   y = r * rms(r) * weight,
+ *   rms(v) = 1 / sqrt(mean(v^2) + eps)
+ * y is the norm of r as residual_out holds it.  residual_out may be residual.
+ * ssd_b200_gated_rms_norm: with rms over each of `groups` equal parts of a row,
+ *   y = (x * silu(z)) * rms(x * silu(z)) * weight,  or with norm_first  x * rms(x) * weight * silu(z).
+ * Vectors of d numbers are fp32 or (bit set in vectors_in_dtype: 1 weight, 2 post_weight, 4 scale) of `dtype`, and so
+ * are their gradients.  Strides of rows in elements.  d / groups up to 16384.  inv_rms (fp32 [rows][groups]) and
+ * inv_rms_post ([rows], with post_weight) are written by the forwards unless NULL and read by the backwards.
+ * The backwards write every result whole; sums over rows are in a fixed order. */
+typedef struct SsdNormArgs {
+  const void* x;                /* [rows,d] dtype */
+  const void* z;                /* [rows,d] dtype  (gated) */
+  const void* weight;
+  const void* residual;         /* [rows,d] residual_dtype, or NULL */
+  const void* post_weight;      /* or NULL */
+  const void* scale;            /* or NULL */
+  void* y;                      /* [rows,d] dtype */
+  void* residual_out;           /* [rows,d] residual_dtype: written by the forward, read by the backward */
+  float* inv_rms;
+  float* inv_rms_post;
+  const void* dy;               /* [rows,d] dtype */
+  const void* dresidual_out;    /* [rows,d] residual_dtype, or NULL */
+  void* dx;                     /* [rows,d] dtype */
+  void* dz;                     /* [rows,d] dtype  (gated) */
+  void* dresidual;              /* [rows,d] residual_dtype, or NULL where it is not wanted */
+  void* dweight;                /* [d], or NULL; dpost_weight and dscale the same */
+  void* dpost_weight;
+  void* dscale;
+  void* workspace;              /* backwards: ssd_b200_norm_workspace_bytes() bytes, 16-byte aligned */
+  size_t workspace_bytes;
+  int64_t rows;
+  float eps;
+  int32_t d, groups, norm_first;
+  int32_t dtype, residual_dtype, vectors_in_dtype;
+  int64_t x_stride, z_stride, residual_stride, y_stride, residual_out_stride;
+  int64_t dy_stride, dresidual_out_stride, dx_stride, dz_stride, dresidual_stride;
+} SsdNormArgs;
+size_t ssd_b200_norm_workspace_bytes(const SsdNormArgs* args);
+int ssd_b200_rms_norm(const SsdNormArgs* args, void* stream);
+int ssd_b200_rms_norm_backward(const SsdNormArgs* args, void* stream);
+int ssd_b200_gated_rms_norm(const SsdNormArgs* args, void* stream);
+int ssd_b200_gated_rms_norm_backward(const SsdNormArgs* args, void* stream);
+
+/* Gradient of ssd_b200_conv1d_silu(): dx [batch, seqlen, channels] (strided like x), dweight [channels, taps] and dbias [channels]
+ * (NULL with bias NULL) in `dtype`, of dy.  x, weight and bias are the forward's.  workspace:
+ * ssd_b200_conv1d_silu_workspace_bytes() bytes, 16-byte aligned. */
+size_t ssd_b200_conv1d_silu_workspace_bytes(int32_t batch, int32_t seqlen, int32_t channels, int32_t taps);
+int ssd_b200_conv1d_silu_backward(const void* x, const void* weight, const void* bias, const void* dy, void* dx, void* dweight,
+                                  void* dbias, void* workspace, size_t workspace_bytes, int32_t batch, int32_t seqlen,
+                                  int32_t channels, int32_t taps, int32_t dtype, int64_t x_stride_b, int64_t x_stride_l,
+                                  int64_t dy_stride_b, int64_t dy_stride_l, int64_t dx_stride_b, int64_t dx_stride_l, void* stream);
+
 /* Whole forward with HOST buffers: copies X/A/B/C (and dt, initial_state when
  * given) from host memory, runs the forward and copies Y (and final_state) back,
  * pipelined over batch slices on internal streams.  Every pointer in `host` is a

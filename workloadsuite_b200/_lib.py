@@ -36,6 +36,10 @@ EXPORTS = (
     "ssd_b200_conv1d_silu", "ssd_b200_dt_prologue",
     "ssd_b200_xchg_create", "ssd_b200_xchg_connect", "ssd_b200_xchg_buffer", "ssd_b200_xchg_all_gather",
     "ssd_b200_xchg_destroy", "ssd_b200_step", "ssd_b200_step_strided",
+    "ssd_b200_conv1d_silu_workspace_bytes", "ssd_b200_conv1d_silu_backward",
+    "ssd_b200_gated_scan_workspace_bytes", "ssd_b200_gated_scan", "ssd_b200_gated_scan_backward", "ssd_b200_gated_step",
+    "ssd_b200_norm_workspace_bytes", "ssd_b200_rms_norm", "ssd_b200_rms_norm_backward",
+    "ssd_b200_gated_rms_norm", "ssd_b200_gated_rms_norm_backward",
 )
 XCHG_HANDLE_BYTES = 64
 
@@ -55,6 +59,45 @@ class SsdArgs(C.Structure):
         ("c_stride", C.c_int64 * 3), ("dt_stride", C.c_int64 * 3), ("y_stride", C.c_int64 * 3),
         ("D", C.c_void_p), ("Z", C.c_void_p), ("z_stride", C.c_int64 * 3),
     ]
+
+
+def _fields(pointers, rest):
+    return [(n, C.c_void_p) for n in pointers.split()] + rest
+
+
+def _ints(names):
+    return [(n, C.c_int32) for n in names.split()]
+
+
+class GatedScanArgs(C.Structure):
+    """Mirror of ``struct SsdGatedScanArgs``."""
+
+    _fields_ = _fields(
+        "x input_gate decay_gate decay initial_state reset y final_state pieces dy dfinal_state dx dinput_gate ddecay_gate ddecay "
+        "dinitial_state workspace",
+        [("workspace_bytes", C.c_size_t), ("status", C.c_void_p), ("rate", C.c_float),
+         *_ints("batch seqlen channels dtype wait_limit_ms"),
+         *[(n + "_stride", C.c_int64 * 2) for n in "x input_gate decay_gate reset y dy dx dinput_gate ddecay_gate".split()]])
+
+
+class GatedStepArgs(C.Structure):
+    """Mirror of ``struct SsdGatedStepArgs``."""
+
+    _fields_ = _fields(
+        "x input_gate decay_gate decay state state_out y",
+        [("rate", C.c_float), *_ints("batch channels dtype"),
+         *[(n + "_stride", C.c_int64) for n in "x input_gate decay_gate y".split()]])
+
+
+class NormArgs(C.Structure):
+    """Mirror of ``struct SsdNormArgs``."""
+
+    _fields_ = _fields(
+        "x z weight residual post_weight scale y residual_out inv_rms inv_rms_post dy dresidual_out dx dz dresidual dweight dpost_weight "
+        "dscale workspace",
+        [("workspace_bytes", C.c_size_t), ("rows", C.c_int64), ("eps", C.c_float),
+         *_ints("d groups norm_first dtype residual_dtype vectors_in_dtype"),
+         *[(n + "_stride", C.c_int64) for n in "x z residual y residual_out dy dresidual_out dx dz dresidual".split()]])
 
 
 _LIB = None
@@ -108,6 +151,20 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.ssd_b200_step.argtypes = [C.c_void_p] * 9 + [C.c_int32] * 6 + [C.c_void_p]
     lib.ssd_b200_step_strided.restype = C.c_int
     lib.ssd_b200_step_strided.argtypes = [C.c_void_p, C.c_void_p]
+    lib.ssd_b200_conv1d_silu_workspace_bytes.restype = C.c_size_t
+    lib.ssd_b200_conv1d_silu_workspace_bytes.argtypes = [C.c_int32] * 4
+    lib.ssd_b200_conv1d_silu_backward.restype = C.c_int
+    lib.ssd_b200_conv1d_silu_backward.argtypes = [C.c_void_p] * 8 + [C.c_size_t] + [C.c_int32] * 5 + [C.c_int64] * 6 + [C.c_void_p]
+    lib.ssd_b200_gated_scan_workspace_bytes.restype = C.c_size_t
+    lib.ssd_b200_gated_scan_workspace_bytes.argtypes = [C.POINTER(GatedScanArgs), C.c_int32]
+    for f in (lib.ssd_b200_gated_scan, lib.ssd_b200_gated_scan_backward):
+        f.restype, f.argtypes = C.c_int, [C.POINTER(GatedScanArgs), C.c_void_p]
+    lib.ssd_b200_gated_step.restype = C.c_int
+    lib.ssd_b200_gated_step.argtypes = [C.POINTER(GatedStepArgs), C.c_void_p]
+    lib.ssd_b200_norm_workspace_bytes.restype = C.c_size_t
+    lib.ssd_b200_norm_workspace_bytes.argtypes = [C.POINTER(NormArgs)]
+    for f in (lib.ssd_b200_rms_norm, lib.ssd_b200_rms_norm_backward, lib.ssd_b200_gated_rms_norm, lib.ssd_b200_gated_rms_norm_backward):
+        f.restype, f.argtypes = C.c_int, [C.POINTER(NormArgs), C.c_void_p]
     lib.ssd_b200_xchg_create.restype = C.c_int
     lib.ssd_b200_xchg_create.argtypes = [C.c_size_t, C.c_int32, C.POINTER(C.c_void_p), C.c_void_p]
     lib.ssd_b200_xchg_connect.restype = C.c_int
@@ -140,7 +197,12 @@ def fast():
         spec.loader.exec_module(mod)
         addr = lambda f: C.cast(f, C.c_void_p).value
         mod.init(addr(lib.ssd_b200_forward), addr(lib.ssd_b200_workspace_bytes), addr(lib.ssd_b200_step_strided),
-                 addr(lib.ssd_b200_conv1d_silu), addr(lib.ssd_b200_dt_prologue), _raise)
+                 addr(lib.ssd_b200_conv1d_silu), addr(lib.ssd_b200_dt_prologue),
+                 addr(lib.ssd_b200_conv1d_silu_workspace_bytes), addr(lib.ssd_b200_conv1d_silu_backward),
+                 addr(lib.ssd_b200_gated_scan_workspace_bytes), addr(lib.ssd_b200_gated_scan), addr(lib.ssd_b200_gated_scan_backward),
+                 addr(lib.ssd_b200_gated_step), addr(lib.ssd_b200_norm_workspace_bytes), addr(lib.ssd_b200_rms_norm),
+                 addr(lib.ssd_b200_rms_norm_backward), addr(lib.ssd_b200_gated_rms_norm), addr(lib.ssd_b200_gated_rms_norm_backward),
+                 _raise)
         _FAST = mod
     return _FAST
 

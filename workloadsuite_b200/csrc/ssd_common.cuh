@@ -18,7 +18,8 @@ enum : int {
   STATUS_WAIT_TIMEOUT_SYNC = 3,  // a bounded wait between warps of one CTA ran out
   STATUS_TMEM_ALLOC = 4,         // tensor memory could not be allocated
   STATUS_BAD_SMEM_ALIGNMENT = 5, // dynamic shared memory did not start on a 1024-byte boundary
-  STATUS_WAIT_TIMEOUT_CHAIN = 6  // a bounded wait for the previous segment of a chained sequence ran out
+  STATUS_WAIT_TIMEOUT_CHAIN = 6, // a bounded wait for the previous segment of a chained sequence ran out
+  STATUS_WAIT_TIMEOUT_LOOK_BACK = 8  // gated scan: a bounded wait for the tiles before a tile ran out (7: the peer exchange)
 };
 
 // Words of ScanParams::redo: one per CTA of the tensor-core kernel at fp32 precision, and the counters of the scan behind it.

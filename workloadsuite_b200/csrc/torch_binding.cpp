@@ -29,6 +29,17 @@ decltype(&ssd_b200_workspace_bytes) f_workspace;
 decltype(&ssd_b200_step_strided) f_step;
 decltype(&ssd_b200_conv1d_silu) f_conv;
 decltype(&ssd_b200_dt_prologue) f_dt;
+decltype(&ssd_b200_conv1d_silu_workspace_bytes) f_conv_workspace;
+decltype(&ssd_b200_conv1d_silu_backward) f_conv_backward;
+decltype(&ssd_b200_gated_scan_workspace_bytes) f_gated_workspace;
+decltype(&ssd_b200_gated_scan) f_gated;
+decltype(&ssd_b200_gated_scan_backward) f_gated_backward;
+decltype(&ssd_b200_gated_step) f_gated_step;
+decltype(&ssd_b200_norm_workspace_bytes) f_norm_workspace;
+decltype(&ssd_b200_rms_norm) f_norm;
+decltype(&ssd_b200_rms_norm_backward) f_norm_backward;
+decltype(&ssd_b200_gated_rms_norm) f_gated_norm;
+decltype(&ssd_b200_gated_rms_norm_backward) f_gated_norm_backward;
 PyObject* f_raise;   // raises the Python exception of an error code
 
 constexpr int kMaxDevices = 64;
@@ -250,6 +261,377 @@ PyObject* py_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- a recurrent block's other pieces: gradients and norms ----
+
+// A tuple of tensors; undefined ones are None.
+PyObject* tuple_of(std::initializer_list<Tensor> ts) {
+  PyObject* t = PyTuple_New((Py_ssize_t)ts.size());
+  if (!t) return nullptr;
+  Py_ssize_t i = 0;
+  for (const Tensor& v : ts) PyTuple_SET_ITEM(t, i++, v.defined() ? THPVariable_Wrap(v) : (Py_INCREF(Py_None), Py_None));
+  return t;
+}
+Tensor scratch(const Tensor& like, size_t bytes) {   // from the current stream's memory
+  return bytes ? at::empty({(int64_t)bytes}, like.options().dtype(at::kByte)) : Tensor();
+}
+template <typename T = void>
+T* ptr(const Tensor& t) { return t.defined() ? static_cast<T*>(t.data_ptr()) : nullptr; }
+bool real(PyObject* o, float* v) {
+  if (!PyFloat_CheckExact(o)) return false;
+  *v = (float)PyFloat_AS_DOUBLE(o);
+  return true;
+}
+bool fits(int64_t n) { return n > 0 && n <= 0x7fffffff; }
+// fp32, whole and contiguous, or not given
+bool plain32(const Tensor& t, std::initializer_list<int64_t> s) {
+  return !t.defined() || (t.scalar_type() == at::kFloat && shaped(t, s) && t.is_contiguous());
+}
+bool like3(const Tensor& t, const Tensor& x) { return t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && t.stride(2) == 1; }
+void two(const Tensor& t, int64_t* st) {
+  if (!t.defined()) return;
+  st[0] = t.stride(0);
+  st[1] = t.stride(1);
+}
+
+// What the forward and the backward of the gated scan both check and fill in.
+bool gated_args(const Tensor& x, const Tensor& i, const Tensor& r, const Tensor& decay, const Tensor& init, const Tensor& reset, float rate,
+                const Where& w, SsdGatedScanArgs* a) {
+  const int64_t b = x.size(0), s = x.size(1), d = x.size(2);
+  if (!fits(b) || !fits(s) || !fits(d) || x.stride(2) != 1 || !like3(i, x) || !like3(r, x) || decay.scalar_type() != at::kFloat ||
+      !shaped(decay, {d}) || !decay.is_contiguous() || !plain32(init, {b, d}) ||
+      (reset.defined() && (reset.scalar_type() != at::kBool || !shaped(reset, {b, s}))) || !w.here(i) || !w.here(r) || !w.here(decay) ||
+      !w.here(init) || !w.here(reset))
+    return false;
+  a->x = x.data_ptr(); a->input_gate = i.data_ptr(); a->decay_gate = r.data_ptr();
+  a->decay = ptr<float>(decay);
+  a->initial_state = ptr<float>(init);
+  a->reset = ptr<uint8_t>(reset);
+  a->status = ptr<int32_t>(status_word(w.dev.index()));
+  a->rate = rate;
+  a->batch = (int)b; a->seqlen = (int)s; a->channels = (int)d; a->dtype = dtype_of(x);
+  two(x, a->x_stride); two(i, a->input_gate_stride); two(r, a->decay_gate_stride); two(reset, a->reset_stride);
+  return true;
+}
+
+// gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, wait_limit_ms, want_pieces) -> (y, final_state, pieces or None)
+PyObject* py_gated(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *i, *r, *decay, *init, *reset, *out;
+  float rate;
+  if (n != 10 || !get(o[0], &x) || !get(o[1], &i) || !get(o[2], &r) || !get(o[3], &decay) || !get(o[4], &init, true) ||
+      !get(o[5], &reset, true) || !get(o[6], &out, true) || !real(o[7], &rate) || !PyLong_CheckExact(o[8]) || !x->is_cuda() ||
+      x->dim() != 3 || i->dim() != 3 || r->dim() != 3 || dtype_of(*x) < 0)
+    Py_RETURN_NONE;
+  Where w(*x);
+  SsdGatedScanArgs a = {};
+  if (!gated_args(*x, *i, *r, *decay, *init, *reset, rate, w, &a)) Py_RETURN_NONE;
+  if (out->defined() && (out->dim() != 3 || !like3(*out, *x) || !w.here(*out))) Py_RETURN_NONE;
+  a.wait_limit_ms = (int)PyLong_AsLong(o[8]);
+  const auto f32 = x->options().dtype(at::kFloat);
+  Tensor y = out->defined() ? *out : at::empty(x->sizes(), x->options());
+  Tensor fin = at::empty({x->size(0), x->size(2)}, f32), pieces;
+  if (o[9] == Py_True) pieces = at::empty({x->size(0), (x->size(1) + 63) / 64, x->size(2)}, f32);
+  a.y = y.data_ptr(); a.final_state = ptr<float>(fin); a.pieces = ptr<float>(pieces);
+  two(y, a.y_stride);
+  const size_t need = f_gated_workspace(&a, 0);
+  const Tensor ws = scratch(*x, need);
+  a.workspace = ptr(ws);
+  a.workspace_bytes = need;
+  if (const int rc = f_gated(&a, w.stream())) return declined(rc);
+  return tuple_of({y, fin, pieces});
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_scan_backward(x, input_gate, decay_gate, decay, reset, pieces, dy, dfinal_state, rate, want_dinitial)
+//   -> (dx, dinput_gate, ddecay_gate, ddecay, dinitial_state or None)
+PyObject* py_gated_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *i, *r, *decay, *reset, *pieces, *dy, *dfin;
+  float rate;
+  if (n != 10 || !get(o[0], &x) || !get(o[1], &i) || !get(o[2], &r) || !get(o[3], &decay) || !get(o[4], &reset, true) ||
+      !get(o[5], &pieces) || !get(o[6], &dy) || !get(o[7], &dfin, true) || !real(o[8], &rate) || !x->is_cuda() || x->dim() != 3 ||
+      i->dim() != 3 || r->dim() != 3 || dy->dim() != 3 || dtype_of(*x) < 0)
+    Py_RETURN_NONE;
+  Where w(*x);
+  SsdGatedScanArgs a = {};
+  if (!gated_args(*x, *i, *r, *decay, Tensor(), *reset, rate, w, &a)) Py_RETURN_NONE;
+  const int64_t b = x->size(0), s = x->size(1), d = x->size(2);
+  if (!like3(*dy, *x) || !w.here(*dy) || !plain32(*dfin, {b, d}) || !w.here(*dfin) || !plain32(*pieces, {b, (s + 63) / 64, d}) || !w.here(*pieces))
+    Py_RETURN_NONE;
+  const auto f32 = x->options().dtype(at::kFloat);
+  Tensor dx = at::empty(x->sizes(), x->options()), di = at::empty(x->sizes(), x->options()), dr = at::empty(x->sizes(), x->options());
+  Tensor dd = at::empty({d}, f32), dh;
+  if (o[9] == Py_True) dh = at::empty({b, d}, f32);
+  a.pieces = ptr<float>(*pieces); a.dy = dy->data_ptr(); a.dfinal_state = ptr<float>(*dfin);
+  a.dx = dx.data_ptr(); a.dinput_gate = di.data_ptr(); a.ddecay_gate = dr.data_ptr(); a.ddecay = ptr<float>(dd); a.dinitial_state = ptr<float>(dh);
+  two(*dy, a.dy_stride); two(dx, a.dx_stride); two(di, a.dinput_gate_stride); two(dr, a.ddecay_gate_stride);
+  const size_t need = f_gated_workspace(&a, 1);
+  const Tensor ws = scratch(*x, need);
+  a.workspace = ptr(ws);
+  a.workspace_bytes = need;
+  if (const int rc = f_gated_backward(&a, w.stream())) return declined(rc);
+  return tuple_of({dx, di, dr, dd, dh});
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_step(x, input_gate, decay_gate, decay, state, out_state, out, rate) -> y
+PyObject* py_gated_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *i, *r, *decay, *state, *state_out, *out;
+  float rate;
+  if (n != 8 || !get(o[0], &x) || !get(o[1], &i) || !get(o[2], &r) || !get(o[3], &decay) || !get(o[4], &state) ||
+      !get(o[5], &state_out, true) || !get(o[6], &out, true) || !real(o[7], &rate) || !x->is_cuda() || x->dim() != 2 || i->dim() != 2 ||
+      r->dim() != 2 || dtype_of(*x) < 0)
+    Py_RETURN_NONE;
+  const int64_t b = x->size(0), d = x->size(1);
+  auto like = [&](const Tensor& t) { return t.scalar_type() == x->scalar_type() && t.sizes() == x->sizes() && t.stride(1) == 1; };
+  if (!fits(b) || !fits(d) || !like(*x) || !like(*i) || !like(*r) || decay->scalar_type() != at::kFloat || !shaped(*decay, {d}) ||
+      !decay->is_contiguous() || !plain32(*state, {b, d}) || !plain32(*state_out, {b, d}) || (out->defined() && (out->dim() != 2 || !like(*out))))
+    Py_RETURN_NONE;
+  Where w(*x);
+  if (!w.here(*i) || !w.here(*r) || !w.here(*decay) || !w.here(*state) || !w.here(*state_out) || !w.here(*out)) Py_RETURN_NONE;
+  Tensor y = out->defined() ? *out : at::empty({b, d}, x->options());
+  SsdGatedStepArgs a = {};
+  a.x = x->data_ptr(); a.input_gate = i->data_ptr(); a.decay_gate = r->data_ptr(); a.decay = ptr<float>(*decay);
+  a.state = ptr<float>(*state);
+  a.state_out = state_out->defined() ? ptr<float>(*state_out) : ptr<float>(*state);
+  a.y = y.data_ptr();
+  a.rate = rate;
+  a.batch = (int)b; a.channels = (int)d; a.dtype = dtype_of(*x);
+  a.x_stride = x->stride(0); a.input_gate_stride = i->stride(0); a.decay_gate_stride = r->stride(0); a.y_stride = y.stride(0);
+  if (const int rc = f_gated_step(&a, w.stream())) return declined(rc);
+  return THPVariable_Wrap(std::move(y));
+  END_HANDLE_TH_ERRORS
+}
+
+// Rows of [..., d] that lie one stride apart.
+bool rows_of(const Tensor& t, int64_t* rows, int64_t* stride) {
+  if (t.dim() < 1 || !inner(t)) return false;
+  int64_t n = 1, st = t.size(-1);
+  for (int64_t k = t.dim() - 2; k >= 0; --k) {
+    if (t.size(k) == 1) continue;
+    if (n == 1) st = t.stride(k);
+    else if (t.stride(k) != st * n) return false;
+    n *= t.size(k);
+  }
+  *rows = n;
+  *stride = st;
+  return true;
+}
+// The operands of a norm: checked against x, with their strides.
+struct NormCall {
+  const Tensor& x;
+  Where w;
+  SsdNormArgs a = {};
+  bool ok = true;
+  explicit NormCall(const Tensor& t) : x(t), w(t) {
+    a.d = (int)t.size(-1);
+    a.dtype = dtype_of(t);
+    a.residual_dtype = a.dtype;
+    a.groups = 1;
+    ok = fits(t.size(-1)) && rows_of(t, &a.rows, &a.x_stride) && a.rows > 0;
+    a.x = t.data_ptr();
+  }
+  void* rows(const Tensor& t, at::ScalarType type, int64_t* stride) {
+    if (!t.defined()) return nullptr;
+    int64_t n = 0;
+    ok = ok && t.scalar_type() == type && t.sizes() == x.sizes() && w.here(t) && rows_of(t, &n, stride);
+    return t.data_ptr();
+  }
+  void* vector(const Tensor& t, int bit) {
+    if (!t.defined()) return nullptr;
+    ok = ok && shaped(t, {(int64_t)a.d}) && t.is_contiguous() && w.here(t) && (t.scalar_type() == at::kFloat || t.scalar_type() == x.scalar_type());
+    if (t.scalar_type() == x.scalar_type()) a.vectors_in_dtype |= bit;
+    return t.data_ptr();
+  }
+  float* sums(const Tensor& t, int64_t n) {
+    if (!t.defined()) return nullptr;
+    ok = ok && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == n && w.here(t);
+    return ptr<float>(t);
+  }
+};
+bool norm_operand(const Tensor& x) { return x.is_cuda() && x.dim() >= 1 && dtype_of(x) >= 0; }
+
+// rms_norm(x, weight, residual, post_weight, scale, out, eps, keep) -> (y, residual_out or None, inv_rms or None, inv_rms_post or None)
+PyObject* py_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *wt, *res, *post, *scale, *out;
+  float eps;
+  if (n != 8 || !get(o[0], &x) || !get(o[1], &wt) || !get(o[2], &res, true) || !get(o[3], &post, true) || !get(o[4], &scale, true) ||
+      !get(o[5], &out, true) || !real(o[6], &eps) || !norm_operand(*x))
+    Py_RETURN_NONE;
+  NormCall c(*x);
+  const auto st = x->scalar_type();
+  c.a.weight = c.vector(*wt, 1);
+  c.a.post_weight = c.vector(*post, 2);
+  c.a.scale = c.vector(*scale, 4);
+  if (res->defined()) {
+    if (dtype_of(*res) < 0) Py_RETURN_NONE;
+    c.a.residual_dtype = dtype_of(*res);
+    c.a.residual = c.rows(*res, res->scalar_type(), &c.a.residual_stride);
+  }
+  c.a.y = c.rows(*out, st, &c.a.y_stride);
+  if (!c.ok) Py_RETURN_NONE;
+  const bool keep = o[7] == Py_True;
+  Tensor y = *out, r, inv, invp;
+  if (!y.defined()) {
+    y = at::empty(x->sizes(), x->options());
+    c.a.y = y.data_ptr();
+    c.a.y_stride = c.a.d;
+  }
+  if (res->defined()) {
+    r = at::empty(x->sizes(), res->options());
+    c.a.residual_out = r.data_ptr();
+    c.a.residual_out_stride = c.a.d;
+  }
+  if (keep) inv = at::empty({c.a.rows}, x->options().dtype(at::kFloat));
+  if (keep && post->defined()) invp = at::empty({c.a.rows}, x->options().dtype(at::kFloat));
+  c.a.inv_rms = ptr<float>(inv);
+  c.a.inv_rms_post = ptr<float>(invp);
+  c.a.eps = eps;
+  if (const int rc = f_norm(&c.a, c.w.stream())) return declined(rc);
+  return tuple_of({y, r, inv, invp});
+  END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_backward(x, weight, residual_out, post_weight, scale, inv_rms, inv_rms_post, dy, dresidual_out)
+//   -> (dx, dresidual or None, dweight, dpost_weight or None, dscale or None)
+PyObject* py_norm_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *wt, *r, *post, *scale, *inv, *invp, *dy, *dr;
+  if (n != 9 || !get(o[0], &x) || !get(o[1], &wt) || !get(o[2], &r, true) || !get(o[3], &post, true) || !get(o[4], &scale, true) ||
+      !get(o[5], &inv) || !get(o[6], &invp, true) || !get(o[7], &dy) || !get(o[8], &dr, true) || !norm_operand(*x))
+    Py_RETURN_NONE;
+  NormCall c(*x);
+  const auto st = x->scalar_type();
+  c.a.weight = c.vector(*wt, 1);
+  c.a.post_weight = c.vector(*post, 2);
+  c.a.scale = c.vector(*scale, 4);
+  if (r->defined()) {
+    if (dtype_of(*r) < 0) Py_RETURN_NONE;
+    c.a.residual_dtype = dtype_of(*r);
+    c.a.residual_out = c.rows(*r, r->scalar_type(), &c.a.residual_out_stride);
+    c.a.dresidual_out = c.rows(*dr, r->scalar_type(), &c.a.dresidual_out_stride);
+  } else if (dr->defined()) {
+    Py_RETURN_NONE;
+  }
+  c.a.dy = c.rows(*dy, st, &c.a.dy_stride);
+  c.a.inv_rms = c.sums(*inv, c.a.rows);
+  c.a.inv_rms_post = c.sums(*invp, c.a.rows);
+  if (!c.ok) Py_RETURN_NONE;
+  Tensor dx = at::empty(x->sizes(), x->options()), dres, dw = at::empty({(int64_t)c.a.d}, wt->options()), dpost, dscale;
+  c.a.dx = dx.data_ptr();
+  c.a.dx_stride = c.a.d;
+  if (r->defined()) {
+    // without a norm or a scale behind the block its gradient is the residual's; of one type they are one tensor
+    if (!post->defined() && !scale->defined() && r->scalar_type() == st) {
+      dres = dx;
+    } else {
+      dres = at::empty(x->sizes(), r->options());
+      c.a.dresidual = dres.data_ptr();
+      c.a.dresidual_stride = c.a.d;
+    }
+  }
+  if (post->defined()) dpost = at::empty({(int64_t)c.a.d}, post->options());
+  if (scale->defined()) dscale = at::empty({(int64_t)c.a.d}, scale->options());
+  c.a.dweight = dw.data_ptr(); c.a.dpost_weight = ptr(dpost); c.a.dscale = ptr(dscale);
+  const size_t need = f_norm_workspace(&c.a);
+  const Tensor ws = scratch(*x, need);
+  c.a.workspace = ptr(ws);
+  c.a.workspace_bytes = need;
+  if (const int rc = f_norm_backward(&c.a, c.w.stream())) return declined(rc);
+  return tuple_of({dx, dres, dw, dpost, dscale});
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_rms_norm(x, z, weight, out, eps, groups, norm_first, keep) -> (y, inv_rms or None)
+PyObject* py_gated_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *z, *wt, *out;
+  float eps;
+  if (n != 8 || !get(o[0], &x) || !get(o[1], &z) || !get(o[2], &wt) || !get(o[3], &out, true) || !real(o[4], &eps) ||
+      !PyLong_CheckExact(o[5]) || !norm_operand(*x))
+    Py_RETURN_NONE;
+  const long groups = PyLong_AsLong(o[5]);
+  NormCall c(*x);
+  if (groups <= 0 || groups > c.a.d) Py_RETURN_NONE;
+  c.a.groups = (int)groups;
+  c.a.norm_first = o[6] == Py_True;
+  c.a.weight = c.vector(*wt, 1);
+  c.a.z = c.rows(*z, x->scalar_type(), &c.a.z_stride);
+  c.a.y = c.rows(*out, x->scalar_type(), &c.a.y_stride);
+  if (!c.ok) Py_RETURN_NONE;
+  Tensor y = *out, inv;
+  if (!y.defined()) {
+    y = at::empty(x->sizes(), x->options());
+    c.a.y = y.data_ptr();
+    c.a.y_stride = c.a.d;
+  }
+  if (o[7] == Py_True) inv = at::empty({c.a.rows, (int64_t)groups}, x->options().dtype(at::kFloat));
+  c.a.inv_rms = ptr<float>(inv);
+  c.a.eps = eps;
+  if (const int rc = f_gated_norm(&c.a, c.w.stream())) return declined(rc);
+  return tuple_of({y, inv});
+  END_HANDLE_TH_ERRORS
+}
+
+// gated_rms_norm_backward(x, z, weight, inv_rms, dy, groups, norm_first) -> (dx, dz, dweight)
+PyObject* py_gated_norm_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *z, *wt, *inv, *dy;
+  if (n != 7 || !get(o[0], &x) || !get(o[1], &z) || !get(o[2], &wt) || !get(o[3], &inv) || !get(o[4], &dy) || !PyLong_CheckExact(o[5]) ||
+      !norm_operand(*x))
+    Py_RETURN_NONE;
+  const long groups = PyLong_AsLong(o[5]);
+  NormCall c(*x);
+  if (groups <= 0 || groups > c.a.d) Py_RETURN_NONE;
+  c.a.groups = (int)groups;
+  c.a.norm_first = o[6] == Py_True;
+  c.a.weight = c.vector(*wt, 1);
+  c.a.z = c.rows(*z, x->scalar_type(), &c.a.z_stride);
+  c.a.dy = c.rows(*dy, x->scalar_type(), &c.a.dy_stride);
+  c.a.inv_rms = c.sums(*inv, c.a.rows * groups);
+  if (!c.ok) Py_RETURN_NONE;
+  Tensor dx = at::empty(x->sizes(), x->options()), dz = at::empty(x->sizes(), x->options()), dw = at::empty({(int64_t)c.a.d}, wt->options());
+  c.a.dx = dx.data_ptr(); c.a.dz = dz.data_ptr(); c.a.dweight = dw.data_ptr();
+  c.a.dx_stride = c.a.dz_stride = c.a.d;
+  const size_t need = f_norm_workspace(&c.a);
+  const Tensor ws = scratch(*x, need);
+  c.a.workspace = ptr(ws);
+  c.a.workspace_bytes = need;
+  if (const int rc = f_gated_norm_backward(&c.a, c.w.stream())) return declined(rc);
+  return tuple_of({dx, dz, dw});
+  END_HANDLE_TH_ERRORS
+}
+
+// conv1d_silu_backward(x, weight, bias, dy) -> (dx, dweight, dbias or None)
+PyObject* py_conv_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *w, *bias, *dy;
+  if (n != 4 || !get(o[0], &x) || !get(o[1], &w) || !get(o[2], &bias, true) || !get(o[3], &dy) || !x->is_cuda() || x->dim() != 3 ||
+      dy->dim() != 3)
+    Py_RETURN_NONE;
+  const int64_t b = x->size(0), l = x->size(1), d = x->size(2);
+  const auto st = x->scalar_type();
+  if (dtype_of(*x) < 0 || !fits(b) || !fits(l) || !fits(d) || x->stride(2) != 1 || !like3(*dy, *x) || w->scalar_type() != st ||
+      !w->is_contiguous() || w->dim() < 2 || w->size(0) != d || w->numel() != d * w->size(-1) ||
+      (bias->defined() && (!shaped(*bias, {d}) || bias->scalar_type() != st || !bias->is_contiguous())))
+    Py_RETURN_NONE;
+  Where q(*x);
+  if (!q.here(*w) || !q.here(*bias) || !q.here(*dy)) Py_RETURN_NONE;
+  const int taps = (int)w->size(-1);
+  Tensor dx = at::empty({b, l, d}, x->options()), dw = at::empty(w->sizes(), w->options()), db;
+  if (bias->defined()) db = at::empty({d}, bias->options());
+  const size_t need = f_conv_workspace((int)b, (int)l, (int)d, taps);
+  const Tensor ws = scratch(*x, need);
+  if (const int rc = f_conv_backward(x->data_ptr(), w->data_ptr(), ptr(*bias), dy->data_ptr(), dx.data_ptr(), dw.data_ptr(), ptr(db), ptr(ws),
+                                     need, (int)b, (int)l, (int)d, taps, dtype_of(*x), x->stride(0), x->stride(1), dy->stride(0),
+                                     dy->stride(1), dx.stride(0), dx.stride(1), q.stream()))
+    return declined(rc);
+  return tuple_of({dx, dw, db});
+  END_HANDLE_TH_ERRORS
+}
+
 // workspace(device_index, bytes), status_word(device_index): the tensors that the long way uses too
 PyObject* py_workspace(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -269,29 +651,32 @@ PyObject* py_status(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// init(forward, workspace_bytes, step_strided, conv1d_silu, dt_prologue, raise): addresses in the loaded library, and the
-// function that raises the exception of an error code
+// init(addresses in the loaded library, in the order of the entry points above, and the function that raises the exception of an
+// error code)
+template <typename F>
+void bind(F& f, PyObject* address) { f = reinterpret_cast<F>(PyLong_AsVoidPtr(address)); }
 PyObject* py_init(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  if (n != 6) {
-    PyErr_SetString(PyExc_TypeError, "init takes five addresses and a function");
+  if (n != 17) {
+    PyErr_SetString(PyExc_TypeError, "init takes sixteen addresses and a function");
     return nullptr;
   }
-  void* f[5];
-  for (int i = 0; i < 5; ++i) f[i] = PyLong_AsVoidPtr(o[i]);
+  bind(f_forward, o[0]); bind(f_workspace, o[1]); bind(f_step, o[2]); bind(f_conv, o[3]); bind(f_dt, o[4]);
+  bind(f_conv_workspace, o[5]); bind(f_conv_backward, o[6]);
+  bind(f_gated_workspace, o[7]); bind(f_gated, o[8]); bind(f_gated_backward, o[9]); bind(f_gated_step, o[10]);
+  bind(f_norm_workspace, o[11]); bind(f_norm, o[12]); bind(f_norm_backward, o[13]); bind(f_gated_norm, o[14]); bind(f_gated_norm_backward, o[15]);
   if (PyErr_Occurred()) return nullptr;
-  f_forward = reinterpret_cast<decltype(f_forward)>(f[0]);
-  f_workspace = reinterpret_cast<decltype(f_workspace)>(f[1]);
-  f_step = reinterpret_cast<decltype(f_step)>(f[2]);
-  f_conv = reinterpret_cast<decltype(f_conv)>(f[3]);
-  f_dt = reinterpret_cast<decltype(f_dt)>(f[4]);
-  Py_INCREF(o[5]);
-  Py_XSETREF(f_raise, o[5]);
+  Py_INCREF(o[16]);
+  Py_XSETREF(f_raise, o[16]);
   Py_RETURN_NONE;
 }
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"init", FAST(py_init)}, {"step", FAST(py_step)}, {"dt_prologue", FAST(py_dt)},
-                         {"conv1d_silu", FAST(py_conv)}, {"forward", FAST(py_forward)}, {"workspace", FAST(py_workspace)},
+                         {"conv1d_silu", FAST(py_conv)}, {"conv1d_silu_backward", FAST(py_conv_backward)},
+                         {"gated_scan", FAST(py_gated)}, {"gated_scan_backward", FAST(py_gated_backward)},
+                         {"gated_step", FAST(py_gated_step)}, {"rms_norm", FAST(py_norm)}, {"rms_norm_backward", FAST(py_norm_backward)},
+                         {"gated_rms_norm", FAST(py_gated_norm)}, {"gated_rms_norm_backward", FAST(py_gated_norm_backward)},
+                         {"forward", FAST(py_forward)}, {"workspace", FAST(py_workspace)},
                          {"status_word", FAST(py_status)}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ssd_b200_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

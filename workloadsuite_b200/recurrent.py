@@ -1,0 +1,338 @@
+"""A recurrent block's pieces beside the SSD core, with their gradients: a per-channel gated linear recurrence
+(``gated_scan``, ``gated_scan_step``) and the block's RMS norms (``rms_norm``, ``gated_rms_norm``).
+
+The reference has the norms as ``nn.RMSNorm`` with a residual sum of its own (``model_ref.py:49-66, 165-204``) and no
+counterpart of the recurrence.  All run in the kernels of ``csrc/ssd_gated_scan.cu`` and ``csrc/ssd_norm.cu`` on the current
+CUDA stream, without a CPU path, and never synchronise the host.
+"""
+from __future__ import annotations
+
+import math
+from typing import Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import _lib
+from .ssd import _DTYPES, _check_out, _same_device
+
+
+def _records(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _need_cuda(name: str, x: torch.Tensor):
+    if not x.is_cuda:
+        raise RuntimeError(f"{name} needs CUDA tensors (there is no CPU path)")
+
+
+def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A tensor whose channels do not lie side by side is copied once; anything else stays the view it is."""
+    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+
+
+def _done(got, name: str):
+    if got is None:
+        raise NotImplementedError(f"{name}: sizes or strides outside what the kernels cover")
+    return got
+
+
+# ---- gated recurrence -----------------------------------------------------------------------------------
+
+def _check_gates(name, x, input_gate, decay_gate, decay, dims, rate):
+    _need_cuda(name, x)
+    if x.dim() != dims:
+        raise ValueError(f"x must be [{'b,s,d' if dims == 3 else 'b,d'}]")
+    _same_device(x, input_gate=input_gate, decay_gate=decay_gate, decay=decay)
+    if x.dtype not in _DTYPES:
+        raise TypeError("x must be float32, float16 or bfloat16")
+    for what, t in (("input_gate", input_gate), ("decay_gate", decay_gate)):
+        if t.shape != x.shape or t.dtype != x.dtype:
+            raise ValueError(f"{what} must have the shape and dtype of x")
+    if decay.shape != x.shape[-1:] or decay.dtype not in _DTYPES:
+        raise ValueError("decay must be a floating point [d]")
+    if not 0 < rate < math.inf:
+        raise ValueError("rate must be positive and finite")
+
+
+def _check_state(name, t, x):
+    want = (x.shape[0], x.shape[-1])
+    if t.shape != want or t.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 [b,d]")
+
+
+def _gated_forward(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, wait_limit_ms, keep):
+    if x.numel() == 0:      # no tokens: the state stays what it was
+        y = torch.empty_like(x) if out is None else out
+        shape = (x.shape[0], x.shape[2])
+        fin = x.new_zeros(shape, dtype=torch.float32) if initial_state is None else initial_state.clone()
+        return y, fin, x.new_empty((0,), dtype=torch.float32)
+    return _done(_lib.fast().gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, wait_limit_ms, keep), "gated_scan")
+
+
+class _GatedScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, input_gate, decay_gate, decay, initial_state, reset, rate, wait_limit_ms):
+        y, fin, pieces = _gated_forward(x, input_gate, decay_gate, decay, initial_state, reset, None, rate, wait_limit_ms, True)
+        ctx.save_for_backward(x, input_gate, decay_gate, decay, reset, pieces)
+        ctx.rate, ctx.has_state = rate, initial_state is not None
+        ctx.set_materialize_grads(False)
+        return y, fin
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dfin):
+        x, input_gate, decay_gate, decay, reset, pieces = ctx.saved_tensors
+        if dy is None and dfin is None:
+            return (None,) * 8
+        if x.numel() == 0:
+            return (torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(decay),
+                    (torch.zeros_like(pieces.new_empty((x.shape[0], x.shape[2]))) if dfin is None else dfin.clone())
+                    if ctx.has_state else None, None, None, None)
+        dy = torch.zeros_like(x, memory_format=torch.contiguous_format) if dy is None else _rows(dy)
+        dfin = None if dfin is None else dfin.contiguous()
+        grads = _done(_lib.fast().gated_scan_backward(x, input_gate, decay_gate, decay, reset, pieces, dy, dfin, ctx.rate, ctx.has_state),
+                      "gated_scan")
+        return (*grads, None, None, None)
+
+
+def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tensor, decay: torch.Tensor,
+               initial_state: Optional[torch.Tensor] = None, reset: Optional[torch.Tensor] = None,
+               return_final_state: bool = False, rate: float = 8.0, out: Optional[torch.Tensor] = None,
+               wait_limit_ms: int = 0):
+    """Per-channel gated linear recurrence over a sequence, on the current CUDA stream, with its gradient::
+
+        log a[t] = -rate * softplus(decay) * sigmoid(decay_gate[t])
+        h[t]     = a[t] * h[t-1] + sqrt(1 - a[t]^2) * sigmoid(input_gate[t]) * x[t],      y = h
+
+    x, input_gate, decay_gate [b,s,d] in one dtype of float32/float16/bfloat16 (views with contiguous channels, such as columns of
+    a projection's output, are read where they lie); decay [d], one number per channel, float32 or any of those;
+    initial_state float32 [b,d] or None for zeros; reset bool [b,s]: a token that is marked starts anew, as if the state
+    before it were zero, whatever it was (documents packed into one row).  Gates, decays and the state are float32
+    throughout; y is rounded once, to x's dtype.  Sequences of no tokens are allowed.
+
+    Returns y [b,s,d], with ``return_final_state`` also the float32 state [b,d] behind the last token (the
+    ``initial_state`` of a call that goes on, or the ``state`` of ``gated_scan_step``).  Differentiable in x, both gates, decay and
+    initial_state, through y and through the final state; the gradient makes the states again in float32 from those of
+    every 64th token, which the forward then keeps (d / 16 bytes a token).  ``out`` receives y where no gradient is recorded.
+    Results and gradients do not vary from run to run.  Waits between the CTAs of a launch are bounded as in ``ssd_forward``
+    (``device_status`` 8).
+    """
+    rate = float(rate)
+    records = _records(x, input_gate, decay_gate, decay, initial_state)
+    if not records and wait_limit_ms == 0:
+        got = _lib.fast().gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, 0, False) if 0 < rate < math.inf else None
+        if got is not None:
+            return got[:2] if return_final_state else got[0]
+    _check_gates("gated_scan", x, input_gate, decay_gate, decay, 3, rate)
+    _same_device(x, initial_state=initial_state, reset=reset, out=out)
+    if wait_limit_ms < 0:
+        raise ValueError("wait_limit_ms must not be negative")
+    if initial_state is not None:
+        _check_state("initial_state", initial_state, x)
+        initial_state = initial_state.contiguous()
+    if reset is not None and (reset.shape != x.shape[:2] or reset.dtype != torch.bool):
+        raise ValueError("reset must be bool [b,s]")
+    if out is not None:
+        if records:
+            raise ValueError("out cannot be given where a gradient is recorded")
+        _check_out(out, x)
+    x, input_gate, decay_gate, decay = _rows(x), _rows(input_gate), _rows(decay_gate), decay.float().contiguous()
+    if records:
+        y, fin = _GatedScan.apply(x, input_gate, decay_gate, decay, initial_state, reset, rate, int(wait_limit_ms))
+    else:
+        y, fin, _ = _gated_forward(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, int(wait_limit_ms), False)
+    return (y, fin) if return_final_state else y
+
+
+def gated_scan_step(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tensor, decay: torch.Tensor, state: torch.Tensor,
+                    rate: float = 8.0, out: Optional[torch.Tensor] = None, out_state: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """One token of ``gated_scan`` on the current CUDA stream, the state carried in place (decode-style use).
+
+    x, input_gate, decay_gate [b,d] in one dtype, decay [d], state float32 [b,d] contiguous, updated in place, or left as it
+    is where ``out_state`` (the same shape) receives the new one: a token that may yet be taken back.  Returns y [b,d].
+    Records no gradient.
+    """
+    rate = float(rate)
+    got = _lib.fast().gated_step(x, input_gate, decay_gate, decay, state, out_state, out, rate) if 0 < rate < math.inf else None
+    if got is not None:
+        return got
+    _check_gates("gated_scan_step", x, input_gate, decay_gate, decay, 2, rate)
+    _same_device(x, state=state, out_state=out_state, out=out)
+    for name, t in (("state", state), ("out_state", out_state)):
+        if t is not None:
+            _check_state(name, t, x)
+            if not t.is_contiguous():
+                raise ValueError(f"{name} must be contiguous")
+    if out is not None:
+        _check_out(out, x)
+    if x.numel() == 0:
+        return torch.empty_like(x) if out is None else out
+    return _done(_lib.fast().gated_step(_rows(x), _rows(input_gate), _rows(decay_gate), decay.detach().float().contiguous(), state,
+                                        out_state, out, rate), "gated_scan_step")
+
+
+# ---- norms ----------------------------------------------------------------------------------------------
+
+_EPS = torch.finfo(torch.float32).eps     # what nn.RMSNorm takes where none is given
+
+
+def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """[..., d] whose rows do not lie at one distance is copied once."""
+    if t is None or t.dim() < 2:
+        return t if t is None or t.stride(-1) == 1 else t.contiguous()
+    try:
+        t.view(-1, t.shape[-1])
+    except RuntimeError:
+        return t.contiguous()
+    return _rows(t)
+
+
+def _check_norm(name, x, eps, vectors, rows, groups=1):
+    _need_cuda(name, x)
+    if x.dim() < 1 or x.dtype not in _DTYPES:
+        raise TypeError("x must be [...,d] of float32, float16 or bfloat16")
+    _same_device(x, **vectors, **rows)
+    for what, t in vectors.items():
+        if t is not None and (t.shape != x.shape[-1:] or t.dtype not in (torch.float32, x.dtype)):
+            raise ValueError(f"{what} must be [d], float32 or in x's dtype")
+    for what, t in rows.items():
+        if t is not None and t.shape != x.shape:
+            raise ValueError(f"{what} must have the shape of x")
+    if x.shape[-1] == 0:
+        raise ValueError("rows must not be empty")
+    if not 0 <= eps < math.inf:
+        raise ValueError("eps must be finite and not negative")
+    if groups <= 0 or x.shape[-1] % groups != 0:
+        raise ValueError("groups must divide d")
+
+
+def _norm_forward(x, weight, residual, post_weight, scale, out, eps, keep):
+    if x.numel() == 0:
+        empty = x.new_empty((0,), dtype=torch.float32)
+        return (torch.empty_like(x) if out is None else out, None if residual is None else torch.empty_like(residual), empty,
+                empty if post_weight is not None else None)
+    return _done(_lib.fast().rms_norm(x, weight, residual, post_weight, scale, out, eps, keep), "rms_norm")
+
+
+class _RmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, residual, post_weight, scale, eps):
+        y, r, inv, invp = _norm_forward(x, weight, residual, post_weight, scale, None, eps, True)
+        # the block's output itself is needed again only behind a norm or a scale, or where it is what is normalised
+        outer = post_weight is not None or scale is not None
+        ctx.save_for_backward(x if outer or r is None else None, weight, r, post_weight, scale, inv, invp)
+        ctx.dtype = x.dtype
+        ctx.set_materialize_grads(False)
+        return y if r is None else (y, r)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy, dr=None):
+        x, weight, r, post_weight, scale, inv, invp = ctx.saved_tensors
+        if dy is None and dr is None:
+            return (None,) * 6
+        like = x if x is not None else r
+        zero = lambda t: None if t is None else torch.zeros_like(t)
+        if like.numel() == 0:
+            return torch.zeros_like(like, dtype=ctx.dtype), zero(weight), zero(r), zero(post_weight), zero(scale), None
+        dy = torch.zeros(like.shape, dtype=ctx.dtype, device=like.device) if dy is None else _flat(dy)
+        if x is None:       # nothing is read of it but its shape and type
+            x = dy
+        dx, dres, dw, dpost, dscale = _done(
+            _lib.fast().rms_norm_backward(_flat(x), weight, r, post_weight, scale, inv, invp, dy, _flat(dr)), "rms_norm")
+        return dx, dw, dres, dpost, dscale, None
+
+
+def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None, residual: Optional[torch.Tensor] = None,
+             post_weight: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
+    """RMS norm ahead of a block, with what lies between two blocks in the same pass, on the current CUDA stream, and its gradient.
+
+    Without ``residual``: ``x * rms(x) * weight``, ``rms(v) = 1 / sqrt(mean(v^2) + eps)``, the ``nn.RMSNorm`` of
+    ``model_ref.py:49-66``.  With ``residual`` x is what the block before has put out, and the call returns (y, residual_out)::
+
+        o = x,  or with post_weight  x * rms(x) * post_weight  (a norm behind the block);   o *= scale  when given
+        residual_out = residual + o,         y = residual_out * rms(residual_out) * weight
+
+    x [...,d] of float32/float16/bfloat16 (rows may be views); residual and residual_out in x's dtype or float32; weight, post_weight and
+    scale [d], float32 or in x's dtype; d up to 16384.  Sums are float32 and everything is rounded once; y is the norm of
+    residual_out as it is stored.  ``eps`` None is float32's, as in ``nn.RMSNorm``.  ``out`` receives y where no gradient is recorded.
+    """
+    eps = _EPS if eps is None else float(eps)
+    records = _records(x, weight, residual, post_weight, scale)
+    if not records and (residual is not None or (post_weight is None and scale is None)) and 0 <= eps < math.inf:
+        got = _lib.fast().rms_norm(x, weight, residual, post_weight, scale, out, eps, False)
+        if got is not None:
+            return got[0] if residual is None else got[:2]
+    _check_norm("rms_norm", x, eps, dict(weight=weight, post_weight=post_weight, scale=scale), dict(residual=residual, out=out))
+    if residual is None and (post_weight is not None or scale is not None):
+        raise ValueError("post_weight and scale apply to what is added to residual: give one")
+    if residual is not None and residual.dtype not in (torch.float32, x.dtype):
+        raise ValueError("residual must be float32 or in x's dtype")
+    if out is not None:
+        if records:
+            raise ValueError("out cannot be given where a gradient is recorded")
+        _check_out(out, x)
+        if _flat(out) is not out:
+            raise ValueError("out: rows must lie at one distance from each other")
+    vectors = [None if t is None else t.contiguous() for t in (weight, post_weight, scale)]
+    x, residual = _flat(x), _flat(residual)
+    if records:
+        return _RmsNorm.apply(x, vectors[0], residual, vectors[1], vectors[2], eps)
+    y, r, _, _ = _norm_forward(x, vectors[0], residual, vectors[1], vectors[2], out, eps, False)
+    return y if residual is None else (y, r)
+
+
+def _gated_norm_forward(x, z, weight, out, eps, groups, norm_first, keep):
+    if x.numel() == 0:
+        return torch.empty_like(x) if out is None else out, x.new_empty((0,), dtype=torch.float32)
+    return _done(_lib.fast().gated_rms_norm(x, z, weight, out, eps, groups, norm_first, keep), "gated_rms_norm")
+
+
+class _GatedRmsNorm(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, z, weight, eps, groups, norm_first):
+        y, inv = _gated_norm_forward(x, z, weight, None, eps, groups, norm_first, True)
+        ctx.save_for_backward(x, z, weight, inv)
+        ctx.groups, ctx.norm_first = groups, norm_first
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, dy):
+        x, z, weight, inv = ctx.saved_tensors
+        if x.numel() == 0:
+            return torch.zeros_like(x), torch.zeros_like(z), torch.zeros_like(weight), None, None, None
+        grads = _done(_lib.fast().gated_rms_norm_backward(x, z, weight, inv, _flat(dy), ctx.groups, ctx.norm_first), "gated_rms_norm")
+        return (*grads, None, None, None)
+
+
+def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None, groups: int = 1,
+                   norm_first: bool = False, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """RMS norm and gate ahead of a block's output projection, on the current CUDA stream, with its gradient:
+    ``(x * silu(z)) * rms(x * silu(z)) * weight``, or with ``norm_first`` ``x * rms(x) * weight * silu(z)``, rms over each of
+    ``groups`` equal parts of a row.
+
+    x and z [...,d] in one dtype of float32/float16/bfloat16 (rows may be views, such as columns of a projection's output); weight [d],
+    float32 or in x's dtype; d / groups up to 16384.  float32 inside, one rounding.  ``eps`` and ``out`` as in ``rms_norm``.
+    """
+    eps = _EPS if eps is None else float(eps)
+    groups, norm_first = int(groups), bool(norm_first)
+    records = _records(x, z, weight)
+    if not records and 0 <= eps < math.inf:
+        got = _lib.fast().gated_rms_norm(x, z, weight, out, eps, groups, norm_first, False)
+        if got is not None:
+            return got[0]
+    _check_norm("gated_rms_norm", x, eps, dict(weight=weight), dict(z=z, out=out), groups)
+    if z.dtype != x.dtype:
+        raise ValueError("z must be in x's dtype")
+    if out is not None:
+        if records:
+            raise ValueError("out cannot be given where a gradient is recorded")
+        _check_out(out, x)
+        if _flat(out) is not out:
+            raise ValueError("out: rows must lie at one distance from each other")
+    x, z, weight = _flat(x), _flat(z), weight.contiguous()
+    if records:
+        return _GatedRmsNorm.apply(x, z, weight, eps, groups, norm_first)
+    return _gated_norm_forward(x, z, weight, out, eps, groups, norm_first, False)[0]

@@ -30,7 +30,7 @@ def device_status(device="cuda:0", clear: bool = True) -> int:
     """Synchronises and returns the kernels' status word for ``device`` (0 = fine; 1/2/3 = a bounded
     wait on TMA / tensor-core / intra-CTA synchronisation ran out and the kernel gave up; 6 = the wait for
     the piece of a sequence handed over by another CTA ran out; 7 = the peer-memory exchange waited in vain for
-    another rank)."""
+    another rank; 8 = ``gated_scan``'s wait for the tokens before a tile's ran out)."""
     device = torch.device(device)
     st = _status_word(device)
     torch.cuda.synchronize(device)
@@ -293,6 +293,29 @@ def ssd_forward(
     return outs[0] if len(outs) == 1 else tuple(outs)
 
 
+class _ConvSilu(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias):
+        ctx.save_for_backward(x, weight, bias)
+        with torch.no_grad():
+            return conv1d_silu(x, weight, bias)
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, dy):
+        x, weight, bias = ctx.saved_tensors
+        got = _lib.fast().conv1d_silu_backward(_pairs(x), weight, bias, _pairs(dy))
+        if got is None:
+            raise NotImplementedError("conv1d_silu: sizes outside what the kernels cover")
+        return got
+
+
+def _pairs(t: torch.Tensor) -> torch.Tensor:
+    """What the gradient's kernel reads two channels at a time of; other views are copied once."""
+    ok = t.stride(2) == 1 and t.stride(0) % 2 == 0 and t.stride(1) % 2 == 0 and t.data_ptr() % (2 * t.element_size()) == 0
+    return t if ok else t.contiguous()
+
+
 def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal depthwise conv1d + SiLU on the current CUDA stream: ``silu(conv1d(x^T)[..., :l])^T`` of
@@ -300,8 +323,12 @@ def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
 
     x [b,l,d] with a contiguous channel axis (a column slice of the projection output is fine); weight the
     ``nn.Conv1d(d, d, k, groups=d)`` parameter [d,1,k] (or [d,k]); bias [d] or None.  Returns [b,l,d] contiguous
-    in x's dtype (fp32 accumulation, one rounding).
+    in x's dtype (fp32 accumulation, one rounding).  Differentiable in x, weight and bias (where ``out`` is given no
+    gradient is recorded).
     """
+    if out is None and torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
+        if x.is_cuda and x.dim() == 3 and x.dtype in _DTYPES and weight.shape[0] == x.shape[2]:
+            return _ConvSilu.apply(x, weight.to(x.dtype).contiguous(), None if bias is None else bias.to(x.dtype).contiguous())
     got = _lib.fast().conv1d_silu(x, weight, bias, out)
     if got is not None:
         return got
