@@ -6,23 +6,28 @@
 //   dr = (g a h[t-1] - g si x a^2 / b) la (1 - sr),   ddecay = -rate sigmoid(decay) sum_t (...) sr,   dh[0] = a[1] g[1]
 // with b = sqrt(1 - a^2), si = sigmoid(i), sr = sigmoid(r), la = log a.
 //
-// Tokens fall into runs (one thread: kRun tokens of two channels, its a and u in registers), runs into tiles (one CTA: 64
-// channels, up to 16 runs).  A run, a tile: h_out = P h_in + q.  The runs' pairs meet in shared memory, the tiles' in scratch: a
-// tile publishes its pair, finds the state entering it by a look back at the pairs and states before it, publishes the state
-// leaving it, and goes through its tokens again, in registers.  So every input is read once and every output written once.
-// Tiles take their numbers from a counter in the order they start in: what a tile waits for has started before it.
+// Tokens fall into runs (one warp: kRun tokens of 64 channels, two a lane, their a and u in registers), runs into tiles (one CTA at a
+// time), tiles into sequences.  A run, a tile: h_out = P h_in + q.  The runs' pairs (P, q) meet in shared memory, the tiles' in scratch: a
+// tile publishes its pair, finds the state entering it by a look back at the states and pairs before it, publishes the state
+// leaving it, and goes through its tokens again, from registers.  So every input is read once and every output written once.
+// CTAs stay on the chip and take tiles from a counter, time first; the next tile's inputs are on their way (TMA) while one is worked on.
+// What a tile waits for has a lower number, and the lowest one that is not done waits for nothing.
 // A state is only ever folded through whole tiles' pairs, h <- P h + q, one tile after the other, wherever the look back begins:
 // results do not depend on what was published when.
 // Entering states of 64-token pieces are kept for the gradient, which makes every h again in fp32 instead of reading y.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
+#include "tc_common.cuh"
+#include "tc_ptx.cuh"
 #include "vec_io.cuh"
 
 namespace ssd {
 namespace {
 
-constexpr int kRun = 8, kRunGrad = 4, kRuns = 16, kStrip = 64, kPiece = 64;
+constexpr int kRuns = 8, kThreads = 32 * kRuns, kStrip = 64, kPiece = 64, kLook = 2 * kRuns;
+constexpr int kRun = 16, kRunGrad = 8;
 constexpr int kTile = kRun * kRuns, kTileGrad = kRunGrad * kRuns;
 static_assert(kTile % kPiece == 0 && kPiece % kRun == 0 && kTileGrad == kPiece, "pieces start at runs");
 
@@ -33,12 +38,12 @@ struct Scan {
   const unsigned char* reset;
   float *fin, *pieces, *part, *dinit;
   unsigned* counter;             // scratch, all bits set at launch: counter, pairs [tile][64], states [tile][64]
-  unsigned long long* pairs;
-  unsigned* states;
+  unsigned long long *pairs, *states;
   int32_t* status;
   long long wait_clocks;
   float rate;
   int batch, seqlen, channels, strips, tiles, npieces;
+  unsigned total;                // tiles of all sequences
   int64_t xs[2], is[2], rs[2], ys[2], dys[2], dxs[2], dis[2], drs[2], ms[2];
 };
 
@@ -51,18 +56,11 @@ __device__ __forceinline__ unsigned word(float v) {
   const unsigned b = __float_as_uint(v);
   return b == kNone ? 0x7fffffffu : b;
 }
-__device__ __forceinline__ unsigned load_word(const unsigned* p) {
-  unsigned v;
-  asm volatile("ld.relaxed.gpu.global.u32 %0, [%1];" : "=r"(v) : "l"(p) : "memory");
-  return v;
-}
+__device__ __forceinline__ unsigned long long two_words(unsigned lo, unsigned hi) { return (unsigned long long)lo | (unsigned long long)hi << 32; }
 __device__ __forceinline__ unsigned long long load_word(const unsigned long long* p) {
   unsigned long long v;
   asm volatile("ld.relaxed.gpu.global.u64 %0, [%1];" : "=l"(v) : "l"(p) : "memory");
   return v;
-}
-__device__ __forceinline__ void store_word(unsigned* p, unsigned v) {
-  asm volatile("st.relaxed.gpu.global.u32 [%0], %1;" ::"l"(p), "r"(v) : "memory");
 }
 __device__ __forceinline__ void store_word(unsigned long long* p, unsigned long long v) {
   asm volatile("st.relaxed.gpu.global.u64 [%0], %1;" ::"l"(p), "l"(v) : "memory");
@@ -70,377 +68,567 @@ __device__ __forceinline__ void store_word(unsigned long long* p, unsigned long 
 
 // State behind a run or a tile (P, q) that `s` enters.  Where P has underflowed an infinite state stays one, as token by token.
 __device__ __forceinline__ float pass(float P, float q, float s) {
-  if (__float_as_uint(P) == kFresh) return q;
-  if (P == 0.f && isinf(s)) return s + q;
-  return fmaf(P, s, q);
+  float r = fmaf(P, s, q);
+  if (P == 0.f) {
+    if (__float_as_uint(P) == kFresh) r = q;
+    else if (isinf(s)) r = s + q;
+  }
+  return r;
 }
 
-// -rate * softplus(decay), and -rate * sigmoid(decay), its derivative
+// rate * softplus(decay): what -log a is at most
 __device__ __forceinline__ float decay_rate(float rate, float decay) {
-  return -rate * (fmaxf(decay, 0.f) + log1pf(expf(-fabsf(decay))));
+  return rate * (fmaxf(decay, 0.f) + log1pf(expf(-fabsf(decay))));
 }
 
-// One number's gates.  Where a is near 1 it is 1 - q, q = 1 - e^-v (v = -la) by its series: an exponential by itself is off by some 2^-23 of
-// a, and a state that some thousand tokens stay in adds that up.  The series' rest is below 4e-8 of q up to v = 0.4; beyond, a state is
-// gone before errors add up.  1 - a^2 = q (1 + a) loses nothing in either case.
+// The gates of two channels.  v = -log a; where a is near 1 it is 1 - q, q = 1 - e^-v by a polynomial (the minimax one of fifth degree on
+// [0, 1/2], 1.4e-9 of q): an exponential by itself is off by some 2^-23 of a, and a state that some thousand tokens stay in adds that
+// up.  Beyond 1/2 a state is gone before errors add up.  1 - a^2 = q (1 + a) loses nothing in either case.
+// MILD: v stays below 1/2 however far the gate opens (rate * softplus(decay) does), as it does where layers are initialised.
+constexpr float kMild = 0.5f;
+template <bool MILD>
 struct Gates {
-  float sr, la, a, om;
-  __device__ __forceinline__ Gates(float k, float r) {
-    sr = sigmoid_approx(r);
-    la = k * sr;
-    const float v = -la;
-    float p = 1.f / 5040;
-    p = fmaf(p, v, -1.f / 720);
-    p = fmaf(p, v, 1.f / 120);
-    p = fmaf(p, v, -1.f / 24);
-    p = fmaf(p, v, 1.f / 6);
-    p = fmaf(p, v, -0.5f);
-    p = fmaf(p, v, 1.f);
-    const float e = exp2_approx(kLog2E * la), q = v < 0.4f ? p * v : 1.f - e;
-    a = v < 0.4f ? 1.f - q : e;
-    om = q * (1.f + a);
+  Pair sr, v, a, om;
+  __device__ __forceinline__ Gates(Pair k, Pair r) {
+    const Pair one = both(1.f);
+    sr = each(each(r * both(-kLog2E), exp2_approx) + one, rcp_approx);
+    v = k * sr;
+    Pair p = fma(both(-0.001121634905f), v, both(0.008187385975f));
+    p = fma(p, v, both(-0.04162908913f));
+    p = fma(p, v, both(0.1666622408f));
+    p = fma(p, v, both(-0.4999998075f));
+    p = fma(p, v, both(0.9999999986f));
+    Pair q = p * v;
+    a = fma(q, both(-1.f), one);
+    if constexpr (!MILD) {
+      const float2 vv = halves(v), e = halves(each(v * both(-kLog2E), exp2_approx)), qq = halves(q), aa = halves(a);
+      const bool m0 = vv.x < kMild, m1 = vv.y < kMild;
+      q = pair(m0 ? qq.x : 1.f - e.x, m1 ? qq.y : 1.f - e.y);
+      a = pair(m0 ? aa.x : e.x, m1 ? aa.y : e.y);
+    }
+    om = q * (a + one);
   }
-  // 1 / sqrt(1 - a^2), 0 where a is 1: it comes with factors that vanish faster
-  __device__ __forceinline__ float inv() const { return om == 0.f ? 0.f : rsqrt_approx(om); }
+  // 1 / sqrt(1 - a^2); where a is 1 a large number, which comes with factors that are zero
+  __device__ __forceinline__ Pair inv() const { return each(om, [](float f) { return rsqrt_approx(fmaxf(f, 1.17549435e-38f)); }); }
 };
 
-template <typename T, bool VEC>
-struct Lane {
-  int c, apart;        // first channel, distance of the second
-  bool ok0, ok1;
-  int j0, j1;          // their places among the strip's 64
-  __device__ __forceinline__ Lane(int strip, int channels) {
-    const int l = threadIdx.x % 32;
-    j0 = VEC ? 2 * l : l;
-    apart = VEC ? 1 : 32;
-    j1 = j0 + apart;
-    c = strip * kStrip + j0;
-    ok0 = c < channels;
-    ok1 = c + apart < channels;
-  }
+// Pairs of a run or a tile, of a lane's two channels.
+struct Share {
+  Pair P, q;
 };
+__device__ __forceinline__ Pair pass(Share f, Pair s) {
+  const float2 P = halves(f.P), q = halves(f.q), h = halves(s);
+  return pair(pass(P.x, q.x, h.x), pass(P.y, q.y, h.y));
+}
+// `s` through shares first, first + step, .. (n of them).  One multiply-add each unless that gives a NaN, which it does not where
+// infinities are left out by a reset or an underflow: then by the rule.
+template <typename At>
+__device__ __forceinline__ Pair through(Pair s, int n, At at) {
+  Pair r = s;
+#pragma unroll 4
+  for (int v = 0; v < n; ++v) {
+    const Share f = at(v);
+    r = fma(f.P, r, f.q);
+  }
+  const float2 h = halves(r);
+  if (isnan(h.x) || isnan(h.y)) {
+    r = s;
+    for (int v = 0; v < n; ++v) r = pass(at(v), r);
+  }
+  return r;
+}
+__device__ __forceinline__ bool is_fresh(Pair P) { return P.v == two_words(kFresh, kFresh); }
 
+template <int SIDES>
 struct Shared {
-  float P[kRuns][kStrip], q[kRuns][kStrip], in[kRuns][kStrip];
-  float2 seen[kRuns][kStrip];
-  unsigned ticket;
+  Share run[2][SIDES][kRuns][32];   // of the runs, tiles in turn; the gradient's other side is that of the way back
+  Share seen[kLook][32];            // of the tiles before this one, the nearest first
+  unsigned ticket[2];
+  int dead;                         // a wait ran out: no further one
+  alignas(8) uint64_t full[2];
 };
 
-// Which tile this CTA works on: (place in its sequence, strip and batch entry).
-__device__ __forceinline__ int2 take_tile(const Scan& p, Shared& sh) {
+struct Maps {
+  CUtensorMap at[4];
+};
+
+// Takes the next tile's number and sends for its inputs (one thread).
+template <typename T, bool TMA, int N, int TILE>
+__device__ __forceinline__ void send_for(const Scan& p, const Maps& maps, unsigned* ticket, uint64_t* full, unsigned turn, T* stage, bool backwards) {
+  const unsigned t = p.tiles == 1 ? blockIdx.x + turn * gridDim.x : atomicAdd(p.counter, 1u) + 1u;
+  *ticket = t;
+  if (!TMA || t >= p.total) {
+    ptx::mbar_arrive(full);
+    return;
+  }
+  ptx::mbar_expect_tx(full, N * TILE * kStrip * sizeof(T));
   const unsigned units = (unsigned)p.strips * p.batch;
-  if (p.tiles == 1) return make_int2(0, (int)blockIdx.x);
-  if (threadIdx.x == 0) sh.ticket = atomicAdd(p.counter, 1u) + 1u;
-  __syncthreads();
-  return make_int2((int)(sh.ticket / units), (int)(sh.ticket % units));
+  const int u = (int)(t % units), k = backwards ? p.tiles - 1 - (int)(t / units) : (int)(t / units);
+#pragma unroll
+  for (int n = 0; n < N; ++n)
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
+                     ptx::smem_u32(stage + n * TILE * kStrip)),
+                 "l"(&maps.at[n]), "r"(ptx::smem_u32(full)), "r"(u % p.strips * kStrip), "r"(k * TILE), "r"(u / p.strips)
+                 : "memory");
 }
 
-// What stands before tile `k` of the unit, into sh.seen: warp w looks at tile k - 1 - w, for its state or else its pair; the farthest
-// one waits for the state, so that one look is enough.
-__device__ __forceinline__ void look_back(const Scan& p, Shared& sh, int64_t first, int k, int j0, int j1) {
-  const int w = threadIdx.x / 32, nw = blockDim.x / 32;
-  if (w < k) {
-    const int64_t at = (first + k - 1 - w) * kStrip;
-    const bool far = w == nw - 1;
-    unsigned s0, s1;
-    unsigned long long p0 = ~0ull, p1 = ~0ull;
+template <int SIDES>
+__device__ __forceinline__ void wait_for(const Scan& p, Shared<SIDES>& sh, uint64_t* full, unsigned parity) {
+  if (ptx::mbar_try_wait(full, parity)) return;
+  const long long t0 = clock64();
+  while (!ptx::mbar_try_wait(full, parity)) {
+    if (*(volatile int*)&sh.dead) return;
+    if (clock64() - t0 > p.wait_clocks) {
+      *(volatile int*)&sh.dead = 1;
+      if (p.status) *p.status = STATUS_WAIT_TIMEOUT_TMA;
+      return;
+    }
+  }
+}
+
+// One operand's tile where TMA cannot read it (rows that do not start on 16 bytes): two channels a lane, by all threads.
+template <typename T, int TILE>
+__device__ __forceinline__ void fill(T* to, const void* from, int b, int t0, int seqlen, const int64_t* st, int c, int channels) {
+  const int lane = threadIdx.x % 32;
+  const T* at = static_cast<const T*>(from) + b * st[0] + (int64_t)t0 * st[1] + c;
+  for (int t = threadIdx.x / 32; t < TILE; t += kRuns) {
+    const bool there = t0 + t < seqlen;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int l = lane + 32 * e;
+      to[t * kStrip + l] = there && c + l < channels ? at[t * st[1] + l] : Cvt<T>::from_f(0.f);
+    }
+  }
+}
+
+// Tokens of a run that are marked, a bit each.
+template <int L>
+__device__ __forceinline__ unsigned marks_of(const Scan& p, int b, int t0, int here) {
+  if (!p.reset) return 0;
+  const int t = threadIdx.x % 32;
+  return __ballot_sync(~0u, t < here && p.reset[b * p.ms[0] + (int64_t)(t0 + t) * p.ms[1]]);
+}
+
+// The share of the whole tile, runs in their order (or, for the way back, from the last to the first).
+__device__ __forceinline__ Share whole(const Share (&run)[kRuns][32], bool backwards) {
+  const int lane = threadIdx.x % 32;
+  auto at = [&](int v) { return run[backwards ? kRuns - 1 - v : v][lane]; };
+  Share all = {both(1.f), through(both(0.f), kRuns, at)};
+  bool f0 = false, f1 = false;
+#pragma unroll
+  for (int v = 0; v < kRuns; ++v) {
+    const Pair P = at(v).P;
+    f0 |= (unsigned)P.v == kFresh;
+    f1 |= (unsigned)(P.v >> 32) == kFresh;
+    all.P = all.P * P;
+  }
+  const float2 P = halves(all.P);
+  const float fresh = __uint_as_float(kFresh);
+  all.P = pair(f0 ? fresh : P.x, f1 ? fresh : P.y);
+  return all;
+}
+
+__device__ __forceinline__ void publish(const Scan& p, int64_t tile, Share f) {
+  const float2 P = halves(f.P), q = halves(f.q);
+  unsigned long long* at = p.pairs + tile * kStrip + 2 * (threadIdx.x % 32);
+  store_word(at, two_words(word(P.x), __float_as_uint(q.x)));
+  store_word(at + 1, two_words(word(P.y), __float_as_uint(q.y)));
+}
+__device__ __forceinline__ void publish(const Scan& p, int64_t tile, Pair s) {
+  const float2 h = halves(s);
+  store_word(p.states + tile * (kStrip / 2) + threadIdx.x % 32, two_words(word(h.x), word(h.y)));
+}
+
+// What stands before tile `k` of the unit, into sh.seen: warp w looks at tiles k - 1 - w and k - 1 - kRuns - w, for their states or else
+// their pairs; the farthest one waits for the state, so that one look is enough.
+template <int SIDES>
+__device__ __forceinline__ void look_back(const Scan& p, Shared<SIDES>& sh, int64_t first, int k) {
+  const int lane = threadIdx.x % 32;
+#pragma unroll
+  for (int w = threadIdx.x / 32; w < kLook; w += kRuns) {
+    if (w >= k) return;
+    const int64_t tile = first + k - 1 - w;
+    const unsigned long long *at = p.pairs + tile * kStrip + 2 * lane, *state = p.states + tile * (kStrip / 2) + lane;
+    unsigned long long s, p0 = ~0ull, p1 = ~0ull;
     const long long t0 = clock64();
+    bool have;
     while (true) {
-      s0 = load_word(p.states + at + j0);
-      s1 = load_word(p.states + at + j1);
-      if (!far) {
-        p0 = load_word(p.pairs + at + j0);
-        p1 = load_word(p.pairs + at + j1);
+      s = load_word(state);
+      if (w != kLook - 1) {
+        p0 = load_word(at);
+        p1 = load_word(at + 1);
       }
-      if ((s0 != kNone || (unsigned)p0 != kNone) && (s1 != kNone || (unsigned)p1 != kNone)) break;
+      have = (unsigned)s != kNone && (unsigned)(s >> 32) != kNone;
+      if (have || ((unsigned)p0 != kNone && (unsigned)p1 != kNone)) break;
+      if (*(volatile int*)&sh.dead) break;
       if (clock64() - t0 > p.wait_clocks) {
+        *(volatile int*)&sh.dead = 1;
         if (p.status) *p.status = STATUS_WAIT_TIMEOUT_LOOK_BACK;
         break;
       }
       __nanosleep(20);
     }
+    auto lo = [](unsigned long long v) { return __uint_as_float((unsigned)v); };
+    auto hi = [](unsigned long long v) { return __uint_as_float((unsigned)(v >> 32)); };
     const float fresh = __uint_as_float(kFresh);
-    sh.seen[w][j0] = s0 != kNone ? make_float2(fresh, __uint_as_float(s0))
-                                 : make_float2(__uint_as_float((unsigned)p0), __uint_as_float((unsigned)(p0 >> 32)));
-    sh.seen[w][j1] = s1 != kNone ? make_float2(fresh, __uint_as_float(s1))
-                                 : make_float2(__uint_as_float((unsigned)p1), __uint_as_float((unsigned)(p1 >> 32)));
+    sh.seen[w][lane] = have ? Share{both(fresh), pair(lo(s), hi(s))} : Share{pair(lo(p0), lo(p1)), pair(hi(p0), hi(p1))};
   }
 }
 
-// The state entering a tile from what look_back() saw.
-__device__ __forceinline__ float fold_seen(const Shared& sh, int k, int j) {
-  float s = 0.f;
-  for (int w = min(k, (int)blockDim.x / 32) - 1; w >= 0; --w) s = pass(sh.seen[w][j].x, sh.seen[w][j].y, s);
-  return s;
+// The state entering a tile from what look_back() saw: from the nearest place that nothing before it matters to.
+template <int SIDES>
+__device__ __forceinline__ Pair fold_seen(const Shared<SIDES>& sh, int k) {
+  const int n = min(k, kLook), lane = threadIdx.x % 32;
+  int w = 0;
+  while (w < n - 1 && !is_fresh(sh.seen[w][lane].P)) ++w;
+  return through(both(0.f), w + 1, [&](int v) { return sh.seen[w - v][lane]; });
 }
 
-__device__ __forceinline__ void publish_pair(const Scan& p, int64_t tile, int j, float P, float q) {
-  store_word(p.pairs + tile * kStrip + j, (unsigned long long)word(P) | (unsigned long long)__float_as_uint(q) << 32);
-}
+constexpr size_t stage_numbers(int n, int tile) { return (size_t)n * tile * kStrip; }
 
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(32 * kRuns, 2) gated_scan_kernel(const Scan p) {
+// Lane l of a warp works on channels 2 l and 2 l + 1 of the strip.
+struct Lane {
+  int c;
+  bool ok0, ok1;
+  __device__ __forceinline__ Lane(int strip, int channels) {
+    c = strip * kStrip + 2 * (threadIdx.x % 32);
+    ok0 = c < channels;
+    ok1 = c + 1 < channels;
+  }
+  __device__ __forceinline__ Pair get(const float* row) const { return pair(ok0 ? row[c] : 0.f, ok1 ? row[c + 1] : 0.f); }
+  __device__ __forceinline__ void put(float* row, Pair v) const {
+    const float2 h = halves(v);
+    if (ok0) row[c] = h.x;
+    if (ok1) row[c + 1] = h.y;
+  }
+  __device__ __forceinline__ Pair rates(const Scan& p) const {
+    return pair(ok0 ? decay_rate(p.rate, p.decay[c]) : 0.f, ok1 ? decay_rate(p.rate, p.decay[c + 1]) : 0.f);
+  }
+  // two channels of an output's row, at once where the row starts on their boundary
+  template <typename T, bool TMA>
+  __device__ __forceinline__ void store(T* row, Pair v) const {
+    const float2 h = halves(v);
+    const typename Two<T>::Raw raw = Two<T>::down(h.x, h.y);
+    if constexpr (TMA) {
+      if (ok0) *reinterpret_cast<typename Two<T>::Raw*>(row) = raw;   // (channels are even)
+    } else {
+      if (ok0) row[0] = Two<T>::lo(raw);
+      if (ok1) row[1] = Two<T>::hi(raw);
+    }
+  }
+};
+
+// TMA: every tensor's rows start on 16 bytes.
+template <typename T, bool TMA>
+__global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
   using Raw = typename Two<T>::Raw;
-  __shared__ Shared sh;
-  const int2 which = take_tile(p, sh);
-  const int k = which.x, strip = which.y % p.strips, b = which.y / p.strips;
-  const int w = threadIdx.x / 32, nw = blockDim.x / 32;
-  const int t0 = k * kTile + w * kRun;
-  const int here = min(kRun, p.seqlen - t0);   // tokens of this run that are there
-  const Lane<T, VEC> ln(strip, p.channels);
-  const int64_t tile = (int64_t)which.y * p.tiles;   // the sequence's first
-
-  Raw rx[kRun], ri[kRun], rr[kRun];
-  {
-    const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + (int64_t)t0 * p.xs[1] + ln.c;
-    const T* i = static_cast<const T*>(p.i) + b * p.is[0] + (int64_t)t0 * p.is[1] + ln.c;
-    const T* r = static_cast<const T*>(p.r) + b * p.rs[0] + (int64_t)t0 * p.rs[1] + ln.c;
-#pragma unroll
-    for (int t = 0; t < kRun; ++t) {
-      const bool there = t < here;
-      rr[t] = load_two<T, VEC>(r + t * p.rs[1], ln.apart, there && ln.ok0, there && ln.ok1);
-      ri[t] = load_two<T, VEC>(i + t * p.is[1], ln.apart, there && ln.ok0, there && ln.ok1);
-      rx[t] = load_two<T, VEC>(x + t * p.xs[1], ln.apart, there && ln.ok0, there && ln.ok1);
-    }
+  constexpr int L = kRun, kStage = (int)stage_numbers(3, kTile);
+  extern __shared__ __align__(128) unsigned char smem[];
+  T* const stages = reinterpret_cast<T*>(smem);
+  Shared<1>& sh = *reinterpret_cast<Shared<1>*>(smem + 2 * kStage * sizeof(T));
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const unsigned units = (unsigned)p.strips * p.batch;
+  if (threadIdx.x == 0) {
+    sh.dead = 0;
+    ptx::mbar_init(&sh.full[0], 1);
+    ptx::mbar_init(&sh.full[1], 1);
+    ptx::fence_mbar_init();
+    for (int s = 0; s < 2; ++s) send_for<T, TMA, 3, kTile>(p, maps, &sh.ticket[s], &sh.full[s], s, stages + s * kStage, false);
   }
-  unsigned marks = 0;
-  if (p.reset) {
-    const unsigned char* m = p.reset + b * p.ms[0] + (int64_t)t0 * p.ms[1];
-#pragma unroll
-    for (int t = 0; t < kRun; ++t)
-      if (t < here && m[t * p.ms[1]]) marks |= 1u << t;
-  }
-  const float k0 = ln.ok0 ? decay_rate(p.rate, p.decay[ln.c]) : 0.f;
-  const float k1 = ln.ok1 ? decay_rate(p.rate, p.decay[ln.c + ln.apart]) : 0.f;
-
-  float a[kRun][2], u[kRun][2];
-  float P[2] = {1.f, 1.f}, q[2] = {0.f, 0.f};
-  const float fresh = __uint_as_float(kFresh);
-#pragma unroll
-  for (int t = 0; t < kRun; ++t) {
-    const float2 xv = Two<T>::up(rx[t]), iv = Two<T>::up(ri[t]), rv = Two<T>::up(rr[t]);
-    const Gates g0(k0, rv.x), g1(k1, rv.y);
-    a[t][0] = g0.a; a[t][1] = g1.a;
-    u[t][0] = (g0.om * g0.inv()) * (sigmoid_approx(iv.x) * xv.x);
-    u[t][1] = (g1.om * g1.inv()) * (sigmoid_approx(iv.y) * xv.y);
-    if (t >= here) a[t][0] = a[t][1] = 1.f, u[t][0] = u[t][1] = 0.f;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const bool cut = marks >> t & 1;
-      P[e] = cut ? fresh : P[e] * a[t][e];
-      q[e] = cut ? u[t][e] : fmaf(a[t][e], q[e], u[t][e]);
-    }
-  }
-  sh.P[w][ln.j0] = P[0]; sh.P[w][ln.j1] = P[1];
-  sh.q[w][ln.j0] = q[0]; sh.q[w][ln.j1] = q[1];
   __syncthreads();
 
-  const int j = threadIdx.x, cj = strip * kStrip + j;
-  const bool fold = j < kStrip;
-  const bool last = k == p.tiles - 1;
-  auto first_state = [&]() { return p.init && cj < p.channels ? p.init[(int64_t)b * p.channels + cj] : 0.f; };
-  float tp = 1.f, tq = 0.f;   // the tile's pair
-  if (fold) {
-    for (int v = 0; v < nw; ++v) {
-      tq = pass(sh.P[v][j], sh.q[v][j], tq);
-      tp = __float_as_uint(sh.P[v][j]) == kFresh ? fresh : tp * sh.P[v][j];
+  for (unsigned turn = 0;; ++turn) {
+    const int s = turn & 1;
+    T* const stage = stages + s * kStage;
+    wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
+    const unsigned ticket = sh.ticket[s];
+    if (ticket >= p.total) break;
+    const int k = (int)(ticket / units), unit = (int)(ticket % units), strip = unit % p.strips, b = unit / p.strips;
+    const int t0 = k * kTile + w * L;
+    const int here = min(L, p.seqlen - t0);   // tokens of this run that are there
+    const Lane ln(strip, p.channels);
+    const int64_t first = (int64_t)unit * p.tiles;
+    if constexpr (!TMA) {
+      const int c = strip * kStrip;
+      fill<T, kTile>(stage, p.x, b, k * kTile, p.seqlen, p.xs, c, p.channels);
+      fill<T, kTile>(stage + kTile * kStrip, p.i, b, k * kTile, p.seqlen, p.is, c, p.channels);
+      fill<T, kTile>(stage + 2 * kTile * kStrip, p.r, b, k * kTile, p.seqlen, p.rs, c, p.channels);
+      __syncthreads();
     }
-    if (k > 0 && !last) publish_pair(p, tile + k, j, tp, tq);
-  }
-  if (k > 0) {
-    look_back(p, sh, tile, k, ln.j0, ln.j1);
+    const Raw* const raw = reinterpret_cast<const Raw*>(stage + w * L * kStrip) + lane;
+    auto rx = [&](int t) { return raw[t * 32]; };
+    auto ri = [&](int t) { return raw[t * 32 + kTile * 32]; };
+    auto rr = [&](int t) { return raw[t * 32 + 2 * kTile * 32]; };
+    const unsigned marks = marks_of<L>(p, b, t0, here);
+    const Pair rate = ln.rates(p);
+
+    Pair a[L], u[L];
+    Share own = {both(1.f), both(0.f)};
+    if (here > 0) {
+      Raw least = ri(0);
+#pragma unroll
+      for (int t = 1; t < L; ++t) least = Two<T>::least(least, ri(t));
+      const float2 kk = halves(rate), ll = Two<T>::up(least);
+      // u = x om / (sqrt(om) (1 + e^-i)): one reciprocal square root of om (1 + e^-i)^2 where that is no overflow
+      if (__all_sync(~0u, kk.x < kMild && kk.y < kMild && ll.x > -40.f && ll.y > -40.f)) {
+#pragma unroll
+        for (int t = 0; t < L; ++t) {
+          const Gates<true> g(rate, pair_of<T>(rr(t)));
+          const Pair d = each(pair_of<T>(ri(t)) * both(-kLog2E), exp2_approx) + both(1.f);
+          const Pair m = each(g.om * (d * d), [](float f) { return rsqrt_approx(fmaxf(f, 1.17549435e-38f)); });
+          a[t] = g.a;
+          u[t] = (pair_of<T>(rx(t)) * g.om) * m;
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < L; ++t) {
+          const Gates<false> g(rate, pair_of<T>(rr(t)));
+          a[t] = g.a;
+          u[t] = (g.om * g.inv()) * (each(pair_of<T>(ri(t)), sigmoid_approx) * pair_of<T>(rx(t)));
+        }
+      }
+      if (here < L) {
+#pragma unroll
+        for (int t = 0; t < L; ++t)
+          if (t >= here) a[t] = both(1.f), u[t] = both(0.f);
+      }
+      if (marks == 0) {
+#pragma unroll
+        for (int t = 0; t < L; ++t) {
+          own.P = own.P * a[t];
+          own.q = fma(a[t], own.q, u[t]);
+        }
+      } else {
+#pragma unroll
+        for (int t = 0; t < L; ++t) {
+          const bool cut = marks >> t & 1;
+          own.P = own.P * a[t];
+          own.q = fma(a[t], own.q, u[t]);
+          if (cut) own = {both(__uint_as_float(kFresh)), u[t]};
+        }
+      }
+    }
+    auto& run = sh.run[s][0];
+    run[w][lane] = own;
     __syncthreads();
-  }
-  if (fold) {
-    float s = k == 0 ? first_state() : fold_seen(sh, k, j);
-    const float out = pass(tp, tq, s);
-    if (!last) store_word(p.states + (tile + k) * kStrip + j, word(out));
-    if (last && p.fin && cj < p.channels) p.fin[(int64_t)b * p.channels + cj] = out;
-    for (int v = 0; v < nw; ++v) {
-      sh.in[v][j] = s;
-      const int t = k * kTile + v * kRun;
-      if (p.pieces && t % kPiece == 0 && t < p.seqlen && cj < p.channels)
-        p.pieces[((int64_t)b * p.npieces + t / kPiece) * p.channels + cj] = s;
-      s = pass(sh.P[v][j], sh.q[v][j], s);
-    }
-  }
-  __syncthreads();
 
-  float h0 = sh.in[w][ln.j0], h1 = sh.in[w][ln.j1];
-  T* y = static_cast<T*>(p.y) + b * p.ys[0] + (int64_t)t0 * p.ys[1] + ln.c;
+    // (the tile's inputs have been read)
+    if (threadIdx.x == 32 * (kRuns - 1)) send_for<T, TMA, 3, kTile>(p, maps, &sh.ticket[s], &sh.full[s], turn + 2, stage, false);
+    const bool last = k == p.tiles - 1;
+    Share tile = {};
+    if (w == 0) {
+      tile = whole(run, false);
+      if (k > 0 && !last) publish(p, first + k, tile);
+    }
+    Pair h = both(0.f);
+    if (k > 0) {
+      look_back(p, sh, first, k);
+      __syncthreads();
+      h = fold_seen(sh, k);
+    } else if (p.init) {
+      h = ln.get(p.init + (int64_t)b * p.channels);
+    }
+    if (w == 0) {
+      const Pair out = pass(tile, h);
+      if (!last) publish(p, first + k, out);
+      else if (p.fin) ln.put(p.fin + (int64_t)b * p.channels, out);
+    }
+    h = through(h, w, [&](int v) { return run[v][lane]; });
+    if (here <= 0) continue;
+    if (p.pieces && t0 % kPiece == 0) ln.put(p.pieces + ((int64_t)b * p.npieces + t0 / kPiece) * p.channels, h);
+
+    T* y = static_cast<T*>(p.y) + b * p.ys[0] + (int64_t)t0 * p.ys[1] + ln.c;
+    if (marks == 0 && here == L) {
 #pragma unroll
-  for (int t = 0; t < kRun; ++t) {
-    const bool cut = marks >> t & 1;
-    h0 = cut ? u[t][0] : fmaf(a[t][0], h0, u[t][0]);
-    h1 = cut ? u[t][1] : fmaf(a[t][1], h1, u[t][1]);
-    store_two<T, VEC>(y + t * p.ys[1], ln.apart, t < here && ln.ok0, t < here && ln.ok1, h0, h1);
+      for (int t = 0; t < L; ++t, y += p.ys[1]) {
+        h = fma(a[t], h, u[t]);
+        ln.template store<T, TMA>(y, h);
+      }
+    } else {
+#pragma unroll
+      for (int t = 0; t < L; ++t, y += p.ys[1]) {
+        h = fma(a[t], h, u[t]);
+        if (marks >> t & 1) h = u[t];
+        if (t < here) ln.template store<T, TMA>(y, h);
+      }
+    }
   }
 }
 
 // The gradient: the same walk from the last tile to the first, what passes from a token to the one before it being a[t] g[t].
-template <typename T, bool VEC>
-__global__ void __launch_bounds__(32 * kRuns, 1) gated_scan_grad_kernel(const Scan p) {
+// With w = b si, u = w x and m = a^2 / (1 - a^2):  dx = g w,  di = g u (1 - si),  dla = g (a h[t-1] - m u)  (without its first term at a
+// reset),  dr = dla la (1 - sr),  and what decay's gradient sums up is dla la.
+template <typename T, bool TMA>
+__global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
   using Raw = typename Two<T>::Raw;
-  constexpr int L = kRunGrad;
-  __shared__ Shared sh;
-  __shared__ float qb[kRuns][kStrip], back[kRuns][kStrip];   // pairs and entering numbers of the way back
-  const int2 which = take_tile(p, sh);
-  const int kb = which.x, k = p.tiles - 1 - kb, strip = which.y % p.strips, b = which.y / p.strips;
-  const int w = threadIdx.x / 32, nw = blockDim.x / 32;
-  const int t0 = k * kTileGrad + w * L;
-  const int here = min(L, p.seqlen - t0);
-  const Lane<T, VEC> ln(strip, p.channels);
-  const int64_t tile = (int64_t)which.y * p.tiles;
-
-  Raw rx[L], ri[L], rr[L], rd[L];
-  {
-    const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + (int64_t)t0 * p.xs[1] + ln.c;
-    const T* i = static_cast<const T*>(p.i) + b * p.is[0] + (int64_t)t0 * p.is[1] + ln.c;
-    const T* r = static_cast<const T*>(p.r) + b * p.rs[0] + (int64_t)t0 * p.rs[1] + ln.c;
-    const T* d = static_cast<const T*>(p.dy) + b * p.dys[0] + (int64_t)t0 * p.dys[1] + ln.c;
-#pragma unroll
-    for (int t = 0; t < L; ++t) {
-      const bool there = t < here;
-      rr[t] = load_two<T, VEC>(r + t * p.rs[1], ln.apart, there && ln.ok0, there && ln.ok1);
-      ri[t] = load_two<T, VEC>(i + t * p.is[1], ln.apart, there && ln.ok0, there && ln.ok1);
-      rx[t] = load_two<T, VEC>(x + t * p.xs[1], ln.apart, there && ln.ok0, there && ln.ok1);
-      rd[t] = load_two<T, VEC>(d + t * p.dys[1], ln.apart, there && ln.ok0, there && ln.ok1);
-    }
-  }
-  unsigned marks = 0;
-  if (p.reset) {
-    const unsigned char* m = p.reset + b * p.ms[0] + (int64_t)t0 * p.ms[1];
-#pragma unroll
-    for (int t = 0; t < L; ++t)
-      if (t < here && m[t * p.ms[1]]) marks |= 1u << t;
-  }
-  const int j = threadIdx.x, cj = strip * kStrip + j;
-  const bool fold = j < kStrip;
-  float s = 0.f;   // state entering the tile
-  if (fold && cj < p.channels) s = p.pieces[((int64_t)b * p.npieces + k) * p.channels + cj];
-  const float k0 = ln.ok0 ? decay_rate(p.rate, p.decay[ln.c]) : 0.f;
-  const float k1 = ln.ok1 ? decay_rate(p.rate, p.decay[ln.c + ln.apart]) : 0.f;
-  const float fresh = __uint_as_float(kFresh);
-
-  float a[L][2], u[L][2];
-  float P[2] = {1.f, 1.f}, q[2] = {0.f, 0.f}, c[2] = {0.f, 0.f};
-#pragma unroll
-  for (int t = 0; t < L; ++t) {
-    const float2 xv = Two<T>::up(rx[t]), iv = Two<T>::up(ri[t]), rv = Two<T>::up(rr[t]);
-    const Gates g0(k0, rv.x), g1(k1, rv.y);
-    a[t][0] = g0.a; a[t][1] = g1.a;
-    u[t][0] = (g0.om * g0.inv()) * (sigmoid_approx(iv.x) * xv.x);
-    u[t][1] = (g1.om * g1.inv()) * (sigmoid_approx(iv.y) * xv.y);
-    if (t >= here) a[t][0] = a[t][1] = 1.f, u[t][0] = u[t][1] = 0.f;
-    const bool cut = marks >> t & 1;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      P[e] = cut ? fresh : P[e] * a[t][e];
-      q[e] = cut ? u[t][e] : fmaf(a[t][e], q[e], u[t][e]);
-    }
-  }
-#pragma unroll
-  for (int t = L - 1; t >= 0; --t) {
-    const float2 dv = Two<T>::up(rd[t]);
-    const bool cut = marks >> t & 1;
-    c[0] = cut ? 0.f : a[t][0] * (dv.x + c[0]);
-    c[1] = cut ? 0.f : a[t][1] * (dv.y + c[1]);
-  }
-  sh.P[w][ln.j0] = P[0]; sh.P[w][ln.j1] = P[1];
-  sh.q[w][ln.j0] = q[0]; sh.q[w][ln.j1] = q[1];
-  qb[w][ln.j0] = c[0]; qb[w][ln.j1] = c[1];
-  __syncthreads();
-
-  const bool last = kb == p.tiles - 1;   // of the way back: the sequence's first
-  float tp = 1.f, tq = 0.f;
-  if (fold) {
-    for (int v = nw - 1; v >= 0; --v) {
-      tq = pass(sh.P[v][j], qb[v][j], tq);
-      tp = __float_as_uint(sh.P[v][j]) == kFresh ? fresh : tp * sh.P[v][j];
-    }
-    if (kb > 0 && !last) publish_pair(p, tile + kb, j, tp, tq);
-    for (int v = 0; v < nw; ++v) {
-      sh.in[v][j] = s;
-      s = pass(sh.P[v][j], sh.q[v][j], s);
-    }
-  }
-  if (kb > 0) {
-    look_back(p, sh, tile, kb, ln.j0, ln.j1);
-    __syncthreads();
-  }
-  if (fold) {
-    float g = 0.f;
-    if (kb > 0) g = fold_seen(sh, kb, j);
-    else if (p.dfinal && cj < p.channels) g = p.dfinal[(int64_t)b * p.channels + cj];
-    const float out = pass(tp, tq, g);
-    if (!last) store_word(p.states + (tile + kb) * kStrip + j, word(out));
-    if (last && p.dinit && cj < p.channels) p.dinit[(int64_t)b * p.channels + cj] = out;
-    for (int v = nw - 1; v >= 0; --v) {
-      back[v][j] = g;
-      g = pass(sh.P[v][j], qb[v][j], g);
-    }
+  constexpr int L = kRunGrad, kStage = (int)stage_numbers(4, kTileGrad);
+  extern __shared__ __align__(128) unsigned char smem[];
+  T* const stages = reinterpret_cast<T*>(smem);
+  Shared<2>& sh = *reinterpret_cast<Shared<2>*>(smem + 2 * kStage * sizeof(T));
+  __shared__ Pair sums[2][kRuns][32];
+  const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
+  const unsigned units = (unsigned)p.strips * p.batch;
+  if (threadIdx.x == 0) {
+    sh.dead = 0;
+    ptx::mbar_init(&sh.full[0], 1);
+    ptx::mbar_init(&sh.full[1], 1);
+    ptx::fence_mbar_init();
+    for (int s = 0; s < 2; ++s) send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.ticket[s], &sh.full[s], s, stages + s * kStage, true);
   }
   __syncthreads();
 
-  float h[2] = {sh.in[w][ln.j0], sh.in[w][ln.j1]};
+  unsigned turn = 0;
+  float* part = nullptr;   // where the sums of the tile before belong
+  auto leave_sums = [&](int s) {   // (behind a barrier)
+    if (part && w == 0) {
+      Pair v = sums[s][0][lane];
 #pragma unroll
-  for (int t = 0; t < L; ++t) {   // u[t] becomes the state before t
-    const bool cut = marks >> t & 1;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const float before = h[e];
-      h[e] = cut ? u[t][e] : fmaf(a[t][e], before, u[t][e]);
-      u[t][e] = before;
+      for (int n = 1; n < kRuns; ++n) v = v + sums[s][n][lane];
+      *reinterpret_cast<float2*>(part) = halves(v);
     }
-  }
-  c[0] = back[w][ln.j0];
-  c[1] = back[w][ln.j1];
-  float dd[2] = {0.f, 0.f};
-  T* dx = static_cast<T*>(p.dx) + b * p.dxs[0] + (int64_t)t0 * p.dxs[1] + ln.c;
-  T* di = static_cast<T*>(p.di) + b * p.dis[0] + (int64_t)t0 * p.dis[1] + ln.c;
-  T* dr = static_cast<T*>(p.dr) + b * p.drs[0] + (int64_t)t0 * p.drs[1] + ln.c;
+  };
+  for (;; ++turn) {
+    const int s = turn & 1;
+    T* const stage = stages + s * kStage;
+    wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
+    const unsigned ticket = sh.ticket[s];
+    if (ticket >= p.total) break;
+    const int kb = (int)(ticket / units), k = p.tiles - 1 - kb, unit = (int)(ticket % units), strip = unit % p.strips, b = unit / p.strips;
+    const int t0 = k * kTileGrad + w * L;
+    const int here = min(L, p.seqlen - t0);
+    const Lane ln(strip, p.channels);
+    const int64_t first = (int64_t)unit * p.tiles;
+    if constexpr (!TMA) {
+      const int c = strip * kStrip, n = kTileGrad * kStrip;
+      fill<T, kTileGrad>(stage, p.x, b, k * kTileGrad, p.seqlen, p.xs, c, p.channels);
+      fill<T, kTileGrad>(stage + n, p.i, b, k * kTileGrad, p.seqlen, p.is, c, p.channels);
+      fill<T, kTileGrad>(stage + 2 * n, p.r, b, k * kTileGrad, p.seqlen, p.rs, c, p.channels);
+      fill<T, kTileGrad>(stage + 3 * n, p.dy, b, k * kTileGrad, p.seqlen, p.dys, c, p.channels);
+      __syncthreads();
+    }
+    const Raw* const raw = reinterpret_cast<const Raw*>(stage + w * L * kStrip) + lane;
+    constexpr int kNext = kTileGrad * 32;
+    auto x = [&](int t) { return pair_of<T>(raw[t * 32]); };
+    auto ri = [&](int t) { return pair_of<T>(raw[t * 32 + kNext]); };
+    auto rr = [&](int t) { return pair_of<T>(raw[t * 32 + 2 * kNext]); };
+    auto dy = [&](int t) { return pair_of<T>(raw[t * 32 + 3 * kNext]); };
+    const unsigned marks = marks_of<L>(p, b, t0, here);
+    Pair h = ln.get(p.pieces + ((int64_t)b * p.npieces + k) * p.channels);   // the state entering the tile
+    const Pair rate = ln.rates(p), minus = both(-1.f), one = both(1.f);
+
+    Pair a[L], sr[L], si[L], wt[L], m[L];
+    Share own = {both(1.f), both(0.f)};
+    Pair c = both(0.f);
+    if (here > 0) {
+      auto gates = [&](auto mild) {
 #pragma unroll
-  for (int t = L - 1; t >= 0; --t) {
-    const float2 xv = Two<T>::up(rx[t]), iv = Two<T>::up(ri[t]), rv = Two<T>::up(rr[t]), dv = Two<T>::up(rd[t]);
-    const bool cut = marks >> t & 1;
-    float ox[2], oi[2], orr[2];
+        for (int t = 0; t < L; ++t) {
+          const Gates<decltype(mild)::value> g(rate, rr(t));
+          const Pair inv = g.inv();
+          a[t] = g.a;
+          sr[t] = g.sr;
+          si[t] = each(ri(t), sigmoid_approx);
+          wt[t] = (g.om * inv) * si[t];
+          const Pair ai = g.a * inv;
+          m[t] = ai * ai;
+        }
+      };
+      const float2 kk = halves(rate);
+      if (__all_sync(~0u, kk.x < kMild && kk.y < kMild)) gates(std::true_type());
+      else gates(std::false_type());
+      if (here < L) {
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const Gates gt(e ? k1 : k0, e ? rv.y : rv.x);
-      const float xe = e ? xv.y : xv.x;
-      const float si = sigmoid_approx(e ? iv.y : iv.x), inv = gt.inv(), beta = gt.om * inv;
-      const float g = (e ? dv.y : dv.x) + c[e];
-      const float gs = g * si, gb = gs * beta;
-      ox[e] = gb;
-      oi[e] = gb * xe * (1.f - si);
-      const float through = cut ? 0.f : g * u[t][e] * gt.a;         // what a's share of h brings
-      const float root = gs * xe, steep = gt.a * gt.a * inv;        // and b's: -root * steep
-      orr[e] = (1.f - gt.sr) * (through * gt.la - root * (steep * gt.la));
-      if (t < here) {
-        dd[e] += through * gt.sr - root * (steep * gt.sr);
-        c[e] = cut ? 0.f : gt.a * g;
+        for (int t = 0; t < L; ++t)
+          if (t >= here) a[t] = one, sr[t] = si[t] = wt[t] = m[t] = both(0.f);
+      }
+#pragma unroll
+      for (int t = 0; t < L; ++t) {
+        const Pair u = wt[t] * x(t);
+        own.P = own.P * a[t];
+        own.q = fma(a[t], own.q, u);
+        if (marks >> t & 1) own = {both(__uint_as_float(kFresh)), u};
+      }
+#pragma unroll
+      for (int t = L - 1; t >= 0; --t) {
+        c = a[t] * (dy(t) + c);
+        if (marks >> t & 1) c = both(0.f);
       }
     }
-    const bool ok0 = t < here && ln.ok0, ok1 = t < here && ln.ok1;
-    store_two<T, VEC>(dx + t * p.dxs[1], ln.apart, ok0, ok1, ox[0], ox[1]);
-    store_two<T, VEC>(di + t * p.dis[1], ln.apart, ok0, ok1, oi[0], oi[1]);
-    store_two<T, VEC>(dr + t * p.drs[1], ln.apart, ok0, ok1, orr[0], orr[1]);
+    auto &run = sh.run[s][0], &back = sh.run[s][1];
+    run[w][lane] = own;
+    back[w][lane] = {own.P, c};
+    __syncthreads();
+
+    // (the inputs of the tile before have been read)
+    if (turn > 0 && threadIdx.x == 32 * (kRuns - 1))
+      send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.ticket[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true);
+    leave_sums(s ^ 1);
+    part = p.part + ((int64_t)b * p.tiles + k) * ((int64_t)p.strips * kStrip) + ln.c;
+    const bool last = kb == p.tiles - 1;   // of the way back: the sequence's first
+    Share tile = {};
+    if (w == 0) {
+      tile = whole(back, true);
+      if (kb > 0 && !last) publish(p, first + kb, tile);
+    }
+    c = both(0.f);
+    if (kb > 0) {
+      look_back(p, sh, first, kb);
+      __syncthreads();
+      c = fold_seen(sh, kb);
+    } else if (p.dfinal) {
+      c = ln.get(p.dfinal + (int64_t)b * p.channels);
+    }
+    if (w == 0) {
+      const Pair out = pass(tile, c);
+      if (!last) publish(p, first + kb, out);
+      else if (p.dinit) ln.put(p.dinit + (int64_t)b * p.channels, out);
+    }
+    h = through(h, w, [&](int v) { return run[v][lane]; });
+    c = through(c, kRuns - 1 - w, [&](int v) { return back[kRuns - 1 - v][lane]; });
+
+    Pair sum = both(0.f);
+    if (here > 0) {
+#pragma unroll
+      for (int t = 0; t < L; ++t) {   // m becomes a h[t-1] - m u
+        const Pair u = wt[t] * x(t);
+        Pair before = a[t] * h;
+        if (marks >> t & 1) before = both(0.f);
+        h = before + u;
+        m[t] = fma(m[t] * minus, u, before);
+      }
+      T* dx = static_cast<T*>(p.dx) + b * p.dxs[0] + (int64_t)(t0 + L - 1) * p.dxs[1] + ln.c;
+      T* di = static_cast<T*>(p.di) + b * p.dis[0] + (int64_t)(t0 + L - 1) * p.dis[1] + ln.c;
+      T* dr = static_cast<T*>(p.dr) + b * p.drs[0] + (int64_t)(t0 + L - 1) * p.drs[1] + ln.c;
+#pragma unroll
+      for (int t = L - 1; t >= 0; --t, dx -= p.dxs[1], di -= p.dis[1], dr -= p.drs[1]) {
+        const Pair g = dy(t) + c;
+        const Pair dv = (g * m[t]) * (rate * sr[t]);   // -dla la
+        const Pair gw = g * wt[t];
+        sum = sum + dv;
+        c = a[t] * g;
+        if (marks >> t & 1) c = both(0.f);
+        if (t < here) {
+          ln.template store<T, TMA>(dx, gw);
+          ln.template store<T, TMA>(di, (gw * x(t)) * fma(si[t], minus, one));
+          ln.template store<T, TMA>(dr, dv * fma(sr[t], one, minus));
+        }
+      }
+    }
+    sums[s][w][lane] = sum;
   }
-  sh.q[w][ln.j0] = dd[0];
-  sh.q[w][ln.j1] = dd[1];
   __syncthreads();
-  if (fold && cj < p.channels) {
-    float sum = 0.f;
-    for (int v = 0; v < nw; ++v) sum += sh.q[v][j];
-    p.part[((int64_t)b * p.tiles + k) * p.channels + cj] = sum;
-  }
+  leave_sums((turn - 1) & 1);
 }
 
+// From the sum of -dla la: la is -rate softplus(decay) sr, so d la / d decay is la sigmoid(decay) / softplus(decay), a ratio that goes
+// to 1 where both vanish.
 struct FinishDecay {
   const float* decay;
   float* out;
-  float rate;
-  __device__ __forceinline__ void operator()(int c, float v) const { out[c] = v * (-rate / (1.f + expf(-decay[c]))); }
+  __device__ __forceinline__ void operator()(int c, float v) const {
+    const float plus = decay_rate(1.f, decay[c]);
+    out[c] = plus < 1e-30f ? -v : -v * (1.f / (1.f + expf(-decay[c])) / plus);
+  }
 };
 
 // One token.  V channels per thread.
@@ -465,11 +653,22 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const T* __restrict__ x
   copy(rv, r + b * rs + c);
   copy(sv, state + (int64_t)b * channels + c);
   copy(dv, decay + c);
+  if constexpr (V == 1) {   // (as one of two)
+    const Gates<false> g(both(decay_rate(rate, dv[0])), both(Cvt<T>::to_f(rv[0])));
+    const Pair u = (g.om * g.inv()) * both(sigmoid_approx(Cvt<T>::to_f(iv[0])) * Cvt<T>::to_f(xv[0]));
+    sv[0] = halves(fma(g.a, both(sv[0]), u)).x;
+    yv[0] = Cvt<T>::from_f(sv[0]);
+  } else {
 #pragma unroll
-  for (int e = 0; e < V; ++e) {
-    const Gates g(decay_rate(rate, dv[e]), Cvt<T>::to_f(rv[e]));
-    sv[e] = fmaf(g.a, sv[e], (g.om * g.inv()) * (sigmoid_approx(Cvt<T>::to_f(iv[e])) * Cvt<T>::to_f(xv[e])));
-    yv[e] = Cvt<T>::from_f(sv[e]);
+    for (int e = 0; e < V; e += 2) {
+      const Gates<false> g(pair(decay_rate(rate, dv[e]), decay_rate(rate, dv[e + 1])), pair(Cvt<T>::to_f(rv[e]), Cvt<T>::to_f(rv[e + 1])));
+      const Pair x2 = pair(Cvt<T>::to_f(xv[e]), Cvt<T>::to_f(xv[e + 1])), i2 = pair(Cvt<T>::to_f(iv[e]), Cvt<T>::to_f(iv[e + 1]));
+      const float2 h = halves(fma(g.a, pair(sv[e], sv[e + 1]), (g.om * g.inv()) * (each(i2, sigmoid_approx) * x2)));
+      sv[e] = h.x;
+      sv[e + 1] = h.y;
+      yv[e] = Cvt<T>::from_f(h.x);
+      yv[e + 1] = Cvt<T>::from_f(h.y);
+    }
   }
   copy(state_out + (int64_t)b * channels + c, sv);
   copy(y + b * ys + c, yv);
@@ -487,7 +686,7 @@ Sizes sizes_of(const SsdGatedScanArgs& a, bool grad) {
   z.tiles = (a.seqlen + (int64_t)tile - 1) / tile;
   z.units = (int64_t)a.batch * strips_of(a.channels);
   z.words = z.tiles == 1 ? 0 : 256 + z.units * z.tiles * kStrip * 12;
-  z.part = grad ? (int64_t)a.batch * z.tiles * a.channels * 4 : 0;
+  z.part = grad ? z.units * z.tiles * kStrip * 4 : 0;
   return z;
 }
 
@@ -498,6 +697,20 @@ int check(const SsdGatedScanArgs* a, bool grad) {
   const Sizes z = sizes_of(*a, grad);
   if (a->seqlen > 0x7fffff00 || z.tiles * z.units > 0x7fffffff) return SSD_ERR_TOO_LARGE;
   return SSD_OK;
+}
+
+// [b,s,d] as TMA sees it, a box of 64 channels of `rows` tokens; what lies outside reads as zero.
+template <typename T>
+bool operand_map(CUtensorMap* map, const void* base, const SsdGatedScanArgs& a, const int64_t (&st)[2], int rows) {
+  const tc::EncodeFn encode = tc::encode_fn();
+  if (!encode) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)a.channels, (cuuint64_t)a.seqlen, (cuuint64_t)a.batch};
+  const cuuint64_t strides[2] = {(cuuint64_t)st[1] * sizeof(T), (cuuint64_t)st[0] * sizeof(T)};
+  const cuuint32_t box[3] = {kStrip, (cuuint32_t)rows, 1}, each[3] = {1, 1, 1};
+  const CUtensorMapDataType type = a.dtype == SSD_DTYPE_F32 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32
+                                   : a.dtype == SSD_DTYPE_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16;
+  return encode(map, type, 3, const_cast<void*>(base), dims, strides, box, each, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_NONE,
+                CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <typename T>
@@ -518,17 +731,19 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   if (z.words) {
     p.counter = reinterpret_cast<unsigned*>(ws);
     p.pairs = reinterpret_cast<unsigned long long*>(ws + 256);
-    p.states = reinterpret_cast<unsigned*>(ws + 256 + z.units * z.tiles * kStrip * 8);
+    p.states = reinterpret_cast<unsigned long long*>(ws + 256 + z.units * z.tiles * kStrip * 8);
     if (cudaMemsetAsync(ws, 0xff, (size_t)z.words, stream) != cudaSuccess) return SSD_ERR_CUDA;
   }
   p.part = reinterpret_cast<float*>(ws + up256(z.words));
-  bool pairs = a.channels % 2 == 0;   // two channels at once: every row starts on their boundary
+  // by TMA: every row starts on 16 bytes
+  bool tma = a.channels * sizeof(T) % 16 == 0;
   auto strides = [&](int64_t (&to)[2], const int64_t (&from)[2], const void* at) {
     for (int d = 0; d < 2; ++d) {
-      to[d] = from[d];
-      pairs = pairs && from[d] % 2 == 0;
+      to[d] = (d == 0 ? a.batch : a.seqlen) == 1 ? 16 : from[d];   // (the stride of a single one may be anything)
+      const int64_t bytes = to[d] * (int64_t)sizeof(T);
+      tma = tma && bytes % 16 == 0 && bytes > 0 && bytes < (int64_t)1 << 40;
     }
-    pairs = pairs && reinterpret_cast<uintptr_t>(at) % (2 * sizeof(T)) == 0;
+    tma = tma && reinterpret_cast<uintptr_t>(at) % 16 == 0;
   };
   strides(p.xs, a.x_stride, a.x);
   strides(p.is, a.input_gate_stride, a.input_gate);
@@ -542,13 +757,27 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   } else {
     strides(p.ys, a.y_stride, a.y);
   }
-  const unsigned grid = (unsigned)(z.tiles * z.units);
-  const int run = grad ? kRunGrad : kRun;
-  const int threads = z.tiles > 1 ? 32 * kRuns : 32 * std::max(2, (a.seqlen + run - 1) / run);   // (64 fold a strip)
-  if (!grad) return launch(pairs ? gated_scan_kernel<T, true> : gated_scan_kernel<T, false>, grid, threads, 0, stream, p);
-  if (const int rc = launch(pairs ? gated_scan_grad_kernel<T, true> : gated_scan_grad_kernel<T, false>, grid, threads, 0, stream, p))
-    return rc;
-  return launch_column_sum(p.part, a.batch * z.tiles, a.channels, a.channels, FinishDecay{a.decay, a.ddecay, a.rate}, stream);
+  p.total = (unsigned)(z.tiles * z.units);
+  Maps maps = {};
+  if (tma) {
+    const int tile = grad ? kTileGrad : kTile;
+    tma = operand_map<T>(&maps.at[0], a.x, a, p.xs, tile) && operand_map<T>(&maps.at[1], a.input_gate, a, p.is, tile) &&
+          operand_map<T>(&maps.at[2], a.decay_gate, a, p.rs, tile) &&
+          (!grad || operand_map<T>(&maps.at[3], a.dy, a, p.dys, tile));
+  }
+  // two CTAs an SM, one where tiles are of 32-bit numbers
+  const unsigned grid = std::min(p.total, 148u * (sizeof(T) == 2 ? 2 : 1));
+  auto go = [&](auto kernel, size_t smem) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)SSD_ERR_CUDA;
+    return launch(kernel, grid, kThreads, smem, stream, p, maps);
+  };
+  if (!grad) {
+    const size_t smem = 2 * stage_numbers(3, kTile) * sizeof(T) + sizeof(Shared<1>);
+    return tma ? go(gated_scan_kernel<T, true>, smem) : go(gated_scan_kernel<T, false>, smem);
+  }
+  const size_t smem = 2 * stage_numbers(4, kTileGrad) * sizeof(T) + sizeof(Shared<2>);
+  if (const int rc = tma ? go(gated_scan_grad_kernel<T, true>, smem) : go(gated_scan_grad_kernel<T, false>, smem)) return rc;
+  return launch_column_sum(p.part, a.batch * z.tiles, (int64_t)p.strips * kStrip, a.channels, FinishDecay{a.decay, a.ddecay}, stream);
 }
 
 template <typename T>

@@ -10,6 +10,42 @@
 
 namespace ssd {
 
+// Two fp32 numbers that one instruction works on.
+struct Pair {
+  unsigned long long v;
+};
+__device__ __forceinline__ Pair pair(float lo, float hi) {
+  Pair r;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(r.v) : "f"(lo), "f"(hi));
+  return r;
+}
+__device__ __forceinline__ Pair both(float v) { return pair(v, v); }
+__device__ __forceinline__ float2 halves(Pair p) {
+  float2 r;
+  asm("mov.b64 {%0, %1}, %2;" : "=f"(r.x), "=f"(r.y) : "l"(p.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator+(Pair a, Pair b) {
+  Pair r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair operator*(Pair a, Pair b) {
+  Pair r;
+  asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+__device__ __forceinline__ Pair fma(Pair a, Pair b, Pair c) {
+  Pair r;
+  asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(r.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+  return r;
+}
+template <typename F>
+__device__ __forceinline__ Pair each(Pair p, F f) {
+  const float2 h = halves(p);
+  return pair(f(h.x), f(h.y));
+}
+
 // Two numbers of type T as they lie in memory.
 template <typename T> struct Two;
 template <> struct Two<float> {
@@ -20,6 +56,7 @@ template <> struct Two<float> {
   static __device__ __forceinline__ Raw join(float a, float b) { return make_float2(a, b); }
   static __device__ __forceinline__ float lo(Raw v) { return v.x; }
   static __device__ __forceinline__ float hi(Raw v) { return v.y; }
+  static __device__ __forceinline__ Raw least(Raw a, Raw b) { return make_float2(fminf(a.x, b.x), fminf(a.y, b.y)); }
 };
 template <> struct Two<__half> {
   using Raw = uint32_t;
@@ -32,6 +69,10 @@ template <> struct Two<__half> {
   static __device__ __forceinline__ Raw join(__half a, __half b) { return (uint32_t)__half_as_ushort(a) | (uint32_t)__half_as_ushort(b) << 16; }
   static __device__ __forceinline__ __half lo(Raw v) { return __ushort_as_half((unsigned short)v); }
   static __device__ __forceinline__ __half hi(Raw v) { return __ushort_as_half((unsigned short)(v >> 16)); }
+  static __device__ __forceinline__ Raw least(Raw a, Raw b) {
+    const __half2 h = __hmin2(*reinterpret_cast<const __half2*>(&a), *reinterpret_cast<const __half2*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 template <> struct Two<__nv_bfloat16> {
   using Raw = uint32_t;
@@ -46,22 +87,34 @@ template <> struct Two<__nv_bfloat16> {
   }
   static __device__ __forceinline__ __nv_bfloat16 lo(Raw v) { return __ushort_as_bfloat16((unsigned short)v); }
   static __device__ __forceinline__ __nv_bfloat16 hi(Raw v) { return __ushort_as_bfloat16((unsigned short)(v >> 16)); }
+  static __device__ __forceinline__ Raw least(Raw a, Raw b) {
+    const __nv_bfloat162 h = __hmin2(*reinterpret_cast<const __nv_bfloat162*>(&a), *reinterpret_cast<const __nv_bfloat162*>(&b));
+    return *reinterpret_cast<const uint32_t*>(&h);
+  }
 };
 
+template <typename T>
+__device__ __forceinline__ Pair pair_of(typename Two<T>::Raw v) {
+  const float2 f = Two<T>::up(v);
+  return pair(f.x, f.y);
+}
+
 // A lane's two channels: neighbours read at once (VEC), or `apart` elements from each other and each only if it is there.
+// What is not there reads as `missing`.
 template <typename T, bool VEC>
-__device__ __forceinline__ typename Two<T>::Raw load_two(const T* p, int apart, bool ok0, bool ok1) {
+__device__ __forceinline__ typename Two<T>::Raw load_two(const T* p, int apart, bool ok0, bool ok1, float missing = 0.f) {
   if constexpr (VEC) {
-    return ok0 ? *reinterpret_cast<const typename Two<T>::Raw*>(p) : Two<T>::zero();
+    return ok0 ? *reinterpret_cast<const typename Two<T>::Raw*>(p) : Two<T>::down(missing, missing);
   } else {
-    const T z = Cvt<T>::from_f(0.f);
+    const T z = Cvt<T>::from_f(missing);
     const T a = ok0 ? p[0] : z, b = ok1 ? p[apart] : z;
     return Two<T>::join(a, b);
   }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void store_two(T* p, int apart, bool ok0, bool ok1, float a, float b) {
-  const typename Two<T>::Raw v = Two<T>::down(a, b);
+__device__ __forceinline__ void store_two(T* p, int apart, bool ok0, bool ok1, Pair f) {
+  const float2 h = halves(f);
+  const typename Two<T>::Raw v = Two<T>::down(h.x, h.y);
   if constexpr (VEC) {
     if (ok0) *reinterpret_cast<typename Two<T>::Raw*>(p) = v;
   } else {
