@@ -26,7 +26,7 @@
 namespace ssd {
 namespace {
 
-constexpr int kRuns = 8, kThreads = 32 * kRuns, kStrip = 64, kPiece = 64, kLook = 2 * kRuns;
+constexpr int kRuns = 8, kThreads = 32 * kRuns, kStrip = 64, kPiece = 64, kLook = kRuns;
 constexpr int kRun = 16, kRunGrad = 8;
 constexpr int kTile = kRun * kRuns, kTileGrad = kRunGrad * kRuns;
 static_assert(kTile % kPiece == 0 && kPiece % kRun == 0 && kTileGrad == kPiece, "pieces start at runs");
@@ -35,6 +35,7 @@ struct Scan {
   const void *x, *i, *r, *dy;
   void *y, *dx, *di, *dr;
   const float *decay, *init, *dfinal;
+  const float* rates;            // rate * softplus(decay) of every channel, where prepare_kernel has left them
   const unsigned char* reset;
   float *fin, *pieces, *part, *dinit;
   unsigned* counter;             // scratch, all bits set at launch: counter, pairs [tile][64], states [tile][64]
@@ -86,12 +87,13 @@ __device__ __forceinline__ float decay_rate(float rate, float decay) {
 // up.  Beyond 1/2 a state is gone before errors add up.  1 - a^2 = q (1 + a) loses nothing in either case.
 // MILD: v stays below 1/2 however far the gate opens (rate * softplus(decay) does), as it does where layers are initialised.
 constexpr float kMild = 0.5f;
+__device__ __forceinline__ Pair sigmoid(Pair v) { return each(each(v * both(-kLog2E), exp2_approx) + both(1.f), rcp_approx); }
 template <bool MILD>
 struct Gates {
   Pair sr, v, a, om;
   __device__ __forceinline__ Gates(Pair k, Pair r) {
     const Pair one = both(1.f);
-    sr = each(each(r * both(-kLog2E), exp2_approx) + one, rcp_approx);
+    sr = sigmoid(r);
     v = k * sr;
     Pair p = fma(both(-0.001121634905f), v, both(0.008187385975f));
     p = fma(p, v, both(-0.04162908913f));
@@ -143,7 +145,7 @@ template <int SIDES>
 struct Shared {
   Share run[2][SIDES][kRuns][32];   // of the runs, tiles in turn; the gradient's other side is that of the way back
   Share seen[kLook][32];            // of the tiles before this one, the nearest first
-  unsigned ticket[2];
+  int4 which[2];                    // place in its sequence (-1: there is no tile left), unit, strip, batch entry
   int dead;                         // a wait ran out: no further one
   alignas(8) uint64_t full[2];
 };
@@ -154,21 +156,26 @@ struct Maps {
 
 // Takes the next tile's number and sends for its inputs (one thread).
 template <typename T, bool TMA, int N, int TILE>
-__device__ __forceinline__ void send_for(const Scan& p, const Maps& maps, unsigned* ticket, uint64_t* full, unsigned turn, T* stage, bool backwards) {
+__device__ __forceinline__ void send_for(const Scan& p, const Maps& maps, int4* which, uint64_t* full, unsigned turn, T* stage, bool backwards) {
   const unsigned t = p.tiles == 1 ? blockIdx.x + turn * gridDim.x : atomicAdd(p.counter, 1u) + 1u;
-  *ticket = t;
-  if (!TMA || t >= p.total) {
+  if (t >= p.total) {
+    which->x = -1;
+    ptx::mbar_arrive(full);
+    return;
+  }
+  const unsigned units = (unsigned)p.strips * p.batch;
+  const int place = (int)(t / units), unit = (int)(t % units), strip = unit % p.strips, b = unit / p.strips;
+  *which = make_int4(place, unit, strip, b);
+  if (!TMA) {
     ptx::mbar_arrive(full);
     return;
   }
   ptx::mbar_expect_tx(full, N * TILE * kStrip * sizeof(T));
-  const unsigned units = (unsigned)p.strips * p.batch;
-  const int u = (int)(t % units), k = backwards ? p.tiles - 1 - (int)(t / units) : (int)(t / units);
 #pragma unroll
   for (int n = 0; n < N; ++n)
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
                      ptx::smem_u32(stage + n * TILE * kStrip)),
-                 "l"(&maps.at[n]), "r"(ptx::smem_u32(full)), "r"(u % p.strips * kStrip), "r"(k * TILE), "r"(u / p.strips)
+                 "l"(&maps.at[n]), "r"(ptx::smem_u32(full)), "r"(strip * kStrip), "r"((backwards ? p.tiles - 1 - place : place) * TILE), "r"(b)
                  : "memory");
 }
 
@@ -239,40 +246,37 @@ __device__ __forceinline__ void publish(const Scan& p, int64_t tile, Pair s) {
   store_word(p.states + tile * (kStrip / 2) + threadIdx.x % 32, two_words(word(h.x), word(h.y)));
 }
 
-// What stands before tile `k` of the unit, into sh.seen: warp w looks at tiles k - 1 - w and k - 1 - kRuns - w, for their states or else
-// their pairs; the farthest one waits for the state, so that one look is enough.
+// What stands before tile `k` of the unit, into sh.seen: warp w looks at tile k - 1 - w, for its state or else its pair; the farthest
+// one waits for the state, so that one look is enough.
 template <int SIDES>
 __device__ __forceinline__ void look_back(const Scan& p, Shared<SIDES>& sh, int64_t first, int k) {
-  const int lane = threadIdx.x % 32;
-#pragma unroll
-  for (int w = threadIdx.x / 32; w < kLook; w += kRuns) {
-    if (w >= k) return;
-    const int64_t tile = first + k - 1 - w;
-    const unsigned long long *at = p.pairs + tile * kStrip + 2 * lane, *state = p.states + tile * (kStrip / 2) + lane;
-    unsigned long long s, p0 = ~0ull, p1 = ~0ull;
-    const long long t0 = clock64();
-    bool have;
-    while (true) {
-      s = load_word(state);
-      if (w != kLook - 1) {
-        p0 = load_word(at);
-        p1 = load_word(at + 1);
-      }
-      have = (unsigned)s != kNone && (unsigned)(s >> 32) != kNone;
-      if (have || ((unsigned)p0 != kNone && (unsigned)p1 != kNone)) break;
-      if (*(volatile int*)&sh.dead) break;
-      if (clock64() - t0 > p.wait_clocks) {
-        *(volatile int*)&sh.dead = 1;
-        if (p.status) *p.status = STATUS_WAIT_TIMEOUT_LOOK_BACK;
-        break;
-      }
-      __nanosleep(20);
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+  if (w >= k) return;
+  const int64_t tile = first + k - 1 - w;
+  const unsigned long long *at = p.pairs + tile * kStrip + 2 * lane, *state = p.states + tile * (kStrip / 2) + lane;
+  unsigned long long s, p0 = ~0ull, p1 = ~0ull;
+  auto there = [](unsigned long long v) { return (unsigned)v != kNone && (unsigned)(v >> 32) != kNone; };
+  long long t0 = 0;
+  while (true) {
+    s = load_word(state);
+    if (w != kLook - 1) {
+      p0 = load_word(at);
+      p1 = load_word(at + 1);
     }
-    auto lo = [](unsigned long long v) { return __uint_as_float((unsigned)v); };
-    auto hi = [](unsigned long long v) { return __uint_as_float((unsigned)(v >> 32)); };
-    const float fresh = __uint_as_float(kFresh);
-    sh.seen[w][lane] = have ? Share{both(fresh), pair(lo(s), hi(s))} : Share{pair(lo(p0), lo(p1)), pair(hi(p0), hi(p1))};
+    if (there(s) || ((unsigned)p0 != kNone && (unsigned)p1 != kNone)) break;
+    if (*(volatile int*)&sh.dead) break;
+    if (t0 == 0) t0 = clock64();
+    if (clock64() - t0 > p.wait_clocks) {
+      *(volatile int*)&sh.dead = 1;
+      if (p.status) *p.status = STATUS_WAIT_TIMEOUT_LOOK_BACK;
+      break;
+    }
+    __nanosleep(20);
   }
+  auto lo = [](unsigned long long v) { return __uint_as_float((unsigned)v); };
+  auto hi = [](unsigned long long v) { return __uint_as_float((unsigned)(v >> 32)); };
+  const float fresh = __uint_as_float(kFresh);
+  sh.seen[w][lane] = there(s) ? Share{both(fresh), pair(lo(s), hi(s))} : Share{pair(lo(p0), lo(p1)), pair(hi(p0), hi(p1))};
 }
 
 // The state entering a tile from what look_back() saw: from the nearest place that nothing before it matters to.
@@ -302,6 +306,10 @@ struct Lane {
     if (ok1) row[c + 1] = h.y;
   }
   __device__ __forceinline__ Pair rates(const Scan& p) const {
+    if (p.rates) {
+      const float2 f = *reinterpret_cast<const float2*>(p.rates + c);
+      return pair(f.x, f.y);
+    }
     return pair(ok0 ? decay_rate(p.rate, p.decay[c]) : 0.f, ok1 ? decay_rate(p.rate, p.decay[c + 1]) : 0.f);
   }
   // two channels of an output's row, at once where the row starts on their boundary
@@ -327,13 +335,13 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_co
   T* const stages = reinterpret_cast<T*>(smem);
   Shared<1>& sh = *reinterpret_cast<Shared<1>*>(smem + 2 * kStage * sizeof(T));
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const unsigned units = (unsigned)p.strips * p.batch;
   if (threadIdx.x == 0) {
     sh.dead = 0;
     ptx::mbar_init(&sh.full[0], 1);
     ptx::mbar_init(&sh.full[1], 1);
     ptx::fence_mbar_init();
-    for (int s = 0; s < 2; ++s) send_for<T, TMA, 3, kTile>(p, maps, &sh.ticket[s], &sh.full[s], s, stages + s * kStage, false);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words)
+    for (int s = 0; s < 2; ++s) send_for<T, TMA, 3, kTile>(p, maps, &sh.which[s], &sh.full[s], s, stages + s * kStage, false);
   }
   __syncthreads();
 
@@ -341,9 +349,9 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_co
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
-    const unsigned ticket = sh.ticket[s];
-    if (ticket >= p.total) break;
-    const int k = (int)(ticket / units), unit = (int)(ticket % units), strip = unit % p.strips, b = unit / p.strips;
+    const int4 which = sh.which[s];
+    if (which.x < 0) break;
+    const int k = which.x, unit = which.y, strip = which.z, b = which.w;
     const int t0 = k * kTile + w * L;
     const int here = min(L, p.seqlen - t0);   // tokens of this run that are there
     const Lane ln(strip, p.channels);
@@ -384,7 +392,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_co
         for (int t = 0; t < L; ++t) {
           const Gates<false> g(rate, pair_of<T>(rr(t)));
           a[t] = g.a;
-          u[t] = (g.om * g.inv()) * (each(pair_of<T>(ri(t)), sigmoid_approx) * pair_of<T>(rx(t)));
+          u[t] = (g.om * g.inv()) * (sigmoid(pair_of<T>(ri(t))) * pair_of<T>(rx(t)));
         }
       }
       if (here < L) {
@@ -413,7 +421,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_co
     __syncthreads();
 
     // (the tile's inputs have been read)
-    if (threadIdx.x == 32 * (kRuns - 1)) send_for<T, TMA, 3, kTile>(p, maps, &sh.ticket[s], &sh.full[s], turn + 2, stage, false);
+    if (threadIdx.x == 32 * (kRuns - 1)) send_for<T, TMA, 3, kTile>(p, maps, &sh.which[s], &sh.full[s], turn + 2, stage, false);
     const bool last = k == p.tiles - 1;
     Share tile = {};
     if (w == 0) {
@@ -467,13 +475,13 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
   Shared<2>& sh = *reinterpret_cast<Shared<2>*>(smem + 2 * kStage * sizeof(T));
   __shared__ Pair sums[2][kRuns][32];
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
-  const unsigned units = (unsigned)p.strips * p.batch;
   if (threadIdx.x == 0) {
     sh.dead = 0;
     ptx::mbar_init(&sh.full[0], 1);
     ptx::mbar_init(&sh.full[1], 1);
     ptx::fence_mbar_init();
-    for (int s = 0; s < 2; ++s) send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.ticket[s], &sh.full[s], s, stages + s * kStage, true);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words)
+    for (int s = 0; s < 2; ++s) send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s], &sh.full[s], s, stages + s * kStage, true);
   }
   __syncthreads();
 
@@ -491,9 +499,9 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
-    const unsigned ticket = sh.ticket[s];
-    if (ticket >= p.total) break;
-    const int kb = (int)(ticket / units), k = p.tiles - 1 - kb, unit = (int)(ticket % units), strip = unit % p.strips, b = unit / p.strips;
+    const int4 which = sh.which[s];
+    if (which.x < 0) break;
+    const int kb = which.x, k = p.tiles - 1 - kb, unit = which.y, strip = which.z, b = which.w;
     const int t0 = k * kTileGrad + w * L;
     const int here = min(L, p.seqlen - t0);
     const Lane ln(strip, p.channels);
@@ -527,7 +535,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
           const Pair inv = g.inv();
           a[t] = g.a;
           sr[t] = g.sr;
-          si[t] = each(ri(t), sigmoid_approx);
+          si[t] = sigmoid(ri(t));
           wt[t] = (g.om * inv) * si[t];
           const Pair ai = g.a * inv;
           m[t] = ai * ai;
@@ -541,17 +549,27 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
         for (int t = 0; t < L; ++t)
           if (t >= here) a[t] = one, sr[t] = si[t] = wt[t] = m[t] = both(0.f);
       }
+if (marks == 0) {
 #pragma unroll
-      for (int t = 0; t < L; ++t) {
-        const Pair u = wt[t] * x(t);
-        own.P = own.P * a[t];
-        own.q = fma(a[t], own.q, u);
-        if (marks >> t & 1) own = {both(__uint_as_float(kFresh)), u};
-      }
+        for (int t = 0; t < L; ++t) {
+          own.P = own.P * a[t];
+          own.q = fma(a[t], own.q, wt[t] * x(t));
+        }
 #pragma unroll
-      for (int t = L - 1; t >= 0; --t) {
-        c = a[t] * (dy(t) + c);
-        if (marks >> t & 1) c = both(0.f);
+        for (int t = L - 1; t >= 0; --t) c = a[t] * (dy(t) + c);
+      } else {
+#pragma unroll
+        for (int t = 0; t < L; ++t) {
+          const Pair u = wt[t] * x(t);
+          own.P = own.P * a[t];
+          own.q = fma(a[t], own.q, u);
+          if (marks >> t & 1) own = {both(__uint_as_float(kFresh)), u};
+        }
+#pragma unroll
+        for (int t = L - 1; t >= 0; --t) {
+          c = a[t] * (dy(t) + c);
+          if (marks >> t & 1) c = both(0.f);
+        }
       }
     }
     auto &run = sh.run[s][0], &back = sh.run[s][1];
@@ -561,7 +579,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
 
     // (the inputs of the tile before have been read)
     if (turn > 0 && threadIdx.x == 32 * (kRuns - 1))
-      send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.ticket[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true);
+      send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true);
     leave_sums(s ^ 1);
     part = p.part + ((int64_t)b * p.tiles + k) * ((int64_t)p.strips * kStrip) + ln.c;
     const bool last = kb == p.tiles - 1;   // of the way back: the sequence's first
@@ -587,12 +605,14 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
     c = through(c, kRuns - 1 - w, [&](int v) { return back[kRuns - 1 - v][lane]; });
 
     Pair sum = both(0.f);
-    if (here > 0) {
+    // ALL: every token of the run is there and none is marked
+    auto again = [&](auto all) {
+      constexpr bool ALL = decltype(all)::value;
 #pragma unroll
       for (int t = 0; t < L; ++t) {   // m becomes a h[t-1] - m u
         const Pair u = wt[t] * x(t);
         Pair before = a[t] * h;
-        if (marks >> t & 1) before = both(0.f);
+        if (!ALL && (marks >> t & 1)) before = both(0.f);
         h = before + u;
         m[t] = fma(m[t] * minus, u, before);
       }
@@ -606,14 +626,16 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
         const Pair gw = g * wt[t];
         sum = sum + dv;
         c = a[t] * g;
-        if (marks >> t & 1) c = both(0.f);
-        if (t < here) {
+        if (!ALL && (marks >> t & 1)) c = both(0.f);
+        if (ALL || t < here) {
           ln.template store<T, TMA>(dx, gw);
           ln.template store<T, TMA>(di, (gw * x(t)) * fma(si[t], minus, one));
           ln.template store<T, TMA>(dr, dv * fma(sr[t], one, minus));
         }
       }
-    }
+    };
+    if (marks == 0 && here == L) again(std::true_type());
+    else if (here > 0) again(std::false_type());
     sums[s][w][lane] = sum;
   }
   __syncthreads();
@@ -630,6 +652,14 @@ struct FinishDecay {
     out[c] = plus < 1e-30f ? -v : -v * (1.f / (1.f + expf(-decay[c])) / plus);
   }
 };
+
+// Ahead of a scan: sets its words, and works every channel's rate out.
+__global__ void __launch_bounds__(256) prepare_kernel(uint4* words, int64_t n, const float* decay, float* rates, int channels, int padded, float rate) {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+  const int64_t i0 = (int64_t)blockIdx.x * blockDim.x + threadIdx.x, step = (int64_t)gridDim.x * blockDim.x;
+  for (int64_t i = i0; i < n; i += step) words[i] = make_uint4(kNone, kNone, kNone, kNone);
+  for (int64_t c = i0; c < padded; c += step) rates[c] = c < channels ? decay_rate(rate, decay[c]) : 0.f;
+}
 
 // One token.  V channels per thread.
 template <typename T, int V>
@@ -663,7 +693,7 @@ __global__ void __launch_bounds__(128) gated_step_kernel(const T* __restrict__ x
     for (int e = 0; e < V; e += 2) {
       const Gates<false> g(pair(decay_rate(rate, dv[e]), decay_rate(rate, dv[e + 1])), pair(Cvt<T>::to_f(rv[e]), Cvt<T>::to_f(rv[e + 1])));
       const Pair x2 = pair(Cvt<T>::to_f(xv[e]), Cvt<T>::to_f(xv[e + 1])), i2 = pair(Cvt<T>::to_f(iv[e]), Cvt<T>::to_f(iv[e + 1]));
-      const float2 h = halves(fma(g.a, pair(sv[e], sv[e + 1]), (g.om * g.inv()) * (each(i2, sigmoid_approx) * x2)));
+      const float2 h = halves(fma(g.a, pair(sv[e], sv[e + 1]), (g.om * g.inv()) * (sigmoid(i2) * x2)));
       sv[e] = h.x;
       sv[e + 1] = h.y;
       yv[e] = Cvt<T>::from_f(h.x);
@@ -678,7 +708,7 @@ int strips_of(int channels) { return (channels + kStrip - 1) / kStrip; }
 int64_t up256(int64_t v) { return (v + 255) / 256 * 256; }
 
 struct Sizes {
-  int64_t tiles, units, words, part;   // tiles of a sequence, sequences of 64 channels, bytes
+  int64_t tiles, units, words, rates, part;   // tiles of a sequence, sequences of 64 channels, bytes
 };
 Sizes sizes_of(const SsdGatedScanArgs& a, bool grad) {
   Sizes z;
@@ -686,6 +716,8 @@ Sizes sizes_of(const SsdGatedScanArgs& a, bool grad) {
   z.tiles = (a.seqlen + (int64_t)tile - 1) / tile;
   z.units = (int64_t)a.batch * strips_of(a.channels);
   z.words = z.tiles == 1 ? 0 : 256 + z.units * z.tiles * kStrip * 12;
+  // (a CTA that works on one tile works its channels' rates out by itself)
+  z.rates = z.tiles * z.units > 148 ? up256((int64_t)strips_of(a.channels) * kStrip * 4) : 0;
   z.part = grad ? z.units * z.tiles * kStrip * 4 : 0;
   return z;
 }
@@ -732,9 +764,10 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
     p.counter = reinterpret_cast<unsigned*>(ws);
     p.pairs = reinterpret_cast<unsigned long long*>(ws + 256);
     p.states = reinterpret_cast<unsigned long long*>(ws + 256 + z.units * z.tiles * kStrip * 8);
-    if (cudaMemsetAsync(ws, 0xff, (size_t)z.words, stream) != cudaSuccess) return SSD_ERR_CUDA;
   }
-  p.part = reinterpret_cast<float*>(ws + up256(z.words));
+  float* const rates = z.rates ? reinterpret_cast<float*>(ws + up256(z.words)) : nullptr;
+  p.rates = rates;
+  p.part = reinterpret_cast<float*>(ws + up256(z.words) + z.rates);
   // by TMA: every row starts on 16 bytes
   bool tma = a.channels * sizeof(T) % 16 == 0;
   auto strides = [&](int64_t (&to)[2], const int64_t (&from)[2], const void* at) {
@@ -769,7 +802,12 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   const unsigned grid = std::min(p.total, 148u * (sizeof(T) == 2 ? 2 : 1));
   auto go = [&](auto kernel, size_t smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)SSD_ERR_CUDA;
-    return launch(kernel, grid, kThreads, smem, stream, p, maps);
+    if (!z.words && !z.rates) return launch(kernel, grid, kThreads, smem, stream, p, maps);
+    const int64_t n = z.words / 16, padded = z.rates ? (int64_t)p.strips * kStrip : 0;
+    const unsigned blocks = (unsigned)std::min<int64_t>(148 * 4, (std::max(n, padded) + 255) / 256);
+    if (const int rc = launch(prepare_kernel, blocks, 256, 0, stream, reinterpret_cast<uint4*>(ws), n, a.decay, rates, a.channels, (int)padded, a.rate))
+      return rc;
+    return launch_early(kernel, grid, kThreads, smem, stream, p, maps);
   };
   if (!grad) {
     const size_t smem = 2 * stage_numbers(3, kTile) * sizeof(T) + sizeof(Shared<1>);
@@ -802,7 +840,7 @@ int run_step(const SsdGatedStepArgs& a, cudaStream_t stream) {
 extern "C" size_t ssd_b200_gated_scan_workspace_bytes(const SsdGatedScanArgs* args, int32_t backward) {
   if (ssd::check(args, backward != 0) != SSD_OK) return 0;
   const ssd::Sizes z = ssd::sizes_of(*args, backward != 0);
-  return (size_t)(ssd::up256(z.words) + z.part);
+  return (size_t)(ssd::up256(z.words) + z.rates + z.part);
 }
 
 extern "C" int ssd_b200_gated_scan(const SsdGatedScanArgs* args, void* stream) {

@@ -123,20 +123,21 @@ __device__ __forceinline__ void store_two(T* p, int apart, bool ok0, bool ok1, P
   }
 }
 
-// Functions of the special-function unit: relative errors of 2^-22 and less, infinities and NaN as IEEE has them.
+// Functions of the special-function unit: relative errors of 2^-22 and less, infinities and NaN as IEEE has them.  Numbers below the normal
+// ones count as zero: what would keep them takes four more instructions.
 __device__ __forceinline__ float exp2_approx(float v) {
   float r;
-  asm("ex2.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ float rcp_approx(float v) {
   float r;
-  asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 __device__ __forceinline__ float rsqrt_approx(float v) {
   float r;
-  asm("rsqrt.approx.f32 %0, %1;" : "=f"(r) : "f"(v));
+  asm("rsqrt.approx.ftz.f32 %0, %1;" : "=f"(r) : "f"(v));
   return r;
 }
 constexpr float kLog2E = 1.4426950408889634f;
