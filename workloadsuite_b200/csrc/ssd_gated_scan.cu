@@ -26,10 +26,11 @@
 namespace ssd {
 namespace {
 
-constexpr int kRuns = 8, kThreads = 32 * kRuns, kStrip = 64, kPiece = 64, kLook = kRuns;
-constexpr int kRun = 16, kRunGrad = 8;
-constexpr int kTile = kRun * kRuns, kTileGrad = kRunGrad * kRuns;
-static_assert(kTile % kPiece == 0 && kPiece % kRun == 0 && kTileGrad == kPiece, "pieces start at runs");
+constexpr int kStrip = 64, kPiece = 64;
+constexpr int kRun = 16, kRuns = 8, kTile = kRun * kRuns;                       // tokens of a run, runs of a tile
+constexpr int kCtas = 2, kCtasGrad = 2;   // that an SM holds
+constexpr int kRunGrad = 8, kRunsGrad = 8, kTileGrad = kRunGrad * kRunsGrad;
+static_assert(kPiece % kRun == 0 && kTileGrad == kPiece, "pieces start at runs");
 
 struct Scan {
   const void *x, *i, *r, *dy;
@@ -141,10 +142,10 @@ __device__ __forceinline__ Pair through(Pair s, int n, At at) {
 }
 __device__ __forceinline__ bool is_fresh(Pair P) { return P.v == two_words(kFresh, kFresh); }
 
-template <int SIDES>
+template <int RUNS, int SIDES>
 struct Shared {
-  Share run[2][SIDES][kRuns][32];   // of the runs, tiles in turn; the gradient's other side is that of the way back
-  Share seen[kLook][32];            // of the tiles before this one, the nearest first
+  Share run[2][SIDES][RUNS][32];    // of the runs, tiles in turn; the gradient's other side is that of the way back
+  Share seen[RUNS][32];             // of the tiles before this one, the nearest first
   int4 which[2];                    // place in its sequence (-1: there is no tile left), unit, strip, batch entry
   int dead;                         // a wait ran out: no further one
   alignas(8) uint64_t full[2];
@@ -179,8 +180,8 @@ __device__ __forceinline__ void send_for(const Scan& p, const Maps& maps, int4* 
                  : "memory");
 }
 
-template <int SIDES>
-__device__ __forceinline__ void wait_for(const Scan& p, Shared<SIDES>& sh, uint64_t* full, unsigned parity) {
+template <typename S>
+__device__ __forceinline__ void wait_for(const Scan& p, S& sh, uint64_t* full, unsigned parity) {
   if (ptx::mbar_try_wait(full, parity)) return;
   const long long t0 = clock64();
   while (!ptx::mbar_try_wait(full, parity)) {
@@ -194,11 +195,11 @@ __device__ __forceinline__ void wait_for(const Scan& p, Shared<SIDES>& sh, uint6
 }
 
 // One operand's tile where TMA cannot read it (rows that do not start on 16 bytes): two channels a lane, by all threads.
-template <typename T, int TILE>
+template <typename T, int TILE, int RUNS>
 __device__ __forceinline__ void fill(T* to, const void* from, int b, int t0, int seqlen, const int64_t* st, int c, int channels) {
   const int lane = threadIdx.x % 32;
   const T* at = static_cast<const T*>(from) + b * st[0] + (int64_t)t0 * st[1] + c;
-  for (int t = threadIdx.x / 32; t < TILE; t += kRuns) {
+  for (int t = threadIdx.x / 32; t < TILE; t += RUNS) {
     const bool there = t0 + t < seqlen;
 #pragma unroll
     for (int e = 0; e < 2; ++e) {
@@ -217,13 +218,14 @@ __device__ __forceinline__ unsigned marks_of(const Scan& p, int b, int t0, int h
 }
 
 // The share of the whole tile, runs in their order (or, for the way back, from the last to the first).
-__device__ __forceinline__ Share whole(const Share (&run)[kRuns][32], bool backwards) {
+template <int RUNS>
+__device__ __forceinline__ Share whole(const Share (&run)[RUNS][32], bool backwards) {
   const int lane = threadIdx.x % 32;
-  auto at = [&](int v) { return run[backwards ? kRuns - 1 - v : v][lane]; };
-  Share all = {both(1.f), through(both(0.f), kRuns, at)};
+  auto at = [&](int v) { return run[backwards ? RUNS - 1 - v : v][lane]; };
+  Share all = {both(1.f), through(both(0.f), RUNS, at)};
   bool f0 = false, f1 = false;
 #pragma unroll
-  for (int v = 0; v < kRuns; ++v) {
+  for (int v = 0; v < RUNS; ++v) {
     const Pair P = at(v).P;
     f0 |= (unsigned)P.v == kFresh;
     f1 |= (unsigned)(P.v >> 32) == kFresh;
@@ -248,8 +250,8 @@ __device__ __forceinline__ void publish(const Scan& p, int64_t tile, Pair s) {
 
 // What stands before tile `k` of the unit, into sh.seen: warp w looks at tile k - 1 - w, for its state or else its pair; the farthest
 // one waits for the state, so that one look is enough.
-template <int SIDES>
-__device__ __forceinline__ void look_back(const Scan& p, Shared<SIDES>& sh, int64_t first, int k) {
+template <int RUNS, int SIDES>
+__device__ __forceinline__ void look_back(const Scan& p, Shared<RUNS, SIDES>& sh, int64_t first, int k) {
   const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
   if (w >= k) return;
   const int64_t tile = first + k - 1 - w;
@@ -259,7 +261,7 @@ __device__ __forceinline__ void look_back(const Scan& p, Shared<SIDES>& sh, int6
   long long t0 = 0;
   while (true) {
     s = load_word(state);
-    if (w != kLook - 1) {
+    if (w != RUNS - 1) {
       p0 = load_word(at);
       p1 = load_word(at + 1);
     }
@@ -280,9 +282,9 @@ __device__ __forceinline__ void look_back(const Scan& p, Shared<SIDES>& sh, int6
 }
 
 // The state entering a tile from what look_back() saw: from the nearest place that nothing before it matters to.
-template <int SIDES>
-__device__ __forceinline__ Pair fold_seen(const Shared<SIDES>& sh, int k) {
-  const int n = min(k, kLook), lane = threadIdx.x % 32;
+template <int RUNS, int SIDES>
+__device__ __forceinline__ Pair fold_seen(const Shared<RUNS, SIDES>& sh, int k) {
+  const int n = min(k, RUNS), lane = threadIdx.x % 32;
   int w = 0;
   while (w < n - 1 && !is_fresh(sh.seen[w][lane].P)) ++w;
   return through(both(0.f), w + 1, [&](int v) { return sh.seen[w - v][lane]; });
@@ -328,12 +330,12 @@ struct Lane {
 
 // TMA: every tensor's rows start on 16 bytes.
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(32 * kRuns, kCtas) gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
   using Raw = typename Two<T>::Raw;
   constexpr int L = kRun, kStage = (int)stage_numbers(3, kTile);
   extern __shared__ __align__(128) unsigned char smem[];
   T* const stages = reinterpret_cast<T*>(smem);
-  Shared<1>& sh = *reinterpret_cast<Shared<1>*>(smem + 2 * kStage * sizeof(T));
+  Shared<kRuns, 1>& sh = *reinterpret_cast<Shared<kRuns, 1>*>(smem + 2 * kStage * sizeof(T));
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     sh.dead = 0;
@@ -358,9 +360,9 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_co
     const int64_t first = (int64_t)unit * p.tiles;
     if constexpr (!TMA) {
       const int c = strip * kStrip;
-      fill<T, kTile>(stage, p.x, b, k * kTile, p.seqlen, p.xs, c, p.channels);
-      fill<T, kTile>(stage + kTile * kStrip, p.i, b, k * kTile, p.seqlen, p.is, c, p.channels);
-      fill<T, kTile>(stage + 2 * kTile * kStrip, p.r, b, k * kTile, p.seqlen, p.rs, c, p.channels);
+      fill<T, kTile, kRuns>(stage, p.x, b, k * kTile, p.seqlen, p.xs, c, p.channels);
+      fill<T, kTile, kRuns>(stage + kTile * kStrip, p.i, b, k * kTile, p.seqlen, p.is, c, p.channels);
+      fill<T, kTile, kRuns>(stage + 2 * kTile * kStrip, p.r, b, k * kTile, p.seqlen, p.rs, c, p.channels);
       __syncthreads();
     }
     const Raw* const raw = reinterpret_cast<const Raw*>(stage + w * L * kStrip) + lane;
@@ -467,13 +469,13 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_kernel(const __grid_co
 // With w = b si, u = w x and m = a^2 / (1 - a^2):  dx = g w,  di = g u (1 - si),  dla = g (a h[t-1] - m u)  (without its first term at a
 // reset),  dr = dla la (1 - sr),  and what decay's gradient sums up is dla la.
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(32 * kRunsGrad, kCtasGrad) gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
   using Raw = typename Two<T>::Raw;
   constexpr int L = kRunGrad, kStage = (int)stage_numbers(4, kTileGrad);
   extern __shared__ __align__(128) unsigned char smem[];
   T* const stages = reinterpret_cast<T*>(smem);
-  Shared<2>& sh = *reinterpret_cast<Shared<2>*>(smem + 2 * kStage * sizeof(T));
-  __shared__ Pair sums[2][kRuns][32];
+  Shared<kRunsGrad, 2>& sh = *reinterpret_cast<Shared<kRunsGrad, 2>*>(smem + 2 * kStage * sizeof(T));
+  __shared__ Pair sums[2][kRunsGrad][32];
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     sh.dead = 0;
@@ -491,7 +493,7 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
     if (part && w == 0) {
       Pair v = sums[s][0][lane];
 #pragma unroll
-      for (int n = 1; n < kRuns; ++n) v = v + sums[s][n][lane];
+      for (int n = 1; n < kRunsGrad; ++n) v = v + sums[s][n][lane];
       *reinterpret_cast<float2*>(part) = halves(v);
     }
   };
@@ -508,10 +510,10 @@ __global__ void __launch_bounds__(kThreads, 2) gated_scan_grad_kernel(const __gr
     const int64_t first = (int64_t)unit * p.tiles;
     if constexpr (!TMA) {
       const int c = strip * kStrip, n = kTileGrad * kStrip;
-      fill<T, kTileGrad>(stage, p.x, b, k * kTileGrad, p.seqlen, p.xs, c, p.channels);
-      fill<T, kTileGrad>(stage + n, p.i, b, k * kTileGrad, p.seqlen, p.is, c, p.channels);
-      fill<T, kTileGrad>(stage + 2 * n, p.r, b, k * kTileGrad, p.seqlen, p.rs, c, p.channels);
-      fill<T, kTileGrad>(stage + 3 * n, p.dy, b, k * kTileGrad, p.seqlen, p.dys, c, p.channels);
+      fill<T, kTileGrad, kRunsGrad>(stage, p.x, b, k * kTileGrad, p.seqlen, p.xs, c, p.channels);
+      fill<T, kTileGrad, kRunsGrad>(stage + n, p.i, b, k * kTileGrad, p.seqlen, p.is, c, p.channels);
+      fill<T, kTileGrad, kRunsGrad>(stage + 2 * n, p.r, b, k * kTileGrad, p.seqlen, p.rs, c, p.channels);
+      fill<T, kTileGrad, kRunsGrad>(stage + 3 * n, p.dy, b, k * kTileGrad, p.seqlen, p.dys, c, p.channels);
       __syncthreads();
     }
     const Raw* const raw = reinterpret_cast<const Raw*>(stage + w * L * kStrip) + lane;
@@ -578,7 +580,7 @@ if (marks == 0) {
     __syncthreads();
 
     // (the inputs of the tile before have been read)
-    if (turn > 0 && threadIdx.x == 32 * (kRuns - 1))
+    if (turn > 0 && threadIdx.x == 32 * (kRunsGrad - 1))
       send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true);
     leave_sums(s ^ 1);
     part = p.part + ((int64_t)b * p.tiles + k) * ((int64_t)p.strips * kStrip) + ln.c;
@@ -602,7 +604,7 @@ if (marks == 0) {
       else if (p.dinit) ln.put(p.dinit + (int64_t)b * p.channels, out);
     }
     h = through(h, w, [&](int v) { return run[v][lane]; });
-    c = through(c, kRuns - 1 - w, [&](int v) { return back[kRuns - 1 - v][lane]; });
+    c = through(c, kRunsGrad - 1 - w, [&](int v) { return back[kRunsGrad - 1 - v][lane]; });
 
     Pair sum = both(0.f);
     // ALL: every token of the run is there and none is marked
@@ -799,22 +801,22 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
           (!grad || operand_map<T>(&maps.at[3], a.dy, a, p.dys, tile));
   }
   // two CTAs an SM, one where tiles are of 32-bit numbers
-  const unsigned grid = std::min(p.total, 148u * (sizeof(T) == 2 ? 2 : 1));
-  auto go = [&](auto kernel, size_t smem) {
+  const unsigned grid = std::min(p.total, 148u * (sizeof(T) == 2 ? (grad ? kCtasGrad : kCtas) : 1));
+  auto go = [&](auto kernel, int threads, size_t smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)SSD_ERR_CUDA;
-    if (!z.words && !z.rates) return launch(kernel, grid, kThreads, smem, stream, p, maps);
+    if (!z.words && !z.rates) return launch(kernel, grid, threads, smem, stream, p, maps);
     const int64_t n = z.words / 16, padded = z.rates ? (int64_t)p.strips * kStrip : 0;
     const unsigned blocks = (unsigned)std::min<int64_t>(148 * 4, (std::max(n, padded) + 255) / 256);
     if (const int rc = launch(prepare_kernel, blocks, 256, 0, stream, reinterpret_cast<uint4*>(ws), n, a.decay, rates, a.channels, (int)padded, a.rate))
       return rc;
-    return launch_early(kernel, grid, kThreads, smem, stream, p, maps);
+    return launch_early(kernel, grid, threads, smem, stream, p, maps);
   };
   if (!grad) {
-    const size_t smem = 2 * stage_numbers(3, kTile) * sizeof(T) + sizeof(Shared<1>);
-    return tma ? go(gated_scan_kernel<T, true>, smem) : go(gated_scan_kernel<T, false>, smem);
+    const size_t smem = 2 * stage_numbers(3, kTile) * sizeof(T) + sizeof(Shared<kRuns, 1>);
+    return tma ? go(gated_scan_kernel<T, true>, 32 * kRuns, smem) : go(gated_scan_kernel<T, false>, 32 * kRuns, smem);
   }
-  const size_t smem = 2 * stage_numbers(4, kTileGrad) * sizeof(T) + sizeof(Shared<2>);
-  if (const int rc = tma ? go(gated_scan_grad_kernel<T, true>, smem) : go(gated_scan_grad_kernel<T, false>, smem)) return rc;
+  const size_t smem = 2 * stage_numbers(4, kTileGrad) * sizeof(T) + sizeof(Shared<kRunsGrad, 2>);
+  if (const int rc = tma ? go(gated_scan_grad_kernel<T, true>, 32 * kRunsGrad, smem) : go(gated_scan_grad_kernel<T, false>, 32 * kRunsGrad, smem)) return rc;
   return launch_column_sum(p.part, a.batch * z.tiles, (int64_t)p.strips * kStrip, a.channels, FinishDecay{a.decay, a.ddecay}, stream);
 }
 

@@ -1,9 +1,12 @@
 // RMS norms between blocks and their gradients (formulas: ssd_b200.h).
-// A row (of a group) is one warp's or one CTA's, eight numbers a thread and step, kept in registers: every input is read once, every
-// output written once.  The gradients against vectors are sums over rows: a CTA adds those of its rows up in registers and leaves
+// A row (of a group) is one warp's or one CTA's, eight numbers a thread and step, worked on in registers: every input is read once, every
+// output written once.  CTAs stay and take rows in turn; the inputs of the next rows are on their way (cp.async) while one is worked on, each
+// thread's into places that nobody else reads, so that waiting for its own copies is all the synchronisation they need.
+// The gradients against vectors are sums over rows: a CTA adds those of its rows up in registers and leaves
 // them to column_sum_kernel, so that their order is fixed.
 #include <algorithm>
 #include <cmath>
+#include <type_traits>
 
 #include "vec_io.cuh"
 
@@ -16,49 +19,70 @@ template <bool VEC>
 __device__ __forceinline__ int place(int it, int e) {
   return VEC ? (it * (int)blockDim.x + (int)threadIdx.x) * 8 + e : (it * 8 + e) * (int)blockDim.x + (int)threadIdx.x;
 }
+struct Eight {
+  Pair v[4];
+  __device__ __forceinline__ Pair& operator[](int e) { return v[e]; }
+  __device__ __forceinline__ Pair operator[](int e) const { return v[e]; }
+};
+template <typename F>
+__device__ __forceinline__ void four(F f) {
+#pragma unroll
+  for (int e = 0; e < 4; ++e) f(e);
+}
+__device__ __forceinline__ Pair words_to_pair(const float*, const uint4& q, int e) {
+  return e == 0 ? pair(__uint_as_float(q.x), __uint_as_float(q.y)) : pair(__uint_as_float(q.z), __uint_as_float(q.w));
+}
+template <typename T>
+__device__ __forceinline__ Eight widen(const uint4& a, const uint4& b) {
+  Eight r;
+  if constexpr (sizeof(T) == 2) {
+    r[0] = pair_of<T>(a.x); r[1] = pair_of<T>(a.y); r[2] = pair_of<T>(a.z); r[3] = pair_of<T>(a.w);
+  } else {
+    const float* t = nullptr;
+    r[0] = words_to_pair(t, a, 0); r[1] = words_to_pair(t, a, 1); r[2] = words_to_pair(t, b, 0); r[3] = words_to_pair(t, b, 1);
+  }
+  return r;
+}
 template <typename T, bool VEC>
-__device__ __forceinline__ void get8(const T* __restrict__ row, int it, int d, float (&v)[8]) {
+__device__ __forceinline__ Eight get8(const T* __restrict__ row, int it, int d) {
   if constexpr (VEC) {
     const int at = place<true>(it, 0);
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
     if (at < d) {
-      if constexpr (sizeof(T) == 2) {
-        const uint4 q = *reinterpret_cast<const uint4*>(row + at);
-        const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const float2 f = Two<T>::up(w[e]);
-          v[2 * e] = f.x;
-          v[2 * e + 1] = f.y;
-        }
-      } else {
-        const float4 a = *reinterpret_cast<const float4*>(row + at), b = *reinterpret_cast<const float4*>(row + at + 4);
-        v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
-      }
-    } else {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = 0.f;
+      a = *reinterpret_cast<const uint4*>(row + at);
+      if (sizeof(T) == 4) b = *reinterpret_cast<const uint4*>(row + at + 4);
     }
+    return widen<T>(a, b);
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) v[e] = place<false>(it, e) < d ? Cvt<T>::to_f(row[place<false>(it, e)]) : 0.f;
+    Eight r;
+    four([&](int e) {
+      const int i0 = place<false>(it, 2 * e), i1 = place<false>(it, 2 * e + 1);
+      r[e] = pair(i0 < d ? Cvt<T>::to_f(row[i0]) : 0.f, i1 < d ? Cvt<T>::to_f(row[i1]) : 0.f);
+    });
+    return r;
   }
 }
 template <typename T, bool VEC>
-__device__ __forceinline__ void put8(T* row, int it, int d, const float (&v)[8]) {
+__device__ __forceinline__ void put8(T* row, int it, int d, const Eight& v) {
   if constexpr (VEC) {
     const int at = place<true>(it, 0);
     if (at < d) {
       if constexpr (sizeof(T) == 2) {
-        *reinterpret_cast<uint4*>(row + at) = make_uint4(Two<T>::down(v[0], v[1]), Two<T>::down(v[2], v[3]), Two<T>::down(v[4], v[5]), Two<T>::down(v[6], v[7]));
+        auto word = [&](int e) { return Two<T>::down(halves(v[e]).x, halves(v[e]).y); };
+        *reinterpret_cast<uint4*>(row + at) = make_uint4(word(0), word(1), word(2), word(3));
       } else {
-        *reinterpret_cast<float4*>(row + at) = make_float4(v[0], v[1], v[2], v[3]);
-        *reinterpret_cast<float4*>(row + at + 4) = make_float4(v[4], v[5], v[6], v[7]);
+        const float2 a = halves(v[0]), b = halves(v[1]), c = halves(v[2]), e = halves(v[3]);
+        *reinterpret_cast<float4*>(row + at) = make_float4(a.x, a.y, b.x, b.y);
+        *reinterpret_cast<float4*>(row + at + 4) = make_float4(c.x, c.y, e.x, e.y);
       }
     }
   } else {
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (place<false>(it, e) < d) row[place<false>(it, e)] = Cvt<T>::from_f(v[e]);
+    four([&](int e) {
+      const float2 f = halves(v[e]);
+      const int i0 = place<false>(it, 2 * e), i1 = place<false>(it, 2 * e + 1);
+      if (i0 < d) row[i0] = Cvt<T>::from_f(f.x);
+      if (i1 < d) row[i1] = Cvt<T>::from_f(f.y);
+    });
   }
 }
 
@@ -67,9 +91,8 @@ struct Vector {
   const void* p;
   int in_dtype;
   template <typename T, bool VEC>
-  __device__ __forceinline__ void get(int first, int it, int d, float (&v)[8]) const {
-    if (in_dtype) get8<T, VEC>(static_cast<const T*>(p) + first, it, d, v);
-    else get8<float, VEC>(static_cast<const float*>(p) + first, it, d, v);
+  __device__ __forceinline__ Eight get(int first, int it, int d) const {
+    return in_dtype ? get8<T, VEC>(static_cast<const T*>(p) + first, it, d) : get8<float, VEC>(static_cast<const float*>(p) + first, it, d);
   }
 };
 
@@ -77,7 +100,9 @@ struct Vector {
 struct RowSum {
   float* place;   // [2][32]
   int turn;
-  __device__ __forceinline__ float operator()(float v) {
+  __device__ __forceinline__ float operator()(Pair s) {
+    const float2 h = halves(s);
+    float v = h.x + h.y;
 #pragma unroll
     for (int k = 16; k > 0; k /= 2) v += __shfl_xor_sync(~0u, v, k);
     if (blockDim.x > 32) {
@@ -102,259 +127,388 @@ struct Norm {
   int64_t rows, xs, zs, rs, ys, ros, dys, dros, dxs, dzs, drs;
   int d, groups, norm_first, vectors;   // d: of a group; vectors: of d * groups partial sums a row of `part` holds
   float eps;
+  // what the norm behind the block and the scale multiply by
+  template <typename T, bool VEC>
+  __device__ __forceinline__ Eight outer(int it) const {
+    if (!post.p) return scale.get<T, VEC>(0, it, d);
+    Eight o = post.get<T, VEC>(0, it, d);
+    if (scale.p) {
+      const Eight s = scale.get<T, VEC>(0, it, d);
+      four([&](int e) { o[e] = o[e] * s[e]; });
+    }
+    return o;
+  }
 };
 
-// A row per warp (blockDim.y of them) or per CTA.
-template <typename F>
-__device__ __forceinline__ void for_rows(const Norm& p, F f) {
-  for (int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y; row < p.rows; row += (int64_t)gridDim.x * blockDim.y) f(row);
-}
+// The inputs of the rows to come: a thread's sixteen-byte pieces (PIECES a row), STAGES rows ahead.
+template <int PIECES, int STAGES>
+struct Ahead {
+  uint32_t base;
+  __device__ __forceinline__ Ahead() {
+    extern __shared__ __align__(16) unsigned char smem[];
+    base = (uint32_t)__cvta_generic_to_shared(smem) + (threadIdx.y * blockDim.x + threadIdx.x) * 16;
+  }
+  __device__ __forceinline__ uint32_t at(int stage, int piece) const {
+    return base + (uint32_t)((stage * PIECES + piece) * (int)(blockDim.x * blockDim.y) * 16);
+  }
+  // pieces first, first + 1 .. of a row's numbers of this thread
+  template <typename T, int I>
+  __device__ __forceinline__ void send(int stage, int first, const T* row, int d) const {
+#pragma unroll
+    for (int it = 0; it < I; ++it) {
+      const int n = place<true>(it, 0);
+      if (n < d) {
+#pragma unroll
+        for (int q = 0; q < (int)sizeof(T) / 2; ++q)
+          asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(at(stage, first + it * (int)sizeof(T) / 2 + q)), "l"(row + n + 8 * q / ((int)sizeof(T) / 2)) : "memory");
+      }
+    }
+  }
+  template <typename T>
+  __device__ __forceinline__ Eight get(int stage, int first, int it, int d) const {
+    uint4 a = make_uint4(0, 0, 0, 0), b = a;
+    if (place<true>(it, 0) < d) {
+      auto load = [&](uint4& v, int q) {
+        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(at(stage, first + it * (int)sizeof(T) / 2 + q)) : "memory");
+      };
+      load(a, 0);
+      if (sizeof(T) == 4) load(b, 1);
+    }
+    return widen<T>(a, b);
+  }
+};
+// Rows ahead: as many as shared memory holds for the widest CTA (512 threads), up to four; where that is not even two (fp32 beyond 4 096
+// numbers, 16-bit beyond 8 192) rows are read where they are needed.
+constexpr int stages_of(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 3 : pieces <= 13 ? 2 : 0; }
 
-template <typename T, typename R, int I, bool VEC>
-__global__ void __launch_bounds__(I == 1 ? 256 : 512) rms_norm_kernel(const Norm p) {
+// Goes through a CTA's rows (a row per warp, blockDim.y of them, or one per CTA): send(stage, row) asks for a row's inputs,
+// work(stage, row) takes them.
+template <bool AHEAD, int STAGES, typename Send, typename Work>
+__device__ __forceinline__ void for_rows(int64_t rows, Send send, Work work) {
+  const int64_t step = (int64_t)gridDim.x * blockDim.y;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if constexpr (AHEAD) {
+#pragma unroll
+    for (int s = 0; s < STAGES - 1; ++s) {
+      if (row + s * step < rows) send(s, row + s * step);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+    }
+  }
+  int stage = 0;
+  for (; row < rows; row += step) {
+    if constexpr (AHEAD) {
+      const int64_t next = row + (STAGES - 1) * step;
+      if (next < rows) send(stage == 0 ? STAGES - 1 : stage - 1, next);
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
+    }
+    work(stage, row);
+    if (++stage == STAGES) stage = 0;
+  }
+  if constexpr (AHEAD) asm volatile("cp.async.wait_group 0;" ::: "memory");
+}
+__device__ __forceinline__ float inv_rms(float sum, const Norm& p) { return rsqrtf(sum / p.d + p.eps); }
+
+// OUTER: with post_weight or scale.
+template <typename T, typename R, int I, bool VEC, bool OUTER>
+struct Forward {
+  static constexpr int kPieces = I * (int)(sizeof(T) + sizeof(R)) / 2, kStages = stages_of(kPieces);
+  static constexpr bool kAhead = VEC && kStages > 0;
+  static constexpr bool kKeep = I == 1;   // vectors stay in registers
+};
+template <typename T, typename R, int I, bool VEC, bool OUTER>
+__global__ void __launch_bounds__(512) rms_norm_kernel(const Norm p) {
+  using F = Forward<T, R, I, VEC, OUTER>;
+  constexpr int kRes = I * (int)sizeof(T) / 2;
   __shared__ float sums[64];
   RowSum row_sum{sums, 0};
-  for_rows(p, [&](int64_t row) {
-    float v[I][8], old[I][8];
+  const Ahead<F::kPieces, F::kStages> ahead;
+  Eight w[I], ps[I];
+  if constexpr (F::kKeep) {
 #pragma unroll
     for (int it = 0; it < I; ++it) {
-      get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d, v[it]);
-      if (p.res) get8<R, VEC>(static_cast<const R*>(p.res) + row * p.rs, it, p.d, old[it]);
+      w[it] = p.w.get<T, VEC>(0, it, p.d);
+      if constexpr (OUTER) ps[it] = p.outer<T, VEC>(it);
     }
-    if (p.post.p) {
-      float ss = 0.f;
+  }
+  for_rows<F::kAhead, F::kStages>(
+      p.rows,
+      [&](int s, int64_t row) {
+        ahead.template send<T, I>(s, 0, static_cast<const T*>(p.x) + row * p.xs, p.d);
+        if (p.res) ahead.template send<R, I>(s, kRes, static_cast<const R*>(p.res) + row * p.rs, p.d);
+      },
+      [&](int s, int64_t row) {
+        Eight v[I];
 #pragma unroll
-      for (int it = 0; it < I; ++it)
+        for (int it = 0; it < I; ++it)
+          v[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d);
+        if constexpr (OUTER) {
+          float inv = 1.f;
+          if (p.post.p) {
+            Pair ss = both(0.f);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) ss = fmaf(v[it][e], v[it][e], ss);
-      const float inv = rsqrtf(row_sum(ss) / p.d + p.eps);
-      if (p.inv_post && threadIdx.x == 0) p.inv_post[row] = inv;
+            for (int it = 0; it < I; ++it) four([&](int e) { ss = fma(v[it][e], v[it][e], ss); });
+            inv = inv_rms(row_sum(ss), p);
+            if (p.inv_post && threadIdx.x == 0) p.inv_post[row] = inv;
+          }
 #pragma unroll
-      for (int it = 0; it < I; ++it) {
-        float w[8];
-        p.post.get<T, VEC>(0, it, p.d, w);
+          for (int it = 0; it < I; ++it) {
+            if constexpr (!F::kKeep) ps[it] = p.outer<T, VEC>(it);
+            four([&](int e) { v[it][e] = v[it][e] * both(inv) * ps[it][e]; });
+          }
+        }
+        if (p.res) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[it][e] *= inv * w[e];
-      }
-    }
-    if (p.scale.p) {
+          for (int it = 0; it < I; ++it) {
+            const Eight old = F::kAhead ? ahead.template get<R>(s, kRes, it, p.d) : get8<R, VEC>(static_cast<const R*>(p.res) + row * p.rs, it, p.d);
+            four([&](int e) {   // as it is stored
+              const float2 f = halves(old[e] + v[it][e]);
+              v[it][e] = pair_of<R>(Two<R>::down(f.x, f.y));
+            });
+            put8<R, VEC>(static_cast<R*>(p.res_out) + row * p.ros, it, p.d, v[it]);
+          }
+        }
+        Pair ss = both(0.f);
 #pragma unroll
-      for (int it = 0; it < I; ++it) {
-        float w[8];
-        p.scale.get<T, VEC>(0, it, p.d, w);
+        for (int it = 0; it < I; ++it) four([&](int e) { ss = fma(v[it][e], v[it][e], ss); });
+        const float inv = inv_rms(row_sum(ss), p);
+        if (p.inv && threadIdx.x == 0) p.inv[row] = inv;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) v[it][e] *= w[e];
-      }
-    }
-    if (p.res) {
-#pragma unroll
-      for (int it = 0; it < I; ++it) {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) v[it][e] = Cvt<R>::to_f(Cvt<R>::from_f(old[it][e] + v[it][e]));   // as it is stored
-        put8<R, VEC>(static_cast<R*>(p.res_out) + row * p.ros, it, p.d, v[it]);
-      }
-    }
-    float ss = 0.f;
-#pragma unroll
-    for (int it = 0; it < I; ++it)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) ss = fmaf(v[it][e], v[it][e], ss);
-    const float inv = rsqrtf(row_sum(ss) / p.d + p.eps);
-    if (p.inv && threadIdx.x == 0) p.inv[row] = inv;
-#pragma unroll
-    for (int it = 0; it < I; ++it) {
-      float w[8];
-      p.w.get<T, VEC>(0, it, p.d, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[it][e] *= inv * w[e];
-      put8<T, VEC>(static_cast<T*>(p.y) + row * p.ys, it, p.d, v[it]);
-    }
-  });
+        for (int it = 0; it < I; ++it) {
+          if constexpr (!F::kKeep) w[it] = p.w.get<T, VEC>(0, it, p.d);
+          four([&](int e) { v[it][e] = v[it][e] * both(inv) * w[it][e]; });
+          put8<T, VEC>(static_cast<T*>(p.y) + row * p.ys, it, p.d, v[it]);
+        }
+      });
 }
 
 // Partial sums of this warp's or CTA's rows.
 template <int I, bool VEC>
-__device__ __forceinline__ void leave(const Norm& p, int which, const float (&sum)[I][8]) {
+__device__ __forceinline__ void leave(const Norm& p, int which, const Eight (&sum)[I]) {
   const int64_t all = (int64_t)p.d * p.groups;
   float* to = p.part + (((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * p.vectors + which) * all + (int64_t)blockIdx.y * p.d;
 #pragma unroll
   for (int it = 0; it < I; ++it)
-#pragma unroll
-    for (int e = 0; e < 8; ++e)
-      if (place<VEC>(it, e) < p.d) to[place<VEC>(it, e)] = sum[it][e];
+    four([&](int e) {
+      const float2 f = halves(sum[it][e]);
+      if (place<VEC>(it, 2 * e) < p.d) to[place<VEC>(it, 2 * e)] = f.x;
+      if (place<VEC>(it, 2 * e + 1) < p.d) to[place<VEC>(it, 2 * e + 1)] = f.y;
+    });
 }
 
-// OUTER: with post_weight or scale.
 template <typename T, typename R, int I, bool VEC, bool OUTER>
-__global__ void __launch_bounds__(I == 1 ? 256 : 512) rms_norm_grad_kernel(const Norm p) {
+struct Backward {
+  static constexpr int kPieces = I * (int)(sizeof(T) + 2 * sizeof(R) + (OUTER ? sizeof(T) : 0)) / 2, kStages = stages_of(kPieces);
+  static constexpr bool kAhead = VEC && kStages > 0;
+  static constexpr bool kKeep = I == 1;
+};
+template <typename T, typename R, int I, bool VEC, bool OUTER>
+__global__ void __launch_bounds__(512) rms_norm_grad_kernel(const Norm p) {
+  using F = Backward<T, R, I, VEC, OUTER>;
+  constexpr int kOut = I * (int)sizeof(T) / 2, kIn = kOut + I * (int)sizeof(R) / 2, kX = kIn + I * (int)sizeof(R) / 2;
   __shared__ float sums[64];
   RowSum row_sum{sums, 0};
-  float dw[I][8] = {}, both[I][8] = {};
-  for_rows(p, [&](int64_t row) {
-    float g[I][8], v[I][8], in[I][8];
-    const float inv = p.inv[row];
+  const Ahead<F::kPieces, F::kStages> ahead;
+  Eight dw[I], acc[I], w[I], ps[I];
 #pragma unroll
-    for (int it = 0; it < I; ++it) {
-      get8<T, VEC>(static_cast<const T*>(p.dy) + row * p.dys, it, p.d, g[it]);
-      if (p.res_out) get8<R, VEC>(static_cast<const R*>(p.res_out) + row * p.ros, it, p.d, v[it]);
-      else get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d, v[it]);
-      if (p.dres_out) get8<R, VEC>(static_cast<const R*>(p.dres_out) + row * p.dros, it, p.d, in[it]);
+  for (int it = 0; it < I; ++it) {
+    four([&](int e) { dw[it][e] = acc[it][e] = both(0.f); });
+    if constexpr (F::kKeep) {
+      w[it] = p.w.get<T, VEC>(0, it, p.d);
+      if constexpr (OUTER) ps[it] = p.outer<T, VEC>(it);
     }
-    float c = 0.f;
+  }
+  for_rows<F::kAhead, F::kStages>(
+      p.rows,
+      [&](int s, int64_t row) {
+        ahead.template send<T, I>(s, 0, static_cast<const T*>(p.dy) + row * p.dys, p.d);
+        if (p.res_out) ahead.template send<R, I>(s, kOut, static_cast<const R*>(p.res_out) + row * p.ros, p.d);
+        else ahead.template send<T, I>(s, kOut, static_cast<const T*>(p.x) + row * p.xs, p.d);   // (R is T)
+        if (p.dres_out) ahead.template send<R, I>(s, kIn, static_cast<const R*>(p.dres_out) + row * p.dros, p.d);
+        if constexpr (OUTER) ahead.template send<T, I>(s, kX, static_cast<const T*>(p.x) + row * p.xs, p.d);
+      },
+      [&](int s, int64_t row) {
+        Eight g[I], v[I];
+        const float inv = p.inv[row], invp = OUTER && p.post.p ? p.inv_post[row] : 1.f;
+        Pair c = both(0.f);
 #pragma unroll
-    for (int it = 0; it < I; ++it) {
-      float w[8];
-      p.w.get<T, VEC>(0, it, p.d, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[it][e] *= inv;
-        dw[it][e] = fmaf(g[it][e], v[it][e], dw[it][e]);
-        g[it][e] *= w[e];
-        c = fmaf(g[it][e], v[it][e], c);
-      }
-    }
-    c = row_sum(c) / p.d;
-#pragma unroll
-    for (int it = 0; it < I; ++it) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        g[it][e] = inv * fmaf(-v[it][e], c, g[it][e]);
-        if (p.dres_out) g[it][e] += in[it][e];
-      }
-      if (p.dres) put8<R, VEC>(static_cast<R*>(p.dres) + row * p.drs, it, p.d, g[it]);
-    }
-    if constexpr (OUTER) {
-      const float invp = p.post.p ? p.inv_post[row] : 1.f;
-      float c2 = 0.f;
-#pragma unroll
-      for (int it = 0; it < I; ++it) {
-        float w[8];
-        get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d, v[it]);
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          v[it][e] *= invp;
-          both[it][e] = fmaf(g[it][e], v[it][e], both[it][e]);
+        for (int it = 0; it < I; ++it) {
+          if constexpr (F::kAhead) {
+            g[it] = ahead.template get<T>(s, 0, it, p.d);
+            v[it] = ahead.template get<R>(s, kOut, it, p.d);
+          } else {
+            g[it] = get8<T, VEC>(static_cast<const T*>(p.dy) + row * p.dys, it, p.d);
+            if (p.res_out) v[it] = get8<R, VEC>(static_cast<const R*>(p.res_out) + row * p.ros, it, p.d);
+            else v[it] = get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d);
+          }
+          if constexpr (!F::kKeep) w[it] = p.w.get<T, VEC>(0, it, p.d);
+          four([&](int e) {
+            v[it][e] = v[it][e] * both(inv);
+            dw[it][e] = fma(g[it][e], v[it][e], dw[it][e]);
+            g[it][e] = g[it][e] * w[it][e];
+            c = fma(g[it][e], v[it][e], c);
+          });
         }
-        if (p.scale.p) {
-          p.scale.get<T, VEC>(0, it, p.d, w);
+        const Pair mean = both(-row_sum(c) / p.d);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) g[it][e] *= w[e];
+        for (int it = 0; it < I; ++it) {
+          four([&](int e) { g[it][e] = both(inv) * fma(v[it][e], mean, g[it][e]); });
+          if (p.dres_out) {
+            const Eight in = F::kAhead ? ahead.template get<R>(s, kIn, it, p.d) : get8<R, VEC>(static_cast<const R*>(p.dres_out) + row * p.dros, it, p.d);
+            four([&](int e) { g[it][e] = g[it][e] + in[e]; });
+          }
+          if (p.dres) put8<R, VEC>(static_cast<R*>(p.dres) + row * p.drs, it, p.d, g[it]);
         }
-        if (p.post.p) {
-          p.post.get<T, VEC>(0, it, p.d, w);
+        if constexpr (OUTER) {
+          Pair c2 = both(0.f);
 #pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            g[it][e] *= w[e];
-            c2 = fmaf(g[it][e], v[it][e], c2);
+          for (int it = 0; it < I; ++it) {
+            v[it] = F::kAhead ? ahead.template get<T>(s, kX, it, p.d) : get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d);
+            if constexpr (!F::kKeep) ps[it] = p.outer<T, VEC>(it);
+            four([&](int e) {
+              v[it][e] = v[it][e] * both(invp);
+              acc[it][e] = fma(g[it][e], v[it][e], acc[it][e]);
+              g[it][e] = g[it][e] * ps[it][e];
+              c2 = fma(g[it][e], v[it][e], c2);
+            });
+          }
+          if (p.post.p) {
+            const Pair mean2 = both(-row_sum(c2) / p.d);
+#pragma unroll
+            for (int it = 0; it < I; ++it) four([&](int e) { g[it][e] = both(invp) * fma(v[it][e], mean2, g[it][e]); });
           }
         }
-      }
-      if (p.post.p) {
-        c2 = row_sum(c2) / p.d;
 #pragma unroll
-        for (int it = 0; it < I; ++it)
-#pragma unroll
-          for (int e = 0; e < 8; ++e) g[it][e] = invp * fmaf(-v[it][e], c2, g[it][e]);
-      }
-    }
-#pragma unroll
-    for (int it = 0; it < I; ++it) put8<T, VEC>(static_cast<T*>(p.dx) + row * p.dxs, it, p.d, g[it]);
-  });
+        for (int it = 0; it < I; ++it) put8<T, VEC>(static_cast<T*>(p.dx) + row * p.dxs, it, p.d, g[it]);
+      });
   leave<I, VEC>(p, 0, dw);
-  if constexpr (OUTER) leave<I, VEC>(p, 1, both);
+  if constexpr (OUTER) leave<I, VEC>(p, 1, acc);
+}
+
+__device__ __forceinline__ Pair sigmoid(Pair v) { return each(each(v * both(-kLog2E), exp2_approx) + both(1.f), rcp_approx); }
+
+template <typename T, int I, bool VEC>
+struct Gated {
+  static constexpr int kPieces = I * (int)sizeof(T), kStages = stages_of(kPieces);
+  static constexpr bool kAhead = VEC && kStages > 0;
+};
+template <typename T, int I, bool VEC>
+__global__ void __launch_bounds__(512) gated_rms_norm_kernel(const Norm p) {
+  using F = Gated<T, I, VEC>;
+  constexpr int kZ = I * (int)sizeof(T) / 2;
+  __shared__ float sums[64];
+  RowSum row_sum{sums, 0};
+  const Ahead<F::kPieces, F::kStages> ahead;
+  const int first = blockIdx.y * p.d;
+  const T *x0 = static_cast<const T*>(p.x) + first, *z0 = static_cast<const T*>(p.z) + first;
+  Eight w[I];
+  if constexpr (I == 1) w[0] = p.w.get<T, VEC>(first, 0, p.d);
+  for_rows<F::kAhead, F::kStages>(
+      p.rows,
+      [&](int s, int64_t row) {
+        ahead.template send<T, I>(s, 0, x0 + row * p.xs, p.d);
+        ahead.template send<T, I>(s, kZ, z0 + row * p.zs, p.d);
+      },
+      [&](int s, int64_t row) {
+        Eight v[I], z[I];
+        Pair ss = both(0.f);
+#pragma unroll
+        for (int it = 0; it < I; ++it) {
+          v[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(x0 + row * p.xs, it, p.d);
+          z[it] = F::kAhead ? ahead.template get<T>(s, kZ, it, p.d) : get8<T, VEC>(z0 + row * p.zs, it, p.d);
+          four([&](int e) {
+            z[it][e] = z[it][e] * sigmoid(z[it][e]);
+            if (!p.norm_first) v[it][e] = v[it][e] * z[it][e];
+            ss = fma(v[it][e], v[it][e], ss);
+          });
+        }
+        const float inv = inv_rms(row_sum(ss), p);
+        if (p.inv && threadIdx.x == 0) p.inv[row * p.groups + blockIdx.y] = inv;
+#pragma unroll
+        for (int it = 0; it < I; ++it) {
+          if constexpr (I > 1) w[it] = p.w.get<T, VEC>(first, it, p.d);
+          four([&](int e) {
+            v[it][e] = v[it][e] * both(inv) * w[it][e];
+            if (p.norm_first) v[it][e] = v[it][e] * z[it][e];
+          });
+          put8<T, VEC>(static_cast<T*>(p.y) + row * p.ys + first, it, p.d, v[it]);
+        }
+      });
 }
 
 template <typename T, int I, bool VEC>
-__global__ void __launch_bounds__(I == 1 ? 256 : 512) gated_rms_norm_kernel(const Norm p) {
-  __shared__ float sums[64];
-  RowSum row_sum{sums, 0};
-  const int first = blockIdx.y * p.d;
-  for_rows(p, [&](int64_t row) {
-    float v[I][8], z[I][8];
-#pragma unroll
-    for (int it = 0; it < I; ++it) {
-      get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs + first, it, p.d, v[it]);
-      get8<T, VEC>(static_cast<const T*>(p.z) + row * p.zs + first, it, p.d, z[it]);
-    }
-    float ss = 0.f;
-#pragma unroll
-    for (int it = 0; it < I; ++it)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        z[it][e] *= sigmoid_approx(z[it][e]);
-        if (!p.norm_first) v[it][e] *= z[it][e];
-        ss = fmaf(v[it][e], v[it][e], ss);
-      }
-    const float inv = rsqrtf(row_sum(ss) / p.d + p.eps);
-    if (p.inv && threadIdx.x == 0) p.inv[row * p.groups + blockIdx.y] = inv;
-#pragma unroll
-    for (int it = 0; it < I; ++it) {
-      float w[8];
-      p.w.get<T, VEC>(first, it, p.d, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        v[it][e] *= inv * w[e];
-        if (p.norm_first) v[it][e] *= z[it][e];
-      }
-      put8<T, VEC>(static_cast<T*>(p.y) + row * p.ys + first, it, p.d, v[it]);
-    }
-  });
-}
-
+struct GatedBackward {
+  static constexpr int kPieces = I * 3 * (int)sizeof(T) / 2, kStages = stages_of(kPieces);
+  static constexpr bool kAhead = VEC && kStages > 0;
+};
 template <typename T, int I, bool VEC>
-__global__ void __launch_bounds__(I == 1 ? 256 : 512) gated_rms_norm_grad_kernel(const Norm p) {
+__global__ void __launch_bounds__(512) gated_rms_norm_grad_kernel(const Norm p) {
+  using F = GatedBackward<T, I, VEC>;
+  constexpr int kZ = I * (int)sizeof(T) / 2, kG = 2 * kZ;
   __shared__ float sums[64];
   RowSum row_sum{sums, 0};
+  const Ahead<F::kPieces, F::kStages> ahead;
   const int first = blockIdx.y * p.d;
-  float dw[I][8] = {};
-  for_rows(p, [&](int64_t row) {
-    float x[I][8], z[I][8], g[I][8];
-    const float inv = p.inv[row * p.groups + blockIdx.y];
+  const T *x0 = static_cast<const T*>(p.x) + first, *z0 = static_cast<const T*>(p.z) + first, *g0 = static_cast<const T*>(p.dy) + first;
+  Eight dw[I], w[I];
 #pragma unroll
-    for (int it = 0; it < I; ++it) {
-      get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs + first, it, p.d, x[it]);
-      get8<T, VEC>(static_cast<const T*>(p.z) + row * p.zs + first, it, p.d, z[it]);
-      get8<T, VEC>(static_cast<const T*>(p.dy) + row * p.dys + first, it, p.d, g[it]);
-    }
-    float c = 0.f;
+  for (int it = 0; it < I; ++it) {
+    four([&](int e) { dw[it][e] = both(0.f); });
+    if constexpr (I == 1) w[it] = p.w.get<T, VEC>(first, it, p.d);
+  }
+  const Pair one = both(1.f), minus = both(-1.f);
+  for_rows<F::kAhead, F::kStages>(
+      p.rows,
+      [&](int s, int64_t row) {
+        ahead.template send<T, I>(s, 0, x0 + row * p.xs, p.d);
+        ahead.template send<T, I>(s, kZ, z0 + row * p.zs, p.d);
+        ahead.template send<T, I>(s, kG, g0 + row * p.dys, p.d);
+      },
+      [&](int s, int64_t row) {
+        Eight x[I], z[I], g[I], sg[I];
+        const float inv = p.inv[row * p.groups + blockIdx.y];
+        Pair c = both(0.f);
 #pragma unroll
-    for (int it = 0; it < I; ++it) {
-      float w[8];
-      p.w.get<T, VEC>(first, it, p.d, w);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float gate = z[it][e] * sigmoid_approx(z[it][e]);
-        const float vh = inv * (p.norm_first ? x[it][e] : x[it][e] * gate);
-        if (p.norm_first) {
-          dw[it][e] = fmaf(g[it][e] * gate, vh, dw[it][e]);
-          c = fmaf(g[it][e] * gate * w[e], vh, c);
-        } else {
-          dw[it][e] = fmaf(g[it][e], vh, dw[it][e]);
-          c = fmaf(g[it][e] * w[e], vh, c);
+        for (int it = 0; it < I; ++it) {
+          x[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(x0 + row * p.xs, it, p.d);
+          z[it] = F::kAhead ? ahead.template get<T>(s, kZ, it, p.d) : get8<T, VEC>(z0 + row * p.zs, it, p.d);
+          g[it] = F::kAhead ? ahead.template get<T>(s, kG, it, p.d) : get8<T, VEC>(g0 + row * p.dys, it, p.d);
+          if constexpr (I > 1) w[it] = p.w.get<T, VEC>(first, it, p.d);
+          four([&](int e) {
+            sg[it][e] = sigmoid(z[it][e]);
+            const Pair gate = z[it][e] * sg[it][e];
+            if (p.norm_first) {
+              x[it][e] = x[it][e] * both(inv);      // the normalised row
+              dw[it][e] = fma(g[it][e] * gate, x[it][e], dw[it][e]);
+              g[it][e] = g[it][e] * w[it][e];
+              c = fma(g[it][e] * gate, x[it][e], c);
+            } else {
+              const Pair vh = x[it][e] * gate * both(inv);
+              dw[it][e] = fma(g[it][e], vh, dw[it][e]);
+              g[it][e] = g[it][e] * w[it][e];
+              c = fma(g[it][e], vh, c);
+            }
+          });
         }
-        g[it][e] *= w[e];
-      }
-    }
-    c = row_sum(c) / p.d;
+        const Pair mean = both(-row_sum(c) / p.d);
 #pragma unroll
-    for (int it = 0; it < I; ++it) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float s = sigmoid_approx(z[it][e]), gate = z[it][e] * s, slope = s * fmaf(z[it][e], 1.f - s, 1.f);
-        if (p.norm_first) {
-          const float vh = inv * x[it][e];
-          z[it][e] = g[it][e] * vh * slope;
-          x[it][e] = inv * fmaf(-vh, c, g[it][e] * gate);
-        } else {
-          const float dv = inv * fmaf(-inv * (x[it][e] * gate), c, g[it][e]);
-          z[it][e] = dv * x[it][e] * slope;
-          x[it][e] = dv * gate;
+        for (int it = 0; it < I; ++it) {
+          four([&](int e) {
+            const Pair sv = sg[it][e], gate = z[it][e] * sv, slope = sv * fma(z[it][e], fma(sv, minus, one), one);
+            if (p.norm_first) {
+              const Pair vh = x[it][e];
+              z[it][e] = g[it][e] * vh * slope;
+              x[it][e] = both(inv) * fma(vh, mean, g[it][e] * gate);
+            } else {
+              const Pair dv = both(inv) * fma(x[it][e] * gate * both(inv), mean, g[it][e]);
+              z[it][e] = dv * x[it][e] * slope;
+              x[it][e] = dv * gate;
+            }
+          });
+          put8<T, VEC>(static_cast<T*>(p.dx) + row * p.dxs + first, it, p.d, x[it]);
+          put8<T, VEC>(static_cast<T*>(p.dz) + row * p.dzs + first, it, p.d, z[it]);
         }
-      }
-      put8<T, VEC>(static_cast<T*>(p.dx) + row * p.dxs + first, it, p.d, x[it]);
-      put8<T, VEC>(static_cast<T*>(p.dz) + row * p.dzs + first, it, p.d, z[it]);
-    }
-  });
+      });
   leave<I, VEC>(p, 0, dw);
 }
 
@@ -385,19 +539,17 @@ struct FinishVectors {
 
 struct Shape {
   int threads, rows, steps;      // threads of a row, rows of a CTA, eights of a thread
-  unsigned grid;                 // CTAs a group
+  unsigned most;                 // CTAs a group, of a gradient: each leaves its sums over rows
 };
-// Eight numbers a thread up to 2 048 a row, sixteen up to 8 192, 32 beyond.  Rows of a warp go four to a CTA.  Gradients: as many CTAs as
-// stay on the chip, each with its sums over rows.
-Shape shape_of(int64_t rows, int d, int groups, bool grad) {
+// Eight numbers a thread up to 4 096 a row, sixteen up to 8 192, 32 beyond.  Rows of a warp go four to a CTA.
+Shape shape_of(int64_t rows, int d, int groups) {
   Shape s;
   const int eights = (d + 7) / 8;
-  s.steps = eights <= 256 ? 1 : eights <= 1024 ? 2 : 4;
+  s.steps = eights <= 512 ? 1 : eights <= 1024 ? 2 : 4;
   s.threads = ((eights + s.steps - 1) / s.steps + 31) / 32 * 32;
   s.rows = s.threads == 32 ? 4 : 1;
-  int64_t grid = (rows + s.rows - 1) / s.rows;
-  const int64_t most = grad ? std::max(1, 148 * std::max(1, 1024 / (s.threads * s.rows)) / groups) : 0x7fffffff;
-  s.grid = (unsigned)std::min(grid, most);
+  const int64_t an_sm = std::max(1, 1024 / (s.threads * s.rows));
+  s.most = (unsigned)std::min((rows + s.rows - 1) / s.rows, std::max<int64_t>(1, 148 * an_sm / groups));
   return s;
 }
 
@@ -422,11 +574,23 @@ int check(const SsdNormArgs* a, bool gated, bool grad) {
   return SSD_OK;
 }
 
+// How many CTAs of a kernel an SM holds: asked for once a thread, kernel, device and size (as long as no other one takes its place).
+struct Resident {
+  const void* kernel;
+  int device, threads, smem, an_sm;
+  bool is(const Resident& o) const { return kernel == o.kernel && device == o.device && threads == o.threads && smem == o.smem; }
+};
+Resident& resident(const Resident& r) {
+  static thread_local Resident known[128] = {};
+  return known[(reinterpret_cast<uintptr_t>(r.kernel) / 16 * 31 + (unsigned)r.device * 7 + (unsigned)r.threads + (unsigned)r.smem / 512) % 128];
+}
+
 template <typename T>
 struct Launch {
   Norm p = {};
   Shape s;
   bool vec = true;
+  unsigned grid = 0;
   cudaStream_t stream;
   Launch(const SsdNormArgs& a, bool gated, bool grad, cudaStream_t st) : stream(st) {
     p.rows = a.rows; p.groups = gated ? a.groups : 1; p.d = a.d / p.groups; p.eps = a.eps; p.norm_first = a.norm_first;
@@ -437,7 +601,7 @@ struct Launch {
       p.post = {a.post_weight, a.vectors_in_dtype & 2};
       p.scale = {a.scale, a.vectors_in_dtype & 4};
     }
-    s = shape_of(a.rows, p.d, p.groups, grad);
+    s = shape_of(a.rows, p.d, p.groups);
     const int R = a.residual_dtype == SSD_DTYPE_F32 ? 4 : 2;
     vec = p.d % 8 == 0;
     rows_of(a.x, a.x_stride, sizeof(T));
@@ -466,40 +630,72 @@ struct Launch {
   }
   void vector_of(const Vector& v) { vec = vec && reinterpret_cast<uintptr_t>(v.p) % 16 == 0; }
 
+  // As many CTAs as the chip holds at once, where there are rows for them (a gradient: and sums).
   template <typename K>
-  int go(K kernel) const {
+  int go(K kernel, int pieces, int stages) {
+    const size_t smem = vec ? (size_t)pieces * stages * s.threads * s.rows * 16 : 0;
+    int device = 0;
+    if (cudaGetDevice(&device) != cudaSuccess) return SSD_ERR_CUDA;
+    const Resident want = {reinterpret_cast<const void*>(kernel), device, s.threads * s.rows, (int)smem, 0};
+    Resident& known = resident(want);
+    if (!known.is(want)) {
+      int an_sm = 0;
+      // (the most there is, so that no later call's size takes it back)
+      if ((smem && cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, 226 << 10) != cudaSuccess) ||
+          cudaOccupancyMaxActiveBlocksPerMultiprocessor(&an_sm, kernel, want.threads, smem) != cudaSuccess || an_sm < 1)
+        return SSD_ERR_CUDA;
+      known = want;
+      known.an_sm = an_sm;
+    }
+    const int64_t all = (p.rows + s.rows - 1) / s.rows, fit = std::max(1, 148 * known.an_sm / p.groups);
+    grid = (unsigned)std::min<int64_t>(std::min(all, fit), p.part ? s.most : fit);
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(s.grid, (unsigned)p.groups);
+    cfg.gridDim = dim3(grid, (unsigned)p.groups);
     cfg.blockDim = dim3((unsigned)s.threads, (unsigned)s.rows);
+    cfg.dynamicSmemBytes = smem;
     cfg.stream = stream;
     return cudaLaunchKernelEx(&cfg, kernel, p) == cudaSuccess ? SSD_OK : SSD_ERR_CUDA;
   }
-  template <typename R>
-  int forward() const {
-    if (s.steps == 1) return go(vec ? rms_norm_kernel<T, R, 1, true> : rms_norm_kernel<T, R, 1, false>);
-    if (s.steps == 2) return go(vec ? rms_norm_kernel<T, R, 2, true> : rms_norm_kernel<T, R, 2, false>);
-    return go(vec ? rms_norm_kernel<T, R, 4, true> : rms_norm_kernel<T, R, 4, false>);
+  template <typename F>
+  int by_steps(F f) {
+    if (s.steps == 1) return f(std::integral_constant<int, 1>());
+    if (s.steps == 2) return f(std::integral_constant<int, 2>());
+    return f(std::integral_constant<int, 4>());
   }
   template <typename R, bool OUTER>
-  int backward() const {
-    if (s.steps == 1) return go(vec ? rms_norm_grad_kernel<T, R, 1, true, OUTER> : rms_norm_grad_kernel<T, R, 1, false, OUTER>);
-    if (s.steps == 2) return go(vec ? rms_norm_grad_kernel<T, R, 2, true, OUTER> : rms_norm_grad_kernel<T, R, 2, false, OUTER>);
-    return go(vec ? rms_norm_grad_kernel<T, R, 4, true, OUTER> : rms_norm_grad_kernel<T, R, 4, false, OUTER>);
+  int forward() {
+    return by_steps([&](auto i) {
+      constexpr int I = decltype(i)::value;
+      using F = Forward<T, R, I, true, OUTER>;
+      return go(vec ? rms_norm_kernel<T, R, I, true, OUTER> : rms_norm_kernel<T, R, I, false, OUTER>, F::kPieces, F::kStages);
+    });
   }
-  int gated() const {
-    if (s.steps == 1) return go(vec ? gated_rms_norm_kernel<T, 1, true> : gated_rms_norm_kernel<T, 1, false>);
-    if (s.steps == 2) return go(vec ? gated_rms_norm_kernel<T, 2, true> : gated_rms_norm_kernel<T, 2, false>);
-    return go(vec ? gated_rms_norm_kernel<T, 4, true> : gated_rms_norm_kernel<T, 4, false>);
+  template <typename R, bool OUTER>
+  int backward() {
+    return by_steps([&](auto i) {
+      constexpr int I = decltype(i)::value;
+      using F = Backward<T, R, I, true, OUTER>;
+      return go(vec ? rms_norm_grad_kernel<T, R, I, true, OUTER> : rms_norm_grad_kernel<T, R, I, false, OUTER>, F::kPieces, F::kStages);
+    });
   }
-  int gated_backward() const {
-    if (s.steps == 1) return go(vec ? gated_rms_norm_grad_kernel<T, 1, true> : gated_rms_norm_grad_kernel<T, 1, false>);
-    if (s.steps == 2) return go(vec ? gated_rms_norm_grad_kernel<T, 2, true> : gated_rms_norm_grad_kernel<T, 2, false>);
-    return go(vec ? gated_rms_norm_grad_kernel<T, 4, true> : gated_rms_norm_grad_kernel<T, 4, false>);
+  int gated() {
+    return by_steps([&](auto i) {
+      constexpr int I = decltype(i)::value;
+      using F = Gated<T, I, true>;
+      return go(vec ? gated_rms_norm_kernel<T, I, true> : gated_rms_norm_kernel<T, I, false>, F::kPieces, F::kStages);
+    });
+  }
+  int gated_backward() {
+    return by_steps([&](auto i) {
+      constexpr int I = decltype(i)::value;
+      using F = GatedBackward<T, I, true>;
+      return go(vec ? gated_rms_norm_grad_kernel<T, I, true> : gated_rms_norm_grad_kernel<T, I, false>, F::kPieces, F::kStages);
+    });
   }
   int vectors(const SsdNormArgs& a) const {
     if (!a.dweight && !a.dpost_weight && !a.dscale) return SSD_OK;
     const int all = a.d * p.vectors;
-    return launch_column_sum(p.part, (int64_t)s.grid * s.rows, all, all,
+    return launch_column_sum(p.part, (int64_t)grid * s.rows, all, all,
                              FinishVectors<T>{a.d, a.vectors_in_dtype, a.dweight, a.dpost_weight, a.dscale, a.post_weight, a.scale}, stream);
   }
 };
@@ -511,8 +707,8 @@ extern "C" size_t ssd_b200_norm_workspace_bytes(const SsdNormArgs* a) {
   if (!a || a->rows <= 0 || a->d <= 0) return 0;
   const int groups = a->z ? a->groups : 1;
   if (groups <= 0 || a->d % groups != 0 || a->d / groups > 16384) return 0;
-  const ssd::Shape s = ssd::shape_of(a->rows, a->d / groups, groups, true);
-  return (size_t)s.grid * s.rows * a->d * (!a->z && (a->post_weight || a->scale) ? 2 : 1) * sizeof(float);
+  const ssd::Shape s = ssd::shape_of(a->rows, a->d / groups, groups);
+  return (size_t)s.most * s.rows * a->d * (!a->z && (a->post_weight || a->scale) ? 2 : 1) * sizeof(float);
 }
 
 extern "C" int ssd_b200_rms_norm(const SsdNormArgs* args, void* stream) {
@@ -520,9 +716,11 @@ extern "C" int ssd_b200_rms_norm(const SsdNormArgs* args, void* stream) {
   const SsdNormArgs& a = *args;
   return ssd::by_type(a.dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const ssd::Launch<T> l(a, false, false, static_cast<cudaStream_t>(stream));
-    if (!a.residual || a.residual_dtype == a.dtype) return l.template forward<T>();
-    return a.residual_dtype == SSD_DTYPE_F32 ? l.template forward<float>() : (int)SSD_ERR_UNSUPPORTED;
+    ssd::Launch<T> l(a, false, false, static_cast<cudaStream_t>(stream));
+    const bool outer = a.post_weight || a.scale;
+    if (!a.residual || a.residual_dtype == a.dtype) return outer ? l.template forward<T, true>() : l.template forward<T, false>();
+    if (a.residual_dtype != SSD_DTYPE_F32) return (int)SSD_ERR_UNSUPPORTED;
+    return outer ? l.template forward<float, true>() : l.template forward<float, false>();
   });
 }
 
@@ -531,7 +729,7 @@ extern "C" int ssd_b200_rms_norm_backward(const SsdNormArgs* args, void* stream)
   const SsdNormArgs& a = *args;
   return ssd::by_type(a.dtype, [&](auto t) -> int {
     using T = decltype(t);
-    const ssd::Launch<T> l(a, false, true, static_cast<cudaStream_t>(stream));
+    ssd::Launch<T> l(a, false, true, static_cast<cudaStream_t>(stream));
     const bool outer = a.post_weight || a.scale;
     int rc = SSD_ERR_UNSUPPORTED;
     if (!a.residual_out || a.residual_dtype == a.dtype) rc = outer ? l.template backward<T, true>() : l.template backward<T, false>();
@@ -548,7 +746,7 @@ extern "C" int ssd_b200_gated_rms_norm(const SsdNormArgs* args, void* stream) {
 extern "C" int ssd_b200_gated_rms_norm_backward(const SsdNormArgs* args, void* stream) {
   if (const int rc = ssd::check(args, true, true)) return rc;
   return ssd::by_type(args->dtype, [&](auto t) -> int {
-    const ssd::Launch<decltype(t)> l(*args, true, true, static_cast<cudaStream_t>(stream));
+    ssd::Launch<decltype(t)> l(*args, true, true, static_cast<cudaStream_t>(stream));
     const int rc = l.gated_backward();
     return rc ? rc : l.vectors(*args);
   });
