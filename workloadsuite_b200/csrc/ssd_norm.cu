@@ -96,9 +96,10 @@ struct Vector {
   }
 };
 
-// Sum over the threads of a row, in all of them.  `turn` alternates between two places, so that one barrier a sum is enough.
+// Sum over the threads of a row, in all of them, in a fixed order.  `turn` alternates between two places, so that one barrier a sum is
+// enough.
 struct RowSum {
-  float* place;   // [2][32]
+  float (*place)[16];   // [2]: up to sixteen warps
   int turn;
   __device__ __forceinline__ float operator()(Pair s) {
     const float2 h = halves(s);
@@ -106,18 +107,46 @@ struct RowSum {
 #pragma unroll
     for (int k = 16; k > 0; k /= 2) v += __shfl_xor_sync(~0u, v, k);
     if (blockDim.x > 32) {
-      float* s = place + 32 * turn;
+      float* const at = place[turn];
       turn ^= 1;
-      const int lane = threadIdx.x % 32;
-      if (lane == 0) s[threadIdx.x / 32] = v;
+      if (threadIdx.x % 32 == 0) at[threadIdx.x / 32] = v;
       __syncthreads();
-      v = lane < (int)blockDim.x / 32 ? s[lane] : 0.f;
-#pragma unroll
-      for (int k = 16; k > 0; k /= 2) v += __shfl_xor_sync(~0u, v, k);
+      v = 0.f;
+      for (int w = 0; w < (int)blockDim.x / 32; w += 4) {   // (places of warps that are not there hold zero)
+        const float4 a = *reinterpret_cast<const float4*>(at + w);
+        v += (a.x + a.y) + (a.z + a.w);
+      }
     }
     return v;
   }
 };
+__device__ __forceinline__ void clear(float (&sums)[2][16]) {
+  const int t = threadIdx.y * blockDim.x + threadIdx.x;
+  if (t < 32) sums[t / 16][t % 16] = 0.f;
+  __syncthreads();
+}
+
+// One operand's rows, as a CTA goes through them.
+template <typename T>
+struct Rows {
+  T* at;
+  int64_t by;
+  __device__ __forceinline__ Rows(T* p, int64_t stride)
+      : at(p ? p + ((int64_t)blockIdx.x * blockDim.y + threadIdx.y) * stride : nullptr), by((int64_t)gridDim.x * blockDim.y * stride) {}
+  __device__ __forceinline__ T* next() {
+    T* const r = at;
+    at += by;
+    return r;
+  }
+};
+template <typename T>
+__device__ __forceinline__ Rows<const T> rows_in(const void* p, int64_t stride, int first = 0) {
+  return Rows<const T>(p ? static_cast<const T*>(p) + first : nullptr, stride);
+}
+template <typename T>
+__device__ __forceinline__ Rows<T> rows_out(void* p, int64_t stride, int first = 0) {
+  return Rows<T>(p ? static_cast<T*>(p) + first : nullptr, stride);
+}
 
 struct Norm {
   const void *x, *z, *res, *dy, *dres_out;
@@ -177,29 +206,29 @@ struct Ahead {
     return widen<T>(a, b);
   }
 };
-// Rows ahead: as many as shared memory holds for the widest CTA (512 threads), up to four; where that is not even two (fp32 beyond 4 096
-// numbers, 16-bit beyond 8 192) rows are read where they are needed.
+// Rows ahead: fewer of large rows, as CTAs that do not fit cost more than a row ahead; where the widest CTA (512 threads) does not hold
+// two, rows are read where they are needed.
 constexpr int stages_of(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 3 : pieces <= 13 ? 2 : 0; }
 
-// Goes through a CTA's rows (a row per warp, blockDim.y of them, or one per CTA): send(stage, row) asks for a row's inputs,
-// work(stage, row) takes them.
+// Goes through a CTA's rows (a row per warp, blockDim.y of them, or one per CTA): send(stage) asks for the next row's inputs, work(stage, row)
+// takes them.
 template <bool AHEAD, int STAGES, typename Send, typename Work>
 __device__ __forceinline__ void for_rows(int64_t rows, Send send, Work work) {
   const int64_t step = (int64_t)gridDim.x * blockDim.y;
-  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y, ahead = row;
+  auto ask = [&](int stage) {
+    if (ahead < rows) send(stage);
+    ahead += step;
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
   if constexpr (AHEAD) {
 #pragma unroll
-    for (int s = 0; s < STAGES - 1; ++s) {
-      if (row + s * step < rows) send(s, row + s * step);
-      asm volatile("cp.async.commit_group;" ::: "memory");
-    }
+    for (int s = 0; s < STAGES - 1; ++s) ask(s);
   }
   int stage = 0;
   for (; row < rows; row += step) {
     if constexpr (AHEAD) {
-      const int64_t next = row + (STAGES - 1) * step;
-      if (next < rows) send(stage == 0 ? STAGES - 1 : stage - 1, next);
-      asm volatile("cp.async.commit_group;" ::: "memory");
+      ask(stage == 0 ? STAGES - 1 : stage - 1);
       asm volatile("cp.async.wait_group %0;" ::"n"(STAGES - 1) : "memory");
     }
     work(stage, row);
@@ -212,15 +241,18 @@ __device__ __forceinline__ float inv_rms(float sum, const Norm& p) { return rsqr
 // OUTER: with post_weight or scale.
 template <typename T, typename R, int I, bool VEC, bool OUTER>
 struct Forward {
-  static constexpr int kPieces = I * (int)(sizeof(T) + sizeof(R)) / 2, kStages = stages_of(kPieces);
+  // Two sums a row (OUTER): what counts is how many rows an SM has in hand, and rows ahead take the room of CTAs (2 560 numbers, fp32
+  // residual: 50 us for 8 192 rows without, 56 with).  One sum: 52 and 52 at 2 048, 91 and 98 at 8 192.
+  static constexpr int kPieces = I * (int)(sizeof(T) + sizeof(R)) / 2, kStages = OUTER ? 0 : stages_of(kPieces);
   static constexpr bool kAhead = VEC && kStages > 0;
-  static constexpr bool kKeep = I == 1;   // vectors stay in registers
+  static constexpr bool kKeep = I <= 2 && !OUTER;   // vectors stay in registers
 };
 template <typename T, typename R, int I, bool VEC, bool OUTER>
-__global__ void __launch_bounds__(512) rms_norm_kernel(const Norm p) {
+__global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_kernel(const Norm p) {
   using F = Forward<T, R, I, VEC, OUTER>;
   constexpr int kRes = I * (int)sizeof(T) / 2;
-  __shared__ float sums[64];
+  __shared__ __align__(16) float sums[2][16];
+  clear(sums);
   RowSum row_sum{sums, 0};
   const Ahead<F::kPieces, F::kStages> ahead;
   Eight w[I], ps[I];
@@ -231,17 +263,21 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const Norm p) {
       if constexpr (OUTER) ps[it] = p.outer<T, VEC>(it);
     }
   }
+  auto x = rows_in<T>(p.x, p.xs);
+  auto res = rows_in<R>(p.res, p.rs);
+  auto res_out = rows_out<R>(p.res_out, p.ros);
+  auto y = rows_out<T>(p.y, p.ys);
   for_rows<F::kAhead, F::kStages>(
       p.rows,
-      [&](int s, int64_t row) {
-        ahead.template send<T, I>(s, 0, static_cast<const T*>(p.x) + row * p.xs, p.d);
-        if (p.res) ahead.template send<R, I>(s, kRes, static_cast<const R*>(p.res) + row * p.rs, p.d);
+      [&](int s) {
+        ahead.template send<T, I>(s, 0, x.next(), p.d);
+        if (p.res) ahead.template send<R, I>(s, kRes, res.next(), p.d);
       },
       [&](int s, int64_t row) {
         Eight v[I];
+        const T* const xr = F::kAhead ? nullptr : x.next();
 #pragma unroll
-        for (int it = 0; it < I; ++it)
-          v[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d);
+        for (int it = 0; it < I; ++it) v[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(xr, it, p.d);
         if constexpr (OUTER) {
           float inv = 1.f;
           if (p.post.p) {
@@ -258,14 +294,16 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const Norm p) {
           }
         }
         if (p.res) {
+          const R* const rr = F::kAhead ? nullptr : res.next();
+          R* const ro = res_out.next();
 #pragma unroll
           for (int it = 0; it < I; ++it) {
-            const Eight old = F::kAhead ? ahead.template get<R>(s, kRes, it, p.d) : get8<R, VEC>(static_cast<const R*>(p.res) + row * p.rs, it, p.d);
+            const Eight old = F::kAhead ? ahead.template get<R>(s, kRes, it, p.d) : get8<R, VEC>(rr, it, p.d);
             four([&](int e) {   // as it is stored
               const float2 f = halves(old[e] + v[it][e]);
               v[it][e] = pair_of<R>(Two<R>::down(f.x, f.y));
             });
-            put8<R, VEC>(static_cast<R*>(p.res_out) + row * p.ros, it, p.d, v[it]);
+            put8<R, VEC>(ro, it, p.d, v[it]);
           }
         }
         Pair ss = both(0.f);
@@ -273,11 +311,12 @@ __global__ void __launch_bounds__(512) rms_norm_kernel(const Norm p) {
         for (int it = 0; it < I; ++it) four([&](int e) { ss = fma(v[it][e], v[it][e], ss); });
         const float inv = inv_rms(row_sum(ss), p);
         if (p.inv && threadIdx.x == 0) p.inv[row] = inv;
+        T* const yr = y.next();
 #pragma unroll
         for (int it = 0; it < I; ++it) {
           if constexpr (!F::kKeep) w[it] = p.w.get<T, VEC>(0, it, p.d);
           four([&](int e) { v[it][e] = v[it][e] * both(inv) * w[it][e]; });
-          put8<T, VEC>(static_cast<T*>(p.y) + row * p.ys, it, p.d, v[it]);
+          put8<T, VEC>(yr, it, p.d, v[it]);
         }
       });
 }
@@ -300,13 +339,14 @@ template <typename T, typename R, int I, bool VEC, bool OUTER>
 struct Backward {
   static constexpr int kPieces = I * (int)(sizeof(T) + 2 * sizeof(R) + (OUTER ? sizeof(T) : 0)) / 2, kStages = stages_of(kPieces);
   static constexpr bool kAhead = VEC && kStages > 0;
-  static constexpr bool kKeep = I == 1;
+  static constexpr bool kKeep = I <= 2;
 };
 template <typename T, typename R, int I, bool VEC, bool OUTER>
-__global__ void __launch_bounds__(512) rms_norm_grad_kernel(const Norm p) {
+__global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_grad_kernel(const Norm p) {
   using F = Backward<T, R, I, VEC, OUTER>;
   constexpr int kOut = I * (int)sizeof(T) / 2, kIn = kOut + I * (int)sizeof(R) / 2, kX = kIn + I * (int)sizeof(R) / 2;
-  __shared__ float sums[64];
+  __shared__ __align__(16) float sums[2][16];
+  clear(sums);
   RowSum row_sum{sums, 0};
   const Ahead<F::kPieces, F::kStages> ahead;
   Eight dw[I], acc[I], w[I], ps[I];
@@ -318,17 +358,24 @@ __global__ void __launch_bounds__(512) rms_norm_grad_kernel(const Norm p) {
       if constexpr (OUTER) ps[it] = p.outer<T, VEC>(it);
     }
   }
+  auto dy = rows_in<T>(p.dy, p.dys), x = rows_in<T>(p.x, p.xs);
+  auto of = p.res_out ? rows_in<R>(p.res_out, p.ros) : rows_in<R>(p.x, p.xs);   // (of x: R is T)
+  auto dres_out = rows_in<R>(p.dres_out, p.dros);
+  auto dres = rows_out<R>(p.dres, p.drs);
+  auto dx = rows_out<T>(p.dx, p.dxs);
   for_rows<F::kAhead, F::kStages>(
       p.rows,
-      [&](int s, int64_t row) {
-        ahead.template send<T, I>(s, 0, static_cast<const T*>(p.dy) + row * p.dys, p.d);
-        if (p.res_out) ahead.template send<R, I>(s, kOut, static_cast<const R*>(p.res_out) + row * p.ros, p.d);
-        else ahead.template send<T, I>(s, kOut, static_cast<const T*>(p.x) + row * p.xs, p.d);   // (R is T)
-        if (p.dres_out) ahead.template send<R, I>(s, kIn, static_cast<const R*>(p.dres_out) + row * p.dros, p.d);
-        if constexpr (OUTER) ahead.template send<T, I>(s, kX, static_cast<const T*>(p.x) + row * p.xs, p.d);
+      [&](int s) {
+        ahead.template send<T, I>(s, 0, dy.next(), p.d);
+        ahead.template send<R, I>(s, kOut, of.next(), p.d);
+        if (p.dres_out) ahead.template send<R, I>(s, kIn, dres_out.next(), p.d);
+        if constexpr (OUTER) ahead.template send<T, I>(s, kX, x.next(), p.d);
       },
       [&](int s, int64_t row) {
         Eight g[I], v[I];
+        const T* const gr = F::kAhead ? nullptr : dy.next();
+        const R *const vr = F::kAhead ? nullptr : of.next(), *const ir = F::kAhead ? nullptr : dres_out.next();
+        const T* const xr = F::kAhead ? nullptr : x.next();
         const float inv = p.inv[row], invp = OUTER && p.post.p ? p.inv_post[row] : 1.f;
         Pair c = both(0.f);
 #pragma unroll
@@ -337,9 +384,8 @@ __global__ void __launch_bounds__(512) rms_norm_grad_kernel(const Norm p) {
             g[it] = ahead.template get<T>(s, 0, it, p.d);
             v[it] = ahead.template get<R>(s, kOut, it, p.d);
           } else {
-            g[it] = get8<T, VEC>(static_cast<const T*>(p.dy) + row * p.dys, it, p.d);
-            if (p.res_out) v[it] = get8<R, VEC>(static_cast<const R*>(p.res_out) + row * p.ros, it, p.d);
-            else v[it] = get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d);
+            g[it] = get8<T, VEC>(gr, it, p.d);
+            v[it] = get8<R, VEC>(vr, it, p.d);
           }
           if constexpr (!F::kKeep) w[it] = p.w.get<T, VEC>(0, it, p.d);
           four([&](int e) {
@@ -350,20 +396,21 @@ __global__ void __launch_bounds__(512) rms_norm_grad_kernel(const Norm p) {
           });
         }
         const Pair mean = both(-row_sum(c) / p.d);
+        R* const dres_at = p.dres ? dres.next() : nullptr;
 #pragma unroll
         for (int it = 0; it < I; ++it) {
           four([&](int e) { g[it][e] = both(inv) * fma(v[it][e], mean, g[it][e]); });
           if (p.dres_out) {
-            const Eight in = F::kAhead ? ahead.template get<R>(s, kIn, it, p.d) : get8<R, VEC>(static_cast<const R*>(p.dres_out) + row * p.dros, it, p.d);
+            const Eight in = F::kAhead ? ahead.template get<R>(s, kIn, it, p.d) : get8<R, VEC>(ir, it, p.d);
             four([&](int e) { g[it][e] = g[it][e] + in[e]; });
           }
-          if (p.dres) put8<R, VEC>(static_cast<R*>(p.dres) + row * p.drs, it, p.d, g[it]);
+          if (p.dres) put8<R, VEC>(dres_at, it, p.d, g[it]);
         }
         if constexpr (OUTER) {
           Pair c2 = both(0.f);
 #pragma unroll
           for (int it = 0; it < I; ++it) {
-            v[it] = F::kAhead ? ahead.template get<T>(s, kX, it, p.d) : get8<T, VEC>(static_cast<const T*>(p.x) + row * p.xs, it, p.d);
+            v[it] = F::kAhead ? ahead.template get<T>(s, kX, it, p.d) : get8<T, VEC>(xr, it, p.d);
             if constexpr (!F::kKeep) ps[it] = p.outer<T, VEC>(it);
             four([&](int e) {
               v[it][e] = v[it][e] * both(invp);
@@ -378,8 +425,9 @@ __global__ void __launch_bounds__(512) rms_norm_grad_kernel(const Norm p) {
             for (int it = 0; it < I; ++it) four([&](int e) { g[it][e] = both(invp) * fma(v[it][e], mean2, g[it][e]); });
           }
         }
+        T* const dxr = dx.next();
 #pragma unroll
-        for (int it = 0; it < I; ++it) put8<T, VEC>(static_cast<T*>(p.dx) + row * p.dxs, it, p.d, g[it]);
+        for (int it = 0; it < I; ++it) put8<T, VEC>(dxr, it, p.d, g[it]);
       });
   leave<I, VEC>(p, 0, dw);
   if constexpr (OUTER) leave<I, VEC>(p, 1, acc);
@@ -393,45 +441,52 @@ struct Gated {
   static constexpr bool kAhead = VEC && kStages > 0;
 };
 template <typename T, int I, bool VEC>
-__global__ void __launch_bounds__(512) gated_rms_norm_kernel(const Norm p) {
+__global__ void __launch_bounds__(I == 1 ? 128 : 512) gated_rms_norm_kernel(const Norm p) {
   using F = Gated<T, I, VEC>;
   constexpr int kZ = I * (int)sizeof(T) / 2;
-  __shared__ float sums[64];
+  __shared__ __align__(16) float sums[2][16];
+  clear(sums);
   RowSum row_sum{sums, 0};
   const Ahead<F::kPieces, F::kStages> ahead;
   const int first = blockIdx.y * p.d;
-  const T *x0 = static_cast<const T*>(p.x) + first, *z0 = static_cast<const T*>(p.z) + first;
+  auto x = rows_in<T>(p.x, p.xs, first), z = rows_in<T>(p.z, p.zs, first);
+  auto y = rows_out<T>(p.y, p.ys, first);
   Eight w[I];
-  if constexpr (I == 1) w[0] = p.w.get<T, VEC>(first, 0, p.d);
+  if constexpr (I <= 2) {
+#pragma unroll
+    for (int it = 0; it < I; ++it) w[it] = p.w.get<T, VEC>(first, it, p.d);
+  }
   for_rows<F::kAhead, F::kStages>(
       p.rows,
-      [&](int s, int64_t row) {
-        ahead.template send<T, I>(s, 0, x0 + row * p.xs, p.d);
-        ahead.template send<T, I>(s, kZ, z0 + row * p.zs, p.d);
+      [&](int s) {
+        ahead.template send<T, I>(s, 0, x.next(), p.d);
+        ahead.template send<T, I>(s, kZ, z.next(), p.d);
       },
       [&](int s, int64_t row) {
-        Eight v[I], z[I];
+        Eight v[I], g[I];
+        const T *const xr = F::kAhead ? nullptr : x.next(), *const zr = F::kAhead ? nullptr : z.next();
         Pair ss = both(0.f);
 #pragma unroll
         for (int it = 0; it < I; ++it) {
-          v[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(x0 + row * p.xs, it, p.d);
-          z[it] = F::kAhead ? ahead.template get<T>(s, kZ, it, p.d) : get8<T, VEC>(z0 + row * p.zs, it, p.d);
+          v[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(xr, it, p.d);
+          g[it] = F::kAhead ? ahead.template get<T>(s, kZ, it, p.d) : get8<T, VEC>(zr, it, p.d);
           four([&](int e) {
-            z[it][e] = z[it][e] * sigmoid(z[it][e]);
-            if (!p.norm_first) v[it][e] = v[it][e] * z[it][e];
+            g[it][e] = g[it][e] * sigmoid(g[it][e]);
+            if (!p.norm_first) v[it][e] = v[it][e] * g[it][e];
             ss = fma(v[it][e], v[it][e], ss);
           });
         }
         const float inv = inv_rms(row_sum(ss), p);
         if (p.inv && threadIdx.x == 0) p.inv[row * p.groups + blockIdx.y] = inv;
+        T* const yr = y.next();
 #pragma unroll
         for (int it = 0; it < I; ++it) {
-          if constexpr (I > 1) w[it] = p.w.get<T, VEC>(first, it, p.d);
+          if constexpr (I > 2) w[it] = p.w.get<T, VEC>(first, it, p.d);
           four([&](int e) {
             v[it][e] = v[it][e] * both(inv) * w[it][e];
-            if (p.norm_first) v[it][e] = v[it][e] * z[it][e];
+            if (p.norm_first) v[it][e] = v[it][e] * g[it][e];
           });
-          put8<T, VEC>(static_cast<T*>(p.y) + row * p.ys + first, it, p.d, v[it]);
+          put8<T, VEC>(yr, it, p.d, v[it]);
         }
       });
 }
@@ -442,38 +497,41 @@ struct GatedBackward {
   static constexpr bool kAhead = VEC && kStages > 0;
 };
 template <typename T, int I, bool VEC>
-__global__ void __launch_bounds__(512) gated_rms_norm_grad_kernel(const Norm p) {
+__global__ void __launch_bounds__(I == 1 ? 128 : 512) gated_rms_norm_grad_kernel(const Norm p) {
   using F = GatedBackward<T, I, VEC>;
   constexpr int kZ = I * (int)sizeof(T) / 2, kG = 2 * kZ;
-  __shared__ float sums[64];
+  __shared__ __align__(16) float sums[2][16];
+  clear(sums);
   RowSum row_sum{sums, 0};
   const Ahead<F::kPieces, F::kStages> ahead;
   const int first = blockIdx.y * p.d;
-  const T *x0 = static_cast<const T*>(p.x) + first, *z0 = static_cast<const T*>(p.z) + first, *g0 = static_cast<const T*>(p.dy) + first;
+  auto xs = rows_in<T>(p.x, p.xs, first), zs = rows_in<T>(p.z, p.zs, first), gs = rows_in<T>(p.dy, p.dys, first);
+  auto dx = rows_out<T>(p.dx, p.dxs, first), dz = rows_out<T>(p.dz, p.dzs, first);
   Eight dw[I], w[I];
 #pragma unroll
   for (int it = 0; it < I; ++it) {
     four([&](int e) { dw[it][e] = both(0.f); });
-    if constexpr (I == 1) w[it] = p.w.get<T, VEC>(first, it, p.d);
+    if constexpr (I <= 2) w[it] = p.w.get<T, VEC>(first, it, p.d);
   }
   const Pair one = both(1.f), minus = both(-1.f);
   for_rows<F::kAhead, F::kStages>(
       p.rows,
-      [&](int s, int64_t row) {
-        ahead.template send<T, I>(s, 0, x0 + row * p.xs, p.d);
-        ahead.template send<T, I>(s, kZ, z0 + row * p.zs, p.d);
-        ahead.template send<T, I>(s, kG, g0 + row * p.dys, p.d);
+      [&](int s) {
+        ahead.template send<T, I>(s, 0, xs.next(), p.d);
+        ahead.template send<T, I>(s, kZ, zs.next(), p.d);
+        ahead.template send<T, I>(s, kG, gs.next(), p.d);
       },
       [&](int s, int64_t row) {
         Eight x[I], z[I], g[I], sg[I];
+        const T *const xr = F::kAhead ? nullptr : xs.next(), *const zr = F::kAhead ? nullptr : zs.next(), *const gr = F::kAhead ? nullptr : gs.next();
         const float inv = p.inv[row * p.groups + blockIdx.y];
         Pair c = both(0.f);
 #pragma unroll
         for (int it = 0; it < I; ++it) {
-          x[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(x0 + row * p.xs, it, p.d);
-          z[it] = F::kAhead ? ahead.template get<T>(s, kZ, it, p.d) : get8<T, VEC>(z0 + row * p.zs, it, p.d);
-          g[it] = F::kAhead ? ahead.template get<T>(s, kG, it, p.d) : get8<T, VEC>(g0 + row * p.dys, it, p.d);
-          if constexpr (I > 1) w[it] = p.w.get<T, VEC>(first, it, p.d);
+          x[it] = F::kAhead ? ahead.template get<T>(s, 0, it, p.d) : get8<T, VEC>(xr, it, p.d);
+          z[it] = F::kAhead ? ahead.template get<T>(s, kZ, it, p.d) : get8<T, VEC>(zr, it, p.d);
+          g[it] = F::kAhead ? ahead.template get<T>(s, kG, it, p.d) : get8<T, VEC>(gr, it, p.d);
+          if constexpr (I > 2) w[it] = p.w.get<T, VEC>(first, it, p.d);
           four([&](int e) {
             sg[it][e] = sigmoid(z[it][e]);
             const Pair gate = z[it][e] * sg[it][e];
@@ -491,6 +549,7 @@ __global__ void __launch_bounds__(512) gated_rms_norm_grad_kernel(const Norm p) 
           });
         }
         const Pair mean = both(-row_sum(c) / p.d);
+        T *const dxr = dx.next(), *const dzr = dz.next();
 #pragma unroll
         for (int it = 0; it < I; ++it) {
           four([&](int e) {
@@ -505,8 +564,8 @@ __global__ void __launch_bounds__(512) gated_rms_norm_grad_kernel(const Norm p) 
               x[it][e] = dv * gate;
             }
           });
-          put8<T, VEC>(static_cast<T*>(p.dx) + row * p.dxs + first, it, p.d, x[it]);
-          put8<T, VEC>(static_cast<T*>(p.dz) + row * p.dzs + first, it, p.d, z[it]);
+          put8<T, VEC>(dxr, it, p.d, x[it]);
+          put8<T, VEC>(dzr, it, p.d, z[it]);
         }
       });
   leave<I, VEC>(p, 0, dw);
@@ -541,11 +600,11 @@ struct Shape {
   int threads, rows, steps;      // threads of a row, rows of a CTA, eights of a thread
   unsigned most;                 // CTAs a group, of a gradient: each leaves its sums over rows
 };
-// Eight numbers a thread up to 4 096 a row, sixteen up to 8 192, 32 beyond.  Rows of a warp go four to a CTA.
-Shape shape_of(int64_t rows, int d, int groups) {
+// Eight numbers a thread up to 1 024 a row, then sixteen, from 4 096 (a gradient: 8 192) on 32.  Rows of a warp go four to a CTA.
+Shape shape_of(int64_t rows, int d, int groups, bool grad) {
   Shape s;
   const int eights = (d + 7) / 8;
-  s.steps = eights <= 512 ? 1 : eights <= 1024 ? 2 : 4;
+  s.steps = eights <= 128 ? 1 : eights <= (grad ? 1024 : 512) ? 2 : 4;
   s.threads = ((eights + s.steps - 1) / s.steps + 31) / 32 * 32;
   s.rows = s.threads == 32 ? 4 : 1;
   const int64_t an_sm = std::max(1, 1024 / (s.threads * s.rows));
@@ -601,7 +660,7 @@ struct Launch {
       p.post = {a.post_weight, a.vectors_in_dtype & 2};
       p.scale = {a.scale, a.vectors_in_dtype & 4};
     }
-    s = shape_of(a.rows, p.d, p.groups);
+    s = shape_of(a.rows, p.d, p.groups, grad);
     const int R = a.residual_dtype == SSD_DTYPE_F32 ? 4 : 2;
     vec = p.d % 8 == 0;
     rows_of(a.x, a.x_stride, sizeof(T));
@@ -707,7 +766,7 @@ extern "C" size_t ssd_b200_norm_workspace_bytes(const SsdNormArgs* a) {
   if (!a || a->rows <= 0 || a->d <= 0) return 0;
   const int groups = a->z ? a->groups : 1;
   if (groups <= 0 || a->d % groups != 0 || a->d / groups > 16384) return 0;
-  const ssd::Shape s = ssd::shape_of(a->rows, a->d / groups, groups);
+  const ssd::Shape s = ssd::shape_of(a->rows, a->d / groups, groups, true);
   return (size_t)s.most * s.rows * a->d * (!a->z && (a->post_weight || a->scale) ? 2 : 1) * sizeof(float);
 }
 
