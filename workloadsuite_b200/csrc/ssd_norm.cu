@@ -155,7 +155,7 @@ struct Norm {
   float *inv, *inv_post, *part;
   int64_t rows, xs, zs, rs, ys, ros, dys, dros, dxs, dzs, drs;
   int d, groups, norm_first, vectors;   // d: of a group; vectors: of d * groups partial sums a row of `part` holds
-  float eps;
+  float eps, inv_d;
   // what the norm behind the block and the scale multiply by
   template <typename T, bool VEC>
   __device__ __forceinline__ Eight outer(int it) const {
@@ -236,7 +236,7 @@ __device__ __forceinline__ void for_rows(int64_t rows, Send send, Work work) {
   }
   if constexpr (AHEAD) asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
-__device__ __forceinline__ float inv_rms(float sum, const Norm& p) { return rsqrtf(sum / p.d + p.eps); }
+__device__ __forceinline__ float inv_rms(float sum, const Norm& p) { return rsqrtf(fmaf(sum, p.inv_d, p.eps)); }
 
 // OUTER: with post_weight or scale.
 template <typename T, typename R, int I, bool VEC, bool OUTER>
@@ -363,6 +363,13 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_grad_kernel(const
   auto dres_out = rows_in<R>(p.dres_out, p.dros);
   auto dres = rows_out<R>(p.dres, p.drs);
   auto dx = rows_out<T>(p.dx, p.dxs);
+  float inv_now = 0.f, inv_post_now = 1.f;   // the next row's, asked for a row ahead
+  auto rates = [&](int64_t row) {
+    if (row >= p.rows) return;
+    inv_now = p.inv[row];
+    if (OUTER && p.post.p) inv_post_now = p.inv_post[row];
+  };
+  rates((int64_t)blockIdx.x * blockDim.y + threadIdx.y);
   for_rows<F::kAhead, F::kStages>(
       p.rows,
       [&](int s) {
@@ -376,7 +383,8 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_grad_kernel(const
         const T* const gr = F::kAhead ? nullptr : dy.next();
         const R *const vr = F::kAhead ? nullptr : of.next(), *const ir = F::kAhead ? nullptr : dres_out.next();
         const T* const xr = F::kAhead ? nullptr : x.next();
-        const float inv = p.inv[row], invp = OUTER && p.post.p ? p.inv_post[row] : 1.f;
+        const float inv = inv_now, invp = inv_post_now;
+        rates(row + (int64_t)gridDim.x * blockDim.y);
         Pair c = both(0.f);
 #pragma unroll
         for (int it = 0; it < I; ++it) {
@@ -395,7 +403,7 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_grad_kernel(const
             c = fma(g[it][e], v[it][e], c);
           });
         }
-        const Pair mean = both(-row_sum(c) / p.d);
+        const Pair mean = both(-row_sum(c) * p.inv_d);
         R* const dres_at = p.dres ? dres.next() : nullptr;
 #pragma unroll
         for (int it = 0; it < I; ++it) {
@@ -420,7 +428,7 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_grad_kernel(const
             });
           }
           if (p.post.p) {
-            const Pair mean2 = both(-row_sum(c2) / p.d);
+            const Pair mean2 = both(-row_sum(c2) * p.inv_d);
 #pragma unroll
             for (int it = 0; it < I; ++it) four([&](int e) { g[it][e] = both(invp) * fma(v[it][e], mean2, g[it][e]); });
           }
@@ -514,6 +522,11 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) gated_rms_norm_grad_kernel
     if constexpr (I <= 2) w[it] = p.w.get<T, VEC>(first, it, p.d);
   }
   const Pair one = both(1.f), minus = both(-1.f);
+  float inv_now = 0.f;   // the next row's, asked for a row ahead
+  auto rate = [&](int64_t row) {
+    if (row < p.rows) inv_now = p.inv[row * p.groups + blockIdx.y];
+  };
+  rate((int64_t)blockIdx.x * blockDim.y + threadIdx.y);
   for_rows<F::kAhead, F::kStages>(
       p.rows,
       [&](int s) {
@@ -524,7 +537,8 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) gated_rms_norm_grad_kernel
       [&](int s, int64_t row) {
         Eight x[I], z[I], g[I], sg[I];
         const T *const xr = F::kAhead ? nullptr : xs.next(), *const zr = F::kAhead ? nullptr : zs.next(), *const gr = F::kAhead ? nullptr : gs.next();
-        const float inv = p.inv[row * p.groups + blockIdx.y];
+        const float inv = inv_now;
+        rate(row + (int64_t)gridDim.x * blockDim.y);
         Pair c = both(0.f);
 #pragma unroll
         for (int it = 0; it < I; ++it) {
@@ -548,7 +562,7 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) gated_rms_norm_grad_kernel
             }
           });
         }
-        const Pair mean = both(-row_sum(c) / p.d);
+        const Pair mean = both(-row_sum(c) * p.inv_d);
         T *const dxr = dx.next(), *const dzr = dz.next();
 #pragma unroll
         for (int it = 0; it < I; ++it) {
@@ -600,11 +614,11 @@ struct Shape {
   int threads, rows, steps;      // threads of a row, rows of a CTA, eights of a thread
   unsigned most;                 // CTAs a group, of a gradient: each leaves its sums over rows
 };
-// Eight numbers a thread up to 1 024 a row, then sixteen, from 4 096 (a gradient: 8 192) on 32.  Rows of a warp go four to a CTA.
+// Eight numbers a thread up to 512 a row, then sixteen, from 4 096 (a gradient: 8 192) on 32.  Rows of a warp go four to a CTA.
 Shape shape_of(int64_t rows, int d, int groups, bool grad) {
   Shape s;
   const int eights = (d + 7) / 8;
-  s.steps = eights <= 128 ? 1 : eights <= (grad ? 1024 : 512) ? 2 : 4;
+  s.steps = eights <= 64 ? 1 : eights <= (grad ? 1024 : 512) ? 2 : 4;
   s.threads = ((eights + s.steps - 1) / s.steps + 31) / 32 * 32;
   s.rows = s.threads == 32 ? 4 : 1;
   const int64_t an_sm = std::max(1, 1024 / (s.threads * s.rows));
@@ -652,7 +666,7 @@ struct Launch {
   unsigned grid = 0;
   cudaStream_t stream;
   Launch(const SsdNormArgs& a, bool gated, bool grad, cudaStream_t st) : stream(st) {
-    p.rows = a.rows; p.groups = gated ? a.groups : 1; p.d = a.d / p.groups; p.eps = a.eps; p.norm_first = a.norm_first;
+    p.rows = a.rows; p.groups = gated ? a.groups : 1; p.d = a.d / p.groups; p.eps = a.eps; p.inv_d = 1.f / (float)p.d; p.norm_first = a.norm_first;
     p.x = a.x; p.z = a.z; p.res = a.residual; p.y = a.y; p.res_out = a.residual_out; p.inv = a.inv_rms; p.inv_post = a.inv_rms_post;
     p.xs = a.x_stride; p.zs = a.z_stride; p.rs = a.residual_stride; p.ys = a.y_stride; p.ros = a.residual_out_stride;
     p.w = {a.weight, a.vectors_in_dtype & 1};
