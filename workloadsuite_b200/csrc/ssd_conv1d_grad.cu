@@ -5,13 +5,14 @@
 // dpre[t] is known, so x and dy are read once but for K-1 tokens on either side of a run.  A CTA's runs follow one another; it leaves
 // its sums for dw and dbias to column_sum_kernel, in a fixed order.
 #include <algorithm>
+#include <type_traits>
 
 #include "vec_io.cuh"
 
 namespace ssd {
 namespace {
 
-constexpr int kWarps = 8, kAhead = 8;
+constexpr int kWarps = 8, kAhead = 8, kCtas = 2;
 
 struct ConvGrad {
   const void *x, *w, *bias, *dy;
@@ -22,24 +23,25 @@ struct ConvGrad {
 };
 
 template <typename T, int K>
-__global__ void __launch_bounds__(32 * kWarps) conv1d_silu_grad_kernel(const ConvGrad p) {
+__global__ void __launch_bounds__(32 * kWarps, kCtas) conv1d_silu_grad_kernel(const ConvGrad p) {
   using Raw = typename Two<T>::Raw;
-  __shared__ float2 sums[kWarps][K + 1][32];
+  __shared__ Pair sums[kWarps][K + 1][32];
   const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
   const int c = blockIdx.y * 64 + 2 * lane;
   const int cta = blockIdx.x % p.ctas, b = blockIdx.x / p.ctas;
   const bool ok = c < p.channels;
   const int64_t begin = ((int64_t)cta * kWarps + w) * p.run;
   const int t_begin = (int)min((int64_t)p.seqlen, begin), t_end = (int)min((int64_t)p.seqlen, begin + p.run);
+  const Pair zero = both(0.f), one = both(1.f), minus = both(-1.f);
 
-  float2 wk[K], bs = make_float2(0.f, 0.f), dw[K], db = make_float2(0.f, 0.f);
+  Pair wk[K], bs = zero, dw[K], db = zero;
 #pragma unroll
   for (int k = 0; k < K; ++k) {
     const T* at = static_cast<const T*>(p.w) + (int64_t)c * K + k;
-    wk[k] = ok ? make_float2(Cvt<T>::to_f(at[0]), Cvt<T>::to_f(at[K])) : make_float2(0.f, 0.f);
-    dw[k] = make_float2(0.f, 0.f);
+    wk[k] = ok ? pair(Cvt<T>::to_f(at[0]), Cvt<T>::to_f(at[K])) : zero;
+    dw[k] = zero;
   }
-  if (ok && p.bias) bs = make_float2(Cvt<T>::to_f(static_cast<const T*>(p.bias)[c]), Cvt<T>::to_f(static_cast<const T*>(p.bias)[c + 1]));
+  if (ok && p.bias) bs = pair(Cvt<T>::to_f(static_cast<const T*>(p.bias)[c]), Cvt<T>::to_f(static_cast<const T*>(p.bias)[c + 1]));
   const T* x = static_cast<const T*>(p.x) + b * p.xs[0] + c;
   const T* dy = static_cast<const T*>(p.dy) + b * p.dys[0] + c;
   T* dx = static_cast<T*>(p.dx) + b * p.dxs[0] + c;
@@ -48,48 +50,65 @@ __global__ void __launch_bounds__(32 * kWarps) conv1d_silu_grad_kernel(const Con
   };
 
   if (t_begin < t_end) {
-    float2 xw[K], dp[K];   // x[t-(K-1)+k] and dpre[t-(K-1)+k]
+    // x and dpre of token t_begin + n in places n & 7: no row is ever moved
+    Pair xw[kAhead], dp[kAhead];
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
-      xw[k] = k > 0 ? Two<T>::up(row(x, p.xs[1], t_begin - K + k)) : make_float2(0.f, 0.f);
-      dp[k] = make_float2(0.f, 0.f);
-    }
-    const int t_last = t_end + K - 1;   // dpre of the K - 1 tokens behind the run, zero behind the sequence
-    for (int t0 = t_begin; t0 < t_last; t0 += kAhead) {
-      Raw rx[kAhead], rd[kAhead];
+    for (int n = 0; n < kAhead; ++n) dp[n] = zero, xw[n] = n > kAhead - K ? pair_of<T>(row(x, p.xs[1], t_begin - kAhead + n)) : zero;
+    const int t_last = min(t_end + K - 1, p.seqlen + K - 1);   // dpre of the K - 1 tokens behind the run, zero behind the sequence
+    Raw rx[kAhead], rd[kAhead];
+    auto ask = [&](int t0) {
+      if (ok && t0 + kAhead <= p.seqlen) {
+        const T *xa = x + (int64_t)t0 * p.xs[1], *da = dy + (int64_t)t0 * p.dys[1];
 #pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        rx[n] = row(x, p.xs[1], t0 + n < t_last ? t0 + n : -1);
-        rd[n] = row(dy, p.dys[1], t0 + n < t_last ? t0 + n : -1);
-      }
-#pragma unroll
-      for (int n = 0; n < kAhead; ++n) {
-        const int t = t0 + n;
-        if (t < t_last) {
-#pragma unroll
-          for (int k = 0; k < K - 1; ++k) xw[k] = xw[k + 1], dp[k] = dp[k + 1];
-          xw[K - 1] = Two<T>::up(rx[n]);
-          const float2 g = Two<T>::up(rd[n]);
-          float2 pre = bs;
-#pragma unroll
-          for (int k = 0; k < K; ++k) pre.x = fmaf(wk[k].x, xw[k].x, pre.x), pre.y = fmaf(wk[k].y, xw[k].y, pre.y);
-          const float s0 = sigmoid_approx(pre.x), s1 = sigmoid_approx(pre.y);
-          float2 d;
-          d.x = t < p.seqlen ? g.x * s0 * fmaf(pre.x, 1.f - s0, 1.f) : 0.f;
-          d.y = t < p.seqlen ? g.y * s1 * fmaf(pre.y, 1.f - s1, 1.f) : 0.f;
-          dp[K - 1] = d;
-          if (t < t_end) {
-            db.x += d.x, db.y += d.y;
-#pragma unroll
-            for (int k = 0; k < K; ++k) dw[k].x = fmaf(d.x, xw[k].x, dw[k].x), dw[k].y = fmaf(d.y, xw[k].y, dw[k].y);
-          }
-          if (t - (K - 1) >= t_begin && ok) {
-            float2 o = make_float2(0.f, 0.f);
-#pragma unroll
-            for (int k = 0; k < K; ++k) o.x = fmaf(wk[k].x, dp[K - 1 - k].x, o.x), o.y = fmaf(wk[k].y, dp[K - 1 - k].y, o.y);
-            *reinterpret_cast<Raw*>(dx + (int64_t)(t - (K - 1)) * p.dxs[1]) = Two<T>::down(o.x, o.y);
-          }
+        for (int n = 0; n < kAhead; ++n, xa += p.xs[1], da += p.dys[1]) {
+          rx[n] = *reinterpret_cast<const Raw*>(xa);
+          rd[n] = *reinterpret_cast<const Raw*>(da);
         }
+      } else {
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n) rx[n] = row(x, p.xs[1], t0 + n), rd[n] = row(dy, p.dys[1], t0 + n);
+      }
+    };
+    // one token; ALL: it is the run's, and so are those that its dx is of
+    auto token = [&](auto all, int n, int t, Pair xv, Pair g, T* to) {
+      constexpr bool ALL = decltype(all)::value;
+      auto at = [&](int back) { return (n + kAhead - back) % kAhead; };
+      xw[n] = xv;
+      Pair pre = bs;
+#pragma unroll
+      for (int k = 0; k < K; ++k) pre = fma(wk[k], xw[at(K - 1 - k)], pre);
+      const Pair s = each(each(pre * both(-kLog2E), exp2_approx) + one, rcp_approx);
+      Pair d = (g * s) * fma(pre, fma(s, minus, one), one);
+      if (!ALL && t >= p.seqlen) d = zero;
+      dp[n] = d;
+      if (ALL || t < t_end) {
+        db = db + d;
+#pragma unroll
+        for (int k = 0; k < K; ++k) dw[k] = fma(d, xw[at(K - 1 - k)], dw[k]);
+      }
+      Pair o = wk[0] * d;
+#pragma unroll
+      for (int k = 1; k < K; ++k) o = fma(wk[k], dp[at(k)], o);
+      const int u = t - (K - 1);
+      if (ok && (ALL || (u >= t_begin && u < t_end))) {
+        const float2 h = halves(o);
+        *reinterpret_cast<Raw*>(to) = Two<T>::down(h.x, h.y);
+      }
+    };
+    ask(t_begin);
+    for (int t0 = t_begin; t0 < t_last; t0 += kAhead) {
+      Raw cx[kAhead], cd[kAhead];
+#pragma unroll
+      for (int n = 0; n < kAhead; ++n) cx[n] = rx[n], cd[n] = rd[n];
+      if (t0 + kAhead < t_last) ask(t0 + kAhead);
+      T* to = dx + (int64_t)(t0 - (K - 1)) * p.dxs[1];
+      if (t0 > t_begin && t0 + kAhead <= t_end) {
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n, to += p.dxs[1]) token(std::true_type(), n, t0 + n, pair_of<T>(cx[n]), pair_of<T>(cd[n]), to);
+      } else {
+#pragma unroll
+        for (int n = 0; n < kAhead; ++n, to += p.dxs[1])
+          if (t0 + n < t_last) token(std::false_type(), n, t0 + n, pair_of<T>(cx[n]), pair_of<T>(cd[n]), to);
       }
     }
   }
@@ -100,9 +119,10 @@ __global__ void __launch_bounds__(32 * kWarps) conv1d_silu_grad_kernel(const Con
   for (int i = threadIdx.x; i < (K + 1) * 32; i += 32 * kWarps) {
     const int k = i / 32, l = i % 32, cc = blockIdx.y * 64 + 2 * l;
     if (cc >= p.channels) continue;
-    float2 v = make_float2(0.f, 0.f);
-    for (int u = 0; u < kWarps; ++u) v.x += sums[u][k][l].x, v.y += sums[u][k][l].y;
-    *reinterpret_cast<float2*>(p.part + ((int64_t)blockIdx.x * (K + 1) + k) * p.channels + cc) = v;
+    Pair v = sums[0][k][l];
+#pragma unroll
+    for (int u = 1; u < kWarps; ++u) v = v + sums[u][k][l];
+    *reinterpret_cast<float2*>(p.part + ((int64_t)blockIdx.x * (K + 1) + k) * p.channels + cc) = halves(v);
   }
 }
 
@@ -124,7 +144,7 @@ struct Cut {
 Cut cut_of(int batch, int seqlen, int channels) {
   Cut c;
   const int64_t strips = (int64_t)batch * ((channels + 63) / 64);
-  for (c.run = 64; c.run > 8; c.run /= 2) {
+  for (c.run = 128; c.run > 8; c.run /= 2) {
     if (strips * ((seqlen + (int64_t)kWarps * c.run - 1) / (kWarps * c.run)) >= 148 * 4) break;
   }
   c.ctas = (int)(((int64_t)seqlen + kWarps * c.run - 1) / (kWarps * c.run));
