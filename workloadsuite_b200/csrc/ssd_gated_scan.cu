@@ -27,10 +27,17 @@ namespace ssd {
 namespace {
 
 constexpr int kStrip = 64, kPiece = 64;
-constexpr int kRun = 16, kRuns = 8, kTile = kRun * kRuns;                       // tokens of a run, runs of a tile
-constexpr int kCtas = 2, kCtasGrad = 2;   // that an SM holds
-constexpr int kRunGrad = 8, kRunsGrad = 8, kTileGrad = kRunGrad * kRunsGrad;
-static_assert(kPiece % kRun == 0 && kTileGrad == kPiece, "pieces start at runs");
+// Tokens of a run, runs of a tile (warps of a CTA), CTAs that an SM holds (two tiles' inputs a CTA in shared memory).
+// Long runs: what a run costs besides its tokens is some 250 instructions a warp (8 x 2 048 x 2 048 bf16: forward 64 us, with 12 runs of 8
+// tokens 87, with three CTAs of 8 runs of 8 72; gradient 146 us, with 16 runs of 4 244).
+template <typename T, bool GRAD> struct Geometry;
+template <typename T> struct Geometry<T, false> {
+  static constexpr int kRun = sizeof(T) == 2 ? 16 : 8, kRuns = sizeof(T) == 2 ? 8 : 16, kCtas = sizeof(T) == 2 ? 2 : 1;
+};
+template <typename T> struct Geometry<T, true> {
+  static constexpr int kRun = sizeof(T) == 2 ? 8 : 4, kRuns = sizeof(T) == 2 ? 8 : 16, kCtas = sizeof(T) == 2 ? 2 : 1;
+};
+constexpr int kTile = 128, kTileGrad = kPiece;   // tokens of a tile
 
 struct Scan {
   const void *x, *i, *r, *dy;
@@ -194,17 +201,34 @@ __device__ __forceinline__ void wait_for(const Scan& p, S& sh, uint64_t* full, u
   }
 }
 
-// One operand's tile where TMA cannot read it (rows that do not start on 16 bytes): two channels a lane, by all threads.
+// One operand's tile where TMA cannot read it (rows that do not start on 16 bytes), by all threads: fp32 by copies that are waited for
+// later, 16-bit numbers, which no asynchronous copy takes one by one, through registers.
 template <typename T, int TILE, int RUNS>
 __device__ __forceinline__ void fill(T* to, const void* from, int b, int t0, int seqlen, const int64_t* st, int c, int channels) {
-  const int lane = threadIdx.x % 32;
-  const T* at = static_cast<const T*>(from) + b * st[0] + (int64_t)t0 * st[1] + c;
-  for (int t = threadIdx.x / 32; t < TILE; t += RUNS) {
-    const bool there = t0 + t < seqlen;
+  const int lane = threadIdx.x % 32, w = threadIdx.x / 32;
+  const T* at = static_cast<const T*>(from) + b * st[0] + (int64_t)(t0 + w) * st[1] + c + lane;
+  constexpr int kRows = TILE / RUNS, kBatch = 4;
 #pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int l = lane + 32 * e;
-      to[t * kStrip + l] = there && c + l < channels ? at[t * st[1] + l] : Cvt<T>::from_f(0.f);
+  for (int r0 = 0; r0 < kRows; r0 += kBatch) {
+    T v[kBatch][2];
+#pragma unroll
+    for (int r = 0; r < kBatch; ++r, at += RUNS * st[1]) {
+      const int t = w + (r0 + r) * RUNS;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bool there = t0 + t < seqlen && c + lane + 32 * e < channels;
+        if constexpr (sizeof(T) == 4)
+          asm volatile("cp.async.ca.shared.global [%0], [%1], 4, %2;" ::"r"(ptx::smem_u32(to + t * kStrip + lane + 32 * e)),
+                       "l"(there ? at + 32 * e : static_cast<const T*>(from)), "r"(there ? 4 : 0) : "memory");
+        else
+          v[r][e] = there ? at[32 * e] : Cvt<T>::from_f(0.f);
+      }
+    }
+    if constexpr (sizeof(T) == 2) {
+#pragma unroll
+      for (int r = 0; r < kBatch; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) to[(w + (r0 + r) * RUNS) * kStrip + lane + 32 * e] = v[r][e];
     }
   }
 }
@@ -330,9 +354,11 @@ struct Lane {
 
 // TMA: every tensor's rows start on 16 bytes.
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(32 * kRuns, kCtas) gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(32 * Geometry<T, false>::kRuns, Geometry<T, false>::kCtas)
+gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
   using Raw = typename Two<T>::Raw;
-  constexpr int L = kRun, kStage = (int)stage_numbers(3, kTile);
+  constexpr int L = Geometry<T, false>::kRun, kRuns = Geometry<T, false>::kRuns, kStage = (int)stage_numbers(3, kTile);
+  static_assert(L * kRuns == kTile && kPiece % L == 0, "runs make a tile, pieces start at runs");
   extern __shared__ __align__(128) unsigned char smem[];
   T* const stages = reinterpret_cast<T*>(smem);
   Shared<kRuns, 1>& sh = *reinterpret_cast<Shared<kRuns, 1>*>(smem + 2 * kStage * sizeof(T));
@@ -347,6 +373,17 @@ __global__ void __launch_bounds__(32 * kRuns, kCtas) gated_scan_kernel(const __g
   }
   __syncthreads();
 
+  // without TMA: a tile's inputs by all threads, fp32 a tile ahead
+  constexpr bool kLate = sizeof(T) == 4;
+  auto fetch = [&](int s) {
+    const int4 of = sh.which[s];
+    if (of.x < 0) return;
+    T* const to = stages + s * kStage;
+    fill<T, kTile, kRuns>(to, p.x, of.w, of.x * kTile, p.seqlen, p.xs, of.z * kStrip, p.channels);
+    fill<T, kTile, kRuns>(to + kTile * kStrip, p.i, of.w, of.x * kTile, p.seqlen, p.is, of.z * kStrip, p.channels);
+    fill<T, kTile, kRuns>(to + 2 * kTile * kStrip, p.r, of.w, of.x * kTile, p.seqlen, p.rs, of.z * kStrip, p.channels);
+  };
+  if constexpr (!TMA && kLate) fetch(0);
   for (unsigned turn = 0;; ++turn) {
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
@@ -358,11 +395,13 @@ __global__ void __launch_bounds__(32 * kRuns, kCtas) gated_scan_kernel(const __g
     const int here = min(L, p.seqlen - t0);   // tokens of this run that are there
     const Lane ln(strip, p.channels);
     const int64_t first = (int64_t)unit * p.tiles;
-    if constexpr (!TMA) {
-      const int c = strip * kStrip;
-      fill<T, kTile, kRuns>(stage, p.x, b, k * kTile, p.seqlen, p.xs, c, p.channels);
-      fill<T, kTile, kRuns>(stage + kTile * kStrip, p.i, b, k * kTile, p.seqlen, p.is, c, p.channels);
-      fill<T, kTile, kRuns>(stage + 2 * kTile * kStrip, p.r, b, k * kTile, p.seqlen, p.rs, c, p.channels);
+    if constexpr (!TMA && kLate) {
+      asm volatile("cp.async.wait_group 0;" ::: "memory");
+      __syncthreads();
+      wait_for(p, sh, &sh.full[s ^ 1], (turn + 1) >> 1 & 1);
+      fetch(s ^ 1);
+    } else if constexpr (!TMA) {
+      fetch(s);
       __syncthreads();
     }
     const Raw* const raw = reinterpret_cast<const Raw*>(stage + w * L * kStrip) + lane;
@@ -469,13 +508,15 @@ __global__ void __launch_bounds__(32 * kRuns, kCtas) gated_scan_kernel(const __g
 // With w = b si, u = w x and m = a^2 / (1 - a^2):  dx = g w,  di = g u (1 - si),  dla = g (a h[t-1] - m u)  (without its first term at a
 // reset),  dr = dla la (1 - sr),  and what decay's gradient sums up is dla la.
 template <typename T, bool TMA>
-__global__ void __launch_bounds__(32 * kRunsGrad, kCtasGrad) gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
+__global__ void __launch_bounds__(32 * Geometry<T, true>::kRuns, Geometry<T, true>::kCtas)
+gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
   using Raw = typename Two<T>::Raw;
-  constexpr int L = kRunGrad, kStage = (int)stage_numbers(4, kTileGrad);
+  constexpr int L = Geometry<T, true>::kRun, kRuns = Geometry<T, true>::kRuns, kStage = (int)stage_numbers(4, kTileGrad);
+  static_assert(L * kRuns == kTileGrad, "runs make a tile");
   extern __shared__ __align__(128) unsigned char smem[];
   T* const stages = reinterpret_cast<T*>(smem);
-  Shared<kRunsGrad, 2>& sh = *reinterpret_cast<Shared<kRunsGrad, 2>*>(smem + 2 * kStage * sizeof(T));
-  __shared__ Pair sums[2][kRunsGrad][32];
+  Shared<kRuns, 2>& sh = *reinterpret_cast<Shared<kRuns, 2>*>(smem + 2 * kStage * sizeof(T));
+  __shared__ Pair sums[2][kRuns][32];
   const int w = threadIdx.x / 32, lane = threadIdx.x % 32;
   if (threadIdx.x == 0) {
     sh.dead = 0;
@@ -493,10 +534,23 @@ __global__ void __launch_bounds__(32 * kRunsGrad, kCtasGrad) gated_scan_grad_ker
     if (part && w == 0) {
       Pair v = sums[s][0][lane];
 #pragma unroll
-      for (int n = 1; n < kRunsGrad; ++n) v = v + sums[s][n][lane];
+      for (int n = 1; n < kRuns; ++n) v = v + sums[s][n][lane];
       *reinterpret_cast<float2*>(part) = halves(v);
     }
   };
+  constexpr bool kLate = sizeof(T) == 4;
+  auto fetch = [&](int s) {
+    const int4 of = sh.which[s];
+    if (of.x < 0) return;
+    constexpr int n = kTileGrad * kStrip;
+    T* const to = stages + s * kStage;
+    const int at = (p.tiles - 1 - of.x) * kTileGrad;
+    fill<T, kTileGrad, kRuns>(to, p.x, of.w, at, p.seqlen, p.xs, of.z * kStrip, p.channels);
+    fill<T, kTileGrad, kRuns>(to + n, p.i, of.w, at, p.seqlen, p.is, of.z * kStrip, p.channels);
+    fill<T, kTileGrad, kRuns>(to + 2 * n, p.r, of.w, at, p.seqlen, p.rs, of.z * kStrip, p.channels);
+    fill<T, kTileGrad, kRuns>(to + 3 * n, p.dy, of.w, at, p.seqlen, p.dys, of.z * kStrip, p.channels);
+  };
+  if constexpr (!TMA && kLate) fetch(0);
   for (;; ++turn) {
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
@@ -509,11 +563,8 @@ __global__ void __launch_bounds__(32 * kRunsGrad, kCtasGrad) gated_scan_grad_ker
     const Lane ln(strip, p.channels);
     const int64_t first = (int64_t)unit * p.tiles;
     if constexpr (!TMA) {
-      const int c = strip * kStrip, n = kTileGrad * kStrip;
-      fill<T, kTileGrad, kRunsGrad>(stage, p.x, b, k * kTileGrad, p.seqlen, p.xs, c, p.channels);
-      fill<T, kTileGrad, kRunsGrad>(stage + n, p.i, b, k * kTileGrad, p.seqlen, p.is, c, p.channels);
-      fill<T, kTileGrad, kRunsGrad>(stage + 2 * n, p.r, b, k * kTileGrad, p.seqlen, p.rs, c, p.channels);
-      fill<T, kTileGrad, kRunsGrad>(stage + 3 * n, p.dy, b, k * kTileGrad, p.seqlen, p.dys, c, p.channels);
+      if constexpr (kLate) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else fetch(s);
       __syncthreads();
     }
     const Raw* const raw = reinterpret_cast<const Raw*>(stage + w * L * kStrip) + lane;
@@ -580,8 +631,12 @@ if (marks == 0) {
     __syncthreads();
 
     // (the inputs of the tile before have been read)
-    if (turn > 0 && threadIdx.x == 32 * (kRunsGrad - 1))
+    if (turn > 0 && threadIdx.x == 32 * (kRuns - 1))
       send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true);
+    if constexpr (!TMA && kLate) {
+      wait_for(p, sh, &sh.full[s ^ 1], (turn + 1) >> 1 & 1);
+      fetch(s ^ 1);
+    }
     leave_sums(s ^ 1);
     part = p.part + ((int64_t)b * p.tiles + k) * ((int64_t)p.strips * kStrip) + ln.c;
     const bool last = kb == p.tiles - 1;   // of the way back: the sequence's first
@@ -604,7 +659,7 @@ if (marks == 0) {
       else if (p.dinit) ln.put(p.dinit + (int64_t)b * p.channels, out);
     }
     h = through(h, w, [&](int v) { return run[v][lane]; });
-    c = through(c, kRunsGrad - 1 - w, [&](int v) { return back[kRunsGrad - 1 - v][lane]; });
+    c = through(c, kRuns - 1 - w, [&](int v) { return back[kRuns - 1 - v][lane]; });
 
     Pair sum = both(0.f);
     // ALL: every token of the run is there and none is marked
@@ -800,8 +855,9 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
           operand_map<T>(&maps.at[2], a.decay_gate, a, p.rs, tile) &&
           (!grad || operand_map<T>(&maps.at[3], a.dy, a, p.dys, tile));
   }
-  // two CTAs an SM, one where tiles are of 32-bit numbers
-  const unsigned grid = std::min(p.total, 148u * (sizeof(T) == 2 ? (grad ? kCtasGrad : kCtas) : 1));
+  using Fwd = Geometry<T, false>;
+  using Bwd = Geometry<T, true>;
+  const unsigned grid = std::min(p.total, 148u * (grad ? Bwd::kCtas : Fwd::kCtas));
   auto go = [&](auto kernel, int threads, size_t smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)SSD_ERR_CUDA;
     if (!z.words && !z.rates) return launch(kernel, grid, threads, smem, stream, p, maps);
@@ -812,11 +868,11 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
     return launch_early(kernel, grid, threads, smem, stream, p, maps);
   };
   if (!grad) {
-    const size_t smem = 2 * stage_numbers(3, kTile) * sizeof(T) + sizeof(Shared<kRuns, 1>);
-    return tma ? go(gated_scan_kernel<T, true>, 32 * kRuns, smem) : go(gated_scan_kernel<T, false>, 32 * kRuns, smem);
+    const size_t smem = 2 * stage_numbers(3, kTile) * sizeof(T) + sizeof(Shared<Fwd::kRuns, 1>);
+    return tma ? go(gated_scan_kernel<T, true>, 32 * Fwd::kRuns, smem) : go(gated_scan_kernel<T, false>, 32 * Fwd::kRuns, smem);
   }
-  const size_t smem = 2 * stage_numbers(4, kTileGrad) * sizeof(T) + sizeof(Shared<kRunsGrad, 2>);
-  if (const int rc = tma ? go(gated_scan_grad_kernel<T, true>, 32 * kRunsGrad, smem) : go(gated_scan_grad_kernel<T, false>, 32 * kRunsGrad, smem)) return rc;
+  const size_t smem = 2 * stage_numbers(4, kTileGrad) * sizeof(T) + sizeof(Shared<Bwd::kRuns, 2>);
+  if (const int rc = tma ? go(gated_scan_grad_kernel<T, true>, 32 * Bwd::kRuns, smem) : go(gated_scan_grad_kernel<T, false>, 32 * Bwd::kRuns, smem)) return rc;
   return launch_column_sum(p.part, a.batch * z.tiles, (int64_t)p.strips * kStrip, a.channels, FinishDecay{a.decay, a.ddecay}, stream);
 }
 
