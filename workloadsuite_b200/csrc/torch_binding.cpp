@@ -11,6 +11,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "ssd_b200.h"
@@ -176,30 +178,6 @@ PyObject* py_dt(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
-// conv1d_silu(x, weight, bias, out) -> y
-PyObject* py_conv(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  const Tensor *x, *w, *bias, *out;
-  if (n != 4 || !get(o[0], &x) || !get(o[1], &w) || !get(o[2], &bias, true) || !get(o[3], &out, true) || !x->is_cuda() || x->dim() != 3)
-    Py_RETURN_NONE;
-  const int dtype = dtype_of(*x);
-  const int64_t b = x->size(0), l = x->size(1), d = x->size(2);
-  const auto st = x->scalar_type();
-  if (dtype < 0 || x->stride(2) != 1 || d <= 0 || w->scalar_type() != st || !w->is_contiguous() || w->dim() < 2 || w->size(0) != d ||
-      w->numel() != d * w->size(-1))
-    Py_RETURN_NONE;
-  if (bias->defined() && (!shaped(*bias, {d}) || bias->scalar_type() != st || !bias->is_contiguous())) Py_RETURN_NONE;
-  if (out->defined() && (out->scalar_type() != st || out->sizes() != x->sizes() || !inner(*out))) Py_RETURN_NONE;
-  Where q(*x);
-  if (!q.here(*w) || !q.here(*bias) || !q.here(*out)) Py_RETURN_NONE;
-  Tensor y = out->defined() ? *out : at::empty({b, l, d}, x->options());
-  if (const int rc = f_conv(x->data_ptr(), w->data_ptr(), bias->defined() ? bias->data_ptr() : nullptr, y.data_ptr(), (int)b,
-                            (int)l, (int)d, (int)w->size(-1), dtype, x->stride(0), x->stride(1), y.stride(0), y.stride(1), q.stream()))
-    return declined(rc);
-  return THPVariable_Wrap(std::move(y));
-  END_HANDLE_TH_ERRORS
-}
-
 // forward(X, A, B, C, chunk, dt, initial_states, D, z, out, return_final_state) -> Y or (Y, final_state)
 PyObject* py_forward(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
@@ -293,7 +271,43 @@ void two(const Tensor& t, int64_t* st) {
   st[1] = t.stride(1);
 }
 
-// What the forward and the backward of the gated scan both check and fill in.
+// The operators below are recorded for autograd here too: a node in Python costs a training step of a small layer more than its kernels.
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+using Maybe = std::optional<Tensor>;
+
+bool records(std::initializer_list<const Tensor*> ts) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const Tensor* t : ts)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
+Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
+// A gradient whose innermost axis is not contiguous (a sum's is expanded) is copied once.
+Tensor usable(const Tensor& t) { return !t.defined() || inner(t) ? t : t.contiguous(); }
+// Outside of entry points that hold the interpreter: what a refused or failed call raises.
+void must(bool fits, int rc, const char* what) {
+  TORCH_CHECK_NOT_IMPLEMENTED(fits, what, ": sizes or strides outside what the kernels cover");
+  TORCH_CHECK(rc == 0, what, ": the library returned code ", rc);
+}
+// Gradients are not differentiable themselves: to differentiate them is an error, as with once_differentiable in Python.
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  variable_list there;
+  for (Tensor& g : grads)
+    if (g.defined()) there.push_back(g.detach());
+  auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is not twice differentiable", (int)there.size());
+  there = (*error)(std::move(there));
+  size_t n = 0;
+  for (Tensor& g : grads)
+    if (g.defined()) g = there[n++];
+  return grads;
+}
+
+// ---- gated scan ----
+
+// What the forward and the backward both check and fill in.
 bool gated_args(const Tensor& x, const Tensor& i, const Tensor& r, const Tensor& decay, const Tensor& init, const Tensor& reset, float rate,
                 const Where& w, SsdGatedScanArgs* a) {
   const int64_t b = x.size(0), s = x.size(1), d = x.size(2);
@@ -313,64 +327,100 @@ bool gated_args(const Tensor& x, const Tensor& i, const Tensor& r, const Tensor&
   return true;
 }
 
-// gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, wait_limit_ms, want_pieces) -> (y, final_state, pieces or None)
+struct Gated {
+  Tensor y, fin, pieces;
+};
+bool gated_forward(const Tensor& x, const Tensor& i, const Tensor& r, const Tensor& decay, const Tensor& init, const Tensor& reset,
+                   const Tensor& out, float rate, int wait_ms, bool keep, Gated* g, int* rc) {
+  Where w(x);
+  SsdGatedScanArgs a = {};
+  if (!gated_args(x, i, r, decay, init, reset, rate, w, &a)) return false;
+  if (out.defined() && (out.dim() != 3 || !like3(out, x) || !w.here(out))) return false;
+  a.wait_limit_ms = wait_ms;
+  const auto f32 = x.options().dtype(at::kFloat);
+  g->y = out.defined() ? out : at::empty(x.sizes(), x.options());
+  g->fin = at::empty({x.size(0), x.size(2)}, f32);
+  if (keep) g->pieces = at::empty({x.size(0), (x.size(1) + 63) / 64, x.size(2)}, f32);
+  a.y = g->y.data_ptr(); a.final_state = ptr<float>(g->fin); a.pieces = ptr<float>(g->pieces);
+  two(g->y, a.y_stride);
+  const size_t need = f_gated_workspace(&a, 0);
+  const Tensor ws = scratch(x, need);
+  a.workspace = ptr(ws);
+  a.workspace_bytes = need;
+  *rc = f_gated(&a, w.stream());
+  return true;
+}
+bool gated_backward(const Tensor& x, const Tensor& i, const Tensor& r, const Tensor& decay, const Tensor& reset, const Tensor& pieces,
+                    const Tensor& dy, const Tensor& dfin, float rate, bool want_dinit, variable_list* out, int* rc) {
+  Where w(x);
+  SsdGatedScanArgs a = {};
+  if (!gated_args(x, i, r, decay, Tensor(), reset, rate, w, &a)) return false;
+  const int64_t b = x.size(0), s = x.size(1), d = x.size(2);
+  if (!like3(dy, x) || !w.here(dy) || !plain32(dfin, {b, d}) || !w.here(dfin) || !plain32(pieces, {b, (s + 63) / 64, d}) || !w.here(pieces))
+    return false;
+  const auto f32 = x.options().dtype(at::kFloat);
+  Tensor dx = at::empty(x.sizes(), x.options()), di = at::empty(x.sizes(), x.options()), dr = at::empty(x.sizes(), x.options());
+  Tensor dd = at::empty({d}, f32), dh;
+  if (want_dinit) dh = at::empty({b, d}, f32);
+  a.pieces = ptr<float>(pieces); a.dy = dy.data_ptr(); a.dfinal_state = ptr<float>(dfin);
+  a.dx = dx.data_ptr(); a.dinput_gate = di.data_ptr(); a.ddecay_gate = dr.data_ptr(); a.ddecay = ptr<float>(dd); a.dinitial_state = ptr<float>(dh);
+  two(dy, a.dy_stride); two(dx, a.dx_stride); two(di, a.dinput_gate_stride); two(dr, a.ddecay_gate_stride);
+  const size_t need = f_gated_workspace(&a, 1);
+  const Tensor ws = scratch(x, need);
+  a.workspace = ptr(ws);
+  a.workspace_bytes = need;
+  *rc = f_gated_backward(&a, w.stream());
+  *out = {dx, di, dr, dd, dh};
+  return true;
+}
+
+struct GatedNode : torch::autograd::Function<GatedNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& i, const Tensor& r, const Tensor& decay, const Maybe& init,
+                               const Maybe& reset, double rate, int64_t wait_ms, int* rc) {
+    Gated g;
+    *rc = 1;   // (declined)
+    if (!gated_forward(x, i, r, decay, given(init), given(reset), Tensor(), (float)rate, (int)wait_ms, true, &g, rc) || *rc) return {};
+    ctx->save_for_backward({x, i, r, decay, given(reset), g.pieces});
+    ctx->saved_data["rate"] = rate;
+    ctx->saved_data["state"] = init.has_value();
+    ctx->set_materialize_grads(false);
+    return {g.y, g.fin};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    if (!grads[0].defined() && !grads[1].defined()) return variable_list(9);
+    const auto saved = ctx->get_saved_variables();
+    const Tensor& x = saved[0];
+    const Tensor dy = grads[0].defined() ? usable(grads[0]) : at::zeros(x.sizes(), x.options());
+    const Tensor dfin = grads[1].defined() ? grads[1].contiguous() : Tensor();
+    variable_list out;
+    int rc = 0;
+    const bool ok = gated_backward(x, saved[1], saved[2], saved[3], saved[4], saved[5], dy, dfin, (float)ctx->saved_data["rate"].toDouble(),
+                                   ctx->saved_data["state"].toBool(), &out, &rc);
+    must(ok, rc, "gated_scan");
+    out.resize(9);
+    return once(std::move(out), "gated_scan");
+  }
+};
+
+// gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, wait_limit_ms) -> (y, final_state)
 PyObject* py_gated(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Tensor *x, *i, *r, *decay, *init, *reset, *out;
   float rate;
-  if (n != 10 || !get(o[0], &x) || !get(o[1], &i) || !get(o[2], &r) || !get(o[3], &decay) || !get(o[4], &init, true) ||
+  if (n != 9 || !get(o[0], &x) || !get(o[1], &i) || !get(o[2], &r) || !get(o[3], &decay) || !get(o[4], &init, true) ||
       !get(o[5], &reset, true) || !get(o[6], &out, true) || !real(o[7], &rate) || !PyLong_CheckExact(o[8]) || !x->is_cuda() ||
       x->dim() != 3 || i->dim() != 3 || r->dim() != 3 || dtype_of(*x) < 0)
     Py_RETURN_NONE;
-  Where w(*x);
-  SsdGatedScanArgs a = {};
-  if (!gated_args(*x, *i, *r, *decay, *init, *reset, rate, w, &a)) Py_RETURN_NONE;
-  if (out->defined() && (out->dim() != 3 || !like3(*out, *x) || !w.here(*out))) Py_RETURN_NONE;
-  a.wait_limit_ms = (int)PyLong_AsLong(o[8]);
-  const auto f32 = x->options().dtype(at::kFloat);
-  Tensor y = out->defined() ? *out : at::empty(x->sizes(), x->options());
-  Tensor fin = at::empty({x->size(0), x->size(2)}, f32), pieces;
-  if (o[9] == Py_True) pieces = at::empty({x->size(0), (x->size(1) + 63) / 64, x->size(2)}, f32);
-  a.y = y.data_ptr(); a.final_state = ptr<float>(fin); a.pieces = ptr<float>(pieces);
-  two(y, a.y_stride);
-  const size_t need = f_gated_workspace(&a, 0);
-  const Tensor ws = scratch(*x, need);
-  a.workspace = ptr(ws);
-  a.workspace_bytes = need;
-  if (const int rc = f_gated(&a, w.stream())) return declined(rc);
-  return tuple_of({y, fin, pieces});
-  END_HANDLE_TH_ERRORS
-}
-
-// gated_scan_backward(x, input_gate, decay_gate, decay, reset, pieces, dy, dfinal_state, rate, want_dinitial)
-//   -> (dx, dinput_gate, ddecay_gate, ddecay, dinitial_state or None)
-PyObject* py_gated_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  const Tensor *x, *i, *r, *decay, *reset, *pieces, *dy, *dfin;
-  float rate;
-  if (n != 10 || !get(o[0], &x) || !get(o[1], &i) || !get(o[2], &r) || !get(o[3], &decay) || !get(o[4], &reset, true) ||
-      !get(o[5], &pieces) || !get(o[6], &dy) || !get(o[7], &dfin, true) || !real(o[8], &rate) || !x->is_cuda() || x->dim() != 3 ||
-      i->dim() != 3 || r->dim() != 3 || dy->dim() != 3 || dtype_of(*x) < 0)
-    Py_RETURN_NONE;
-  Where w(*x);
-  SsdGatedScanArgs a = {};
-  if (!gated_args(*x, *i, *r, *decay, Tensor(), *reset, rate, w, &a)) Py_RETURN_NONE;
-  const int64_t b = x->size(0), s = x->size(1), d = x->size(2);
-  if (!like3(*dy, *x) || !w.here(*dy) || !plain32(*dfin, {b, d}) || !w.here(*dfin) || !plain32(*pieces, {b, (s + 63) / 64, d}) || !w.here(*pieces))
-    Py_RETURN_NONE;
-  const auto f32 = x->options().dtype(at::kFloat);
-  Tensor dx = at::empty(x->sizes(), x->options()), di = at::empty(x->sizes(), x->options()), dr = at::empty(x->sizes(), x->options());
-  Tensor dd = at::empty({d}, f32), dh;
-  if (o[9] == Py_True) dh = at::empty({b, d}, f32);
-  a.pieces = ptr<float>(*pieces); a.dy = dy->data_ptr(); a.dfinal_state = ptr<float>(*dfin);
-  a.dx = dx.data_ptr(); a.dinput_gate = di.data_ptr(); a.ddecay_gate = dr.data_ptr(); a.ddecay = ptr<float>(dd); a.dinitial_state = ptr<float>(dh);
-  two(*dy, a.dy_stride); two(dx, a.dx_stride); two(di, a.dinput_gate_stride); two(dr, a.ddecay_gate_stride);
-  const size_t need = f_gated_workspace(&a, 1);
-  const Tensor ws = scratch(*x, need);
-  a.workspace = ptr(ws);
-  a.workspace_bytes = need;
-  if (const int rc = f_gated_backward(&a, w.stream())) return declined(rc);
-  return tuple_of({dx, di, dr, dd, dh});
+  const int wait_ms = (int)PyLong_AsLong(o[8]);
+  int rc = 0;
+  if (records({x, i, r, decay, init})) {
+    if (out->defined()) Py_RETURN_NONE;
+    const variable_list v = GatedNode::apply(*x, *i, *r, *decay, maybe(*init), maybe(*reset), (double)rate, (int64_t)wait_ms, &rc);
+    return rc ? declined(rc) : tuple_of({v[0], v[1]});
+  }
+  Gated g;
+  if (!gated_forward(*x, *i, *r, *decay, *init, *reset, *out, rate, wait_ms, false, &g, &rc)) Py_RETURN_NONE;
+  return rc ? declined(rc) : tuple_of({g.y, g.fin});
   END_HANDLE_TH_ERRORS
 }
 
@@ -404,6 +454,8 @@ PyObject* py_gated_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
   END_HANDLE_TH_ERRORS
 }
 
+// ---- norms ----
+
 // Rows of [..., d] that lie one stride apart.
 bool rows_of(const Tensor& t, int64_t* rows, int64_t* stride) {
   if (t.dim() < 1 || !inner(t)) return false;
@@ -417,6 +469,10 @@ bool rows_of(const Tensor& t, int64_t* rows, int64_t* stride) {
   *rows = n;
   *stride = st;
   return true;
+}
+Tensor usable_rows(const Tensor& t) {
+  int64_t n, st;
+  return !t.defined() || rows_of(t, &n, &st) ? t : t.contiguous();
 }
 // The operands of a norm: checked against x, with their strides.
 struct NormCall {
@@ -444,191 +500,271 @@ struct NormCall {
     if (t.scalar_type() == x.scalar_type()) a.vectors_in_dtype |= bit;
     return t.data_ptr();
   }
-  float* sums(const Tensor& t, int64_t n) {
-    if (!t.defined()) return nullptr;
-    ok = ok && t.scalar_type() == at::kFloat && t.is_contiguous() && t.numel() == n && w.here(t);
-    return ptr<float>(t);
+  Tensor fresh(void** at, int64_t* stride) {   // a result like x
+    Tensor t = at::empty(x.sizes(), x.options());
+    *at = t.data_ptr();
+    *stride = a.d;
+    return t;
+  }
+  Tensor scratch_of() {
+    a.workspace_bytes = f_norm_workspace(&a);
+    Tensor ws = scratch(x, a.workspace_bytes);
+    a.workspace = ptr(ws);
+    return ws;
   }
 };
 bool norm_operand(const Tensor& x) { return x.is_cuda() && x.dim() >= 1 && dtype_of(x) >= 0; }
 
-// rms_norm(x, weight, residual, post_weight, scale, out, eps, keep) -> (y, residual_out or None, inv_rms or None, inv_rms_post or None)
-PyObject* py_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  const Tensor *x, *wt, *res, *post, *scale, *out;
-  float eps;
-  if (n != 8 || !get(o[0], &x) || !get(o[1], &wt) || !get(o[2], &res, true) || !get(o[3], &post, true) || !get(o[4], &scale, true) ||
-      !get(o[5], &out, true) || !real(o[6], &eps) || !norm_operand(*x))
-    Py_RETURN_NONE;
-  NormCall c(*x);
-  const auto st = x->scalar_type();
-  c.a.weight = c.vector(*wt, 1);
-  c.a.post_weight = c.vector(*post, 2);
-  c.a.scale = c.vector(*scale, 4);
-  if (res->defined()) {
-    if (dtype_of(*res) < 0) Py_RETURN_NONE;
-    c.a.residual_dtype = dtype_of(*res);
-    c.a.residual = c.rows(*res, res->scalar_type(), &c.a.residual_stride);
+struct Normed {
+  Tensor y, r, inv, invp;
+};
+bool norm_forward(const Tensor& x, const Tensor& wt, const Tensor& res, const Tensor& post, const Tensor& scale, const Tensor& out, float eps,
+                  bool keep, Normed* v, int* rc) {
+  NormCall c(x);
+  c.a.weight = c.vector(wt, 1);
+  c.a.post_weight = c.vector(post, 2);
+  c.a.scale = c.vector(scale, 4);
+  if (res.defined()) {
+    if (dtype_of(res) < 0) return false;
+    c.a.residual_dtype = dtype_of(res);
+    c.a.residual = c.rows(res, res.scalar_type(), &c.a.residual_stride);
   }
-  c.a.y = c.rows(*out, st, &c.a.y_stride);
-  if (!c.ok) Py_RETURN_NONE;
-  const bool keep = o[7] == Py_True;
-  Tensor y = *out, r, inv, invp;
-  if (!y.defined()) {
-    y = at::empty(x->sizes(), x->options());
-    c.a.y = y.data_ptr();
-    c.a.y_stride = c.a.d;
-  }
-  if (res->defined()) {
-    r = at::empty(x->sizes(), res->options());
-    c.a.residual_out = r.data_ptr();
+  c.a.y = c.rows(out, x.scalar_type(), &c.a.y_stride);
+  if (!c.ok) return false;
+  v->y = out.defined() ? out : c.fresh(&c.a.y, &c.a.y_stride);
+  if (res.defined()) {
+    v->r = at::empty(x.sizes(), res.options());
+    c.a.residual_out = v->r.data_ptr();
     c.a.residual_out_stride = c.a.d;
   }
-  if (keep) inv = at::empty({c.a.rows}, x->options().dtype(at::kFloat));
-  if (keep && post->defined()) invp = at::empty({c.a.rows}, x->options().dtype(at::kFloat));
+  const auto f32 = x.options().dtype(at::kFloat);
+  if (keep) v->inv = at::empty({c.a.rows}, f32);
+  if (keep && post.defined()) v->invp = at::empty({c.a.rows}, f32);
+  c.a.inv_rms = ptr<float>(v->inv);
+  c.a.inv_rms_post = ptr<float>(v->invp);
+  c.a.eps = eps;
+  *rc = f_norm(&c.a, c.w.stream());
+  return true;
+}
+// like: x, or where nothing of it is read a tensor of its shape and type
+bool norm_backward(const Tensor& like, const Tensor& wt, const Tensor& r, const Tensor& post, const Tensor& scale, const Tensor& inv,
+                   const Tensor& invp, const Tensor& dy, const Tensor& dr, variable_list* out, int* rc) {
+  NormCall c(like);
+  c.a.weight = c.vector(wt, 1);
+  c.a.post_weight = c.vector(post, 2);
+  c.a.scale = c.vector(scale, 4);
+  if (r.defined()) {
+    c.a.residual_dtype = dtype_of(r);
+    c.a.residual_out = c.rows(r, r.scalar_type(), &c.a.residual_out_stride);
+    c.a.dresidual_out = c.rows(dr, r.scalar_type(), &c.a.dresidual_out_stride);
+  }
+  c.a.dy = c.rows(dy, like.scalar_type(), &c.a.dy_stride);
   c.a.inv_rms = ptr<float>(inv);
   c.a.inv_rms_post = ptr<float>(invp);
-  c.a.eps = eps;
-  if (const int rc = f_norm(&c.a, c.w.stream())) return declined(rc);
-  return tuple_of({y, r, inv, invp});
-  END_HANDLE_TH_ERRORS
-}
-
-// rms_norm_backward(x, weight, residual_out, post_weight, scale, inv_rms, inv_rms_post, dy, dresidual_out)
-//   -> (dx, dresidual or None, dweight, dpost_weight or None, dscale or None)
-PyObject* py_norm_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  const Tensor *x, *wt, *r, *post, *scale, *inv, *invp, *dy, *dr;
-  if (n != 9 || !get(o[0], &x) || !get(o[1], &wt) || !get(o[2], &r, true) || !get(o[3], &post, true) || !get(o[4], &scale, true) ||
-      !get(o[5], &inv) || !get(o[6], &invp, true) || !get(o[7], &dy) || !get(o[8], &dr, true) || !norm_operand(*x))
-    Py_RETURN_NONE;
-  NormCall c(*x);
-  const auto st = x->scalar_type();
-  c.a.weight = c.vector(*wt, 1);
-  c.a.post_weight = c.vector(*post, 2);
-  c.a.scale = c.vector(*scale, 4);
-  if (r->defined()) {
-    if (dtype_of(*r) < 0) Py_RETURN_NONE;
-    c.a.residual_dtype = dtype_of(*r);
-    c.a.residual_out = c.rows(*r, r->scalar_type(), &c.a.residual_out_stride);
-    c.a.dresidual_out = c.rows(*dr, r->scalar_type(), &c.a.dresidual_out_stride);
-  } else if (dr->defined()) {
-    Py_RETURN_NONE;
-  }
-  c.a.dy = c.rows(*dy, st, &c.a.dy_stride);
-  c.a.inv_rms = c.sums(*inv, c.a.rows);
-  c.a.inv_rms_post = c.sums(*invp, c.a.rows);
-  if (!c.ok) Py_RETURN_NONE;
-  Tensor dx = at::empty(x->sizes(), x->options()), dres, dw = at::empty({(int64_t)c.a.d}, wt->options()), dpost, dscale;
-  c.a.dx = dx.data_ptr();
-  c.a.dx_stride = c.a.d;
-  if (r->defined()) {
+  if (!c.ok) return false;
+  Tensor dx = c.fresh(&c.a.dx, &c.a.dx_stride), dres, dw = at::empty({(int64_t)c.a.d}, wt.options()), dpost, dscale;
+  if (r.defined()) {
     // without a norm or a scale behind the block its gradient is the residual's; of one type they are one tensor
-    if (!post->defined() && !scale->defined() && r->scalar_type() == st) {
+    if (!post.defined() && !scale.defined() && r.scalar_type() == like.scalar_type()) {
       dres = dx;
     } else {
-      dres = at::empty(x->sizes(), r->options());
+      dres = at::empty(like.sizes(), r.options());
       c.a.dresidual = dres.data_ptr();
       c.a.dresidual_stride = c.a.d;
     }
   }
-  if (post->defined()) dpost = at::empty({(int64_t)c.a.d}, post->options());
-  if (scale->defined()) dscale = at::empty({(int64_t)c.a.d}, scale->options());
+  if (post.defined()) dpost = at::empty({(int64_t)c.a.d}, post.options());
+  if (scale.defined()) dscale = at::empty({(int64_t)c.a.d}, scale.options());
   c.a.dweight = dw.data_ptr(); c.a.dpost_weight = ptr(dpost); c.a.dscale = ptr(dscale);
-  const size_t need = f_norm_workspace(&c.a);
-  const Tensor ws = scratch(*x, need);
-  c.a.workspace = ptr(ws);
-  c.a.workspace_bytes = need;
-  if (const int rc = f_norm_backward(&c.a, c.w.stream())) return declined(rc);
-  return tuple_of({dx, dres, dw, dpost, dscale});
+  const Tensor ws = c.scratch_of();
+  *rc = f_norm_backward(&c.a, c.w.stream());
+  *out = {dx, dw, dres, dpost, dscale};
+  return true;
+}
+
+struct NormNode : torch::autograd::Function<NormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& wt, const Maybe& res, const Maybe& post, const Maybe& scale,
+                               double eps, int* rc) {
+    Normed v;
+    *rc = 1;
+    if (!norm_forward(x, wt, given(res), given(post), given(scale), Tensor(), (float)eps, true, &v, rc) || *rc) return {};
+    // the block's output itself is needed again only behind a norm or a scale, or where it is what is normalised
+    ctx->save_for_backward({post || scale || !res ? x : Tensor(), wt, v.r, given(post), given(scale), v.inv, v.invp});
+    ctx->saved_data["type"] = (int64_t)x.scalar_type();
+    ctx->set_materialize_grads(false);
+    if (v.r.defined()) return {v.y, v.r};
+    return {v.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor gr = grads.size() > 1 ? grads[1] : Tensor();
+    if (!grads[0].defined() && !gr.defined()) return variable_list(7);
+    const auto s = ctx->get_saved_variables();
+    const Tensor& of = s[0].defined() ? s[0] : s[2];
+    const auto type = (at::ScalarType)ctx->saved_data["type"].toInt();
+    const Tensor dy = grads[0].defined() ? usable_rows(grads[0]) : at::zeros(of.sizes(), of.options().dtype(type));
+    variable_list out;
+    int rc = 0;
+    const bool ok = norm_backward(s[0].defined() ? s[0] : dy, s[1], s[2], s[3], s[4], s[5], s[6], dy, usable_rows(gr), &out, &rc);
+    must(ok, rc, "rms_norm");
+    out.resize(7);
+    return once(std::move(out), "rms_norm");
+  }
+};
+
+// rms_norm(x, weight, residual, post_weight, scale, out, eps) -> (y, residual_out or None)
+PyObject* py_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
+  HANDLE_TH_ERRORS
+  const Tensor *x, *wt, *res, *post, *scale, *out;
+  float eps;
+  if (n != 7 || !get(o[0], &x) || !get(o[1], &wt) || !get(o[2], &res, true) || !get(o[3], &post, true) || !get(o[4], &scale, true) ||
+      !get(o[5], &out, true) || !real(o[6], &eps) || !norm_operand(*x))
+    Py_RETURN_NONE;
+  int rc = 0;
+  if (records({x, wt, res, post, scale})) {
+    if (out->defined()) Py_RETURN_NONE;
+    const variable_list v = NormNode::apply(*x, *wt, maybe(*res), maybe(*post), maybe(*scale), (double)eps, &rc);
+    return rc ? declined(rc) : tuple_of({v[0], v.size() > 1 ? v[1] : Tensor()});
+  }
+  Normed v;
+  if (!norm_forward(*x, *wt, *res, *post, *scale, *out, eps, false, &v, &rc)) Py_RETURN_NONE;
+  return rc ? declined(rc) : tuple_of({v.y, v.r});
   END_HANDLE_TH_ERRORS
 }
 
-// gated_rms_norm(x, z, weight, out, eps, groups, norm_first, keep) -> (y, inv_rms or None)
+bool gated_norm_forward(const Tensor& x, const Tensor& z, const Tensor& wt, const Tensor& out, float eps, int64_t groups, bool first, bool keep,
+                        Normed* v, int* rc) {
+  NormCall c(x);
+  if (groups <= 0 || groups > c.a.d) return false;
+  c.a.groups = (int)groups;
+  c.a.norm_first = first;
+  c.a.weight = c.vector(wt, 1);
+  c.a.z = c.rows(z, x.scalar_type(), &c.a.z_stride);
+  c.a.y = c.rows(out, x.scalar_type(), &c.a.y_stride);
+  if (!c.ok) return false;
+  v->y = out.defined() ? out : c.fresh(&c.a.y, &c.a.y_stride);
+  if (keep) v->inv = at::empty({c.a.rows, groups}, x.options().dtype(at::kFloat));
+  c.a.inv_rms = ptr<float>(v->inv);
+  c.a.eps = eps;
+  *rc = f_gated_norm(&c.a, c.w.stream());
+  return true;
+}
+
+struct GatedNormNode : torch::autograd::Function<GatedNormNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& z, const Tensor& wt, double eps, int64_t groups, bool first,
+                               int* rc) {
+    Normed v;
+    *rc = 1;
+    if (!gated_norm_forward(x, z, wt, Tensor(), (float)eps, groups, first, true, &v, rc) || *rc) return {};
+    ctx->save_for_backward({x, z, wt, v.inv});
+    ctx->saved_data["groups"] = groups;
+    ctx->saved_data["first"] = first;
+    return {v.y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    NormCall c(s[0]);
+    c.a.groups = (int)ctx->saved_data["groups"].toInt();
+    c.a.norm_first = ctx->saved_data["first"].toBool();
+    c.a.weight = c.vector(s[2], 1);
+    c.a.z = c.rows(s[1], s[0].scalar_type(), &c.a.z_stride);
+    const Tensor dy = usable_rows(grads[0]);
+    c.a.dy = c.rows(dy, s[0].scalar_type(), &c.a.dy_stride);
+    c.a.inv_rms = ptr<float>(s[3]);
+    must(c.ok, 0, "gated_rms_norm");
+    Tensor dx = c.fresh(&c.a.dx, &c.a.dx_stride), dz = c.fresh(&c.a.dz, &c.a.dz_stride), dw = at::empty({(int64_t)c.a.d}, s[2].options());
+    c.a.dweight = dw.data_ptr();
+    const Tensor ws = c.scratch_of();
+    must(true, f_gated_norm_backward(&c.a, c.w.stream()), "gated_rms_norm");
+    return once({dx, dz, dw, Tensor(), Tensor(), Tensor(), Tensor()}, "gated_rms_norm");
+  }
+};
+
+// gated_rms_norm(x, z, weight, out, eps, groups, norm_first) -> y
 PyObject* py_gated_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Tensor *x, *z, *wt, *out;
   float eps;
-  if (n != 8 || !get(o[0], &x) || !get(o[1], &z) || !get(o[2], &wt) || !get(o[3], &out, true) || !real(o[4], &eps) ||
+  if (n != 7 || !get(o[0], &x) || !get(o[1], &z) || !get(o[2], &wt) || !get(o[3], &out, true) || !real(o[4], &eps) ||
       !PyLong_CheckExact(o[5]) || !norm_operand(*x))
     Py_RETURN_NONE;
   const long groups = PyLong_AsLong(o[5]);
-  NormCall c(*x);
-  if (groups <= 0 || groups > c.a.d) Py_RETURN_NONE;
-  c.a.groups = (int)groups;
-  c.a.norm_first = o[6] == Py_True;
-  c.a.weight = c.vector(*wt, 1);
-  c.a.z = c.rows(*z, x->scalar_type(), &c.a.z_stride);
-  c.a.y = c.rows(*out, x->scalar_type(), &c.a.y_stride);
-  if (!c.ok) Py_RETURN_NONE;
-  Tensor y = *out, inv;
-  if (!y.defined()) {
-    y = at::empty(x->sizes(), x->options());
-    c.a.y = y.data_ptr();
-    c.a.y_stride = c.a.d;
+  const bool first = o[6] == Py_True;
+  int rc = 0;
+  if (records({x, z, wt})) {
+    if (out->defined()) Py_RETURN_NONE;
+    const variable_list v = GatedNormNode::apply(*x, *z, *wt, (double)eps, (int64_t)groups, first, &rc);
+    return rc ? declined(rc) : THPVariable_Wrap(v[0]);
   }
-  if (o[7] == Py_True) inv = at::empty({c.a.rows, (int64_t)groups}, x->options().dtype(at::kFloat));
-  c.a.inv_rms = ptr<float>(inv);
-  c.a.eps = eps;
-  if (const int rc = f_gated_norm(&c.a, c.w.stream())) return declined(rc);
-  return tuple_of({y, inv});
+  Normed v;
+  if (!gated_norm_forward(*x, *z, *wt, *out, eps, groups, first, false, &v, &rc)) Py_RETURN_NONE;
+  return rc ? declined(rc) : THPVariable_Wrap(v.y);
   END_HANDLE_TH_ERRORS
 }
 
-// gated_rms_norm_backward(x, z, weight, inv_rms, dy, groups, norm_first) -> (dx, dz, dweight)
-PyObject* py_gated_norm_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
-  HANDLE_TH_ERRORS
-  const Tensor *x, *z, *wt, *inv, *dy;
-  if (n != 7 || !get(o[0], &x) || !get(o[1], &z) || !get(o[2], &wt) || !get(o[3], &inv) || !get(o[4], &dy) || !PyLong_CheckExact(o[5]) ||
-      !norm_operand(*x))
-    Py_RETURN_NONE;
-  const long groups = PyLong_AsLong(o[5]);
-  NormCall c(*x);
-  if (groups <= 0 || groups > c.a.d) Py_RETURN_NONE;
-  c.a.groups = (int)groups;
-  c.a.norm_first = o[6] == Py_True;
-  c.a.weight = c.vector(*wt, 1);
-  c.a.z = c.rows(*z, x->scalar_type(), &c.a.z_stride);
-  c.a.dy = c.rows(*dy, x->scalar_type(), &c.a.dy_stride);
-  c.a.inv_rms = c.sums(*inv, c.a.rows * groups);
-  if (!c.ok) Py_RETURN_NONE;
-  Tensor dx = at::empty(x->sizes(), x->options()), dz = at::empty(x->sizes(), x->options()), dw = at::empty({(int64_t)c.a.d}, wt->options());
-  c.a.dx = dx.data_ptr(); c.a.dz = dz.data_ptr(); c.a.dweight = dw.data_ptr();
-  c.a.dx_stride = c.a.dz_stride = c.a.d;
-  const size_t need = f_norm_workspace(&c.a);
-  const Tensor ws = scratch(*x, need);
-  c.a.workspace = ptr(ws);
-  c.a.workspace_bytes = need;
-  if (const int rc = f_gated_norm_backward(&c.a, c.w.stream())) return declined(rc);
-  return tuple_of({dx, dz, dw});
-  END_HANDLE_TH_ERRORS
+// ---- conv1d + SiLU ----
+
+bool conv_operands(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& out) {
+  if (x.dim() != 3) return false;
+  const int64_t d = x.size(2);
+  const auto st = x.scalar_type();
+  return dtype_of(x) >= 0 && x.stride(2) == 1 && d > 0 && w.scalar_type() == st && w.is_contiguous() && w.dim() >= 2 && w.size(0) == d &&
+         w.numel() == d * w.size(-1) && (!bias.defined() || (shaped(bias, {d}) && bias.scalar_type() == st && bias.is_contiguous())) &&
+         (!out.defined() || (out.scalar_type() == st && out.sizes() == x.sizes() && inner(out)));
+}
+bool conv_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Tensor& out, Tensor* y, int* rc) {
+  if (!conv_operands(x, w, bias, out)) return false;
+  Where q(x);
+  if (!q.here(w) || !q.here(bias) || !q.here(out)) return false;
+  *y = out.defined() ? out : at::empty(x.sizes(), x.options());
+  *rc = f_conv(x.data_ptr(), w.data_ptr(), ptr(bias), y->data_ptr(), (int)x.size(0), (int)x.size(1), (int)x.size(2), (int)w.size(-1), dtype_of(x),
+               x.stride(0), x.stride(1), y->stride(0), y->stride(1), q.stream());
+  return true;
+}
+// What the gradient reads two channels at a time of; other views are copied once.
+Tensor usable_pairs(const Tensor& t) {
+  const bool ok = t.stride(2) == 1 && t.stride(0) % 2 == 0 && t.stride(1) % 2 == 0 &&
+                  reinterpret_cast<uintptr_t>(t.data_ptr()) % (2 * t.element_size()) == 0;
+  return ok ? t : t.contiguous();
 }
 
-// conv1d_silu_backward(x, weight, bias, dy) -> (dx, dweight, dbias or None)
-PyObject* py_conv_backward(PyObject*, PyObject* const* o, Py_ssize_t n) {
+struct ConvNode : torch::autograd::Function<ConvNode> {
+  static variable_list forward(AutogradContext* ctx, const Tensor& x, const Tensor& w, const Maybe& bias, int* rc) {
+    Tensor y;
+    *rc = 1;
+    if (!conv_forward(x, w, given(bias), Tensor(), &y, rc) || *rc) return {};
+    ctx->save_for_backward({x, w, given(bias)});
+    return {y};
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto s = ctx->get_saved_variables();
+    const Tensor x = usable_pairs(s[0]), dy = usable_pairs(grads[0]);
+    const Tensor &w = s[1], &bias = s[2];
+    Where q(x);
+    const int b = (int)x.size(0), l = (int)x.size(1), d = (int)x.size(2), taps = (int)w.size(-1);
+    Tensor dx = at::empty(x.sizes(), x.options()), dw = at::empty(w.sizes(), w.options()), db;
+    if (bias.defined()) db = at::empty({(int64_t)d}, bias.options());
+    const size_t need = f_conv_workspace(b, l, d, taps);
+    const Tensor ws = scratch(x, need);
+    must(true, f_conv_backward(x.data_ptr(), w.data_ptr(), ptr(bias), dy.data_ptr(), dx.data_ptr(), dw.data_ptr(), ptr(db), ptr(ws), need, b, l, d,
+                               taps, dtype_of(x), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1), dx.stride(0), dx.stride(1), q.stream()),
+         "conv1d_silu");
+    return once({dx, dw, db, Tensor()}, "conv1d_silu");
+  }
+};
+
+// conv1d_silu(x, weight, bias, out) -> y
+PyObject* py_conv(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
-  const Tensor *x, *w, *bias, *dy;
-  if (n != 4 || !get(o[0], &x) || !get(o[1], &w) || !get(o[2], &bias, true) || !get(o[3], &dy) || !x->is_cuda() || x->dim() != 3 ||
-      dy->dim() != 3)
-    Py_RETURN_NONE;
-  const int64_t b = x->size(0), l = x->size(1), d = x->size(2);
-  const auto st = x->scalar_type();
-  if (dtype_of(*x) < 0 || !fits(b) || !fits(l) || !fits(d) || x->stride(2) != 1 || !like3(*dy, *x) || w->scalar_type() != st ||
-      !w->is_contiguous() || w->dim() < 2 || w->size(0) != d || w->numel() != d * w->size(-1) ||
-      (bias->defined() && (!shaped(*bias, {d}) || bias->scalar_type() != st || !bias->is_contiguous())))
-    Py_RETURN_NONE;
-  Where q(*x);
-  if (!q.here(*w) || !q.here(*bias) || !q.here(*dy)) Py_RETURN_NONE;
-  const int taps = (int)w->size(-1);
-  Tensor dx = at::empty({b, l, d}, x->options()), dw = at::empty(w->sizes(), w->options()), db;
-  if (bias->defined()) db = at::empty({d}, bias->options());
-  const size_t need = f_conv_workspace((int)b, (int)l, (int)d, taps);
-  const Tensor ws = scratch(*x, need);
-  if (const int rc = f_conv_backward(x->data_ptr(), w->data_ptr(), ptr(*bias), dy->data_ptr(), dx.data_ptr(), dw.data_ptr(), ptr(db), ptr(ws),
-                                     need, (int)b, (int)l, (int)d, taps, dtype_of(*x), x->stride(0), x->stride(1), dy->stride(0),
-                                     dy->stride(1), dx.stride(0), dx.stride(1), q.stream()))
-    return declined(rc);
-  return tuple_of({dx, dw, db});
+  const Tensor *x, *w, *bias, *out;
+  if (n != 4 || !get(o[0], &x) || !get(o[1], &w) || !get(o[2], &bias, true) || !get(o[3], &out, true) || !x->is_cuda()) Py_RETURN_NONE;
+  int rc = 0;
+  Tensor y;
+  if (!out->defined() && records({x, w, bias})) {
+    const variable_list v = ConvNode::apply(*x, *w, maybe(*bias), &rc);
+    return rc ? declined(rc) : THPVariable_Wrap(v[0]);
+  }
+  if (!conv_forward(*x, *w, *bias, *out, &y, &rc)) Py_RETURN_NONE;
+  return rc ? declined(rc) : THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }
 
@@ -672,10 +808,8 @@ PyObject* py_init(PyObject*, PyObject* const* o, Py_ssize_t n) {
 
 #define FAST(f) reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(f)), METH_FASTCALL, nullptr
 PyMethodDef methods[] = {{"init", FAST(py_init)}, {"step", FAST(py_step)}, {"dt_prologue", FAST(py_dt)},
-                         {"conv1d_silu", FAST(py_conv)}, {"conv1d_silu_backward", FAST(py_conv_backward)},
-                         {"gated_scan", FAST(py_gated)}, {"gated_scan_backward", FAST(py_gated_backward)},
-                         {"gated_step", FAST(py_gated_step)}, {"rms_norm", FAST(py_norm)}, {"rms_norm_backward", FAST(py_norm_backward)},
-                         {"gated_rms_norm", FAST(py_gated_norm)}, {"gated_rms_norm_backward", FAST(py_gated_norm_backward)},
+                         {"conv1d_silu", FAST(py_conv)}, {"gated_scan", FAST(py_gated)}, {"gated_step", FAST(py_gated_step)},
+                         {"rms_norm", FAST(py_norm)}, {"gated_rms_norm", FAST(py_gated_norm)},
                          {"forward", FAST(py_forward)}, {"workspace", FAST(py_workspace)},
                          {"status_word", FAST(py_status)}, {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "ssd_b200_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};

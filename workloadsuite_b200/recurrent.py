@@ -11,7 +11,6 @@ import math
 from typing import Optional
 
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import _lib
 from .ssd import _DTYPES, _check_out, _same_device
@@ -61,41 +60,6 @@ def _check_state(name, t, x):
         raise ValueError(f"{name} must be float32 [b,d]")
 
 
-def _gated_forward(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, wait_limit_ms, keep):
-    if x.numel() == 0:      # no tokens: the state stays what it was
-        y = torch.empty_like(x) if out is None else out
-        shape = (x.shape[0], x.shape[2])
-        fin = x.new_zeros(shape, dtype=torch.float32) if initial_state is None else initial_state.clone()
-        return y, fin, x.new_empty((0,), dtype=torch.float32)
-    return _done(_lib.fast().gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, wait_limit_ms, keep), "gated_scan")
-
-
-class _GatedScan(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, input_gate, decay_gate, decay, initial_state, reset, rate, wait_limit_ms):
-        y, fin, pieces = _gated_forward(x, input_gate, decay_gate, decay, initial_state, reset, None, rate, wait_limit_ms, True)
-        ctx.save_for_backward(x, input_gate, decay_gate, decay, reset, pieces)
-        ctx.rate, ctx.has_state = rate, initial_state is not None
-        ctx.set_materialize_grads(False)
-        return y, fin
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dfin):
-        x, input_gate, decay_gate, decay, reset, pieces = ctx.saved_tensors
-        if dy is None and dfin is None:
-            return (None,) * 8
-        if x.numel() == 0:
-            return (torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(x), torch.zeros_like(decay),
-                    (torch.zeros_like(pieces.new_empty((x.shape[0], x.shape[2]))) if dfin is None else dfin.clone())
-                    if ctx.has_state else None, None, None, None)
-        dy = torch.zeros_like(x, memory_format=torch.contiguous_format) if dy is None else _rows(dy)
-        dfin = None if dfin is None else dfin.contiguous()
-        grads = _done(_lib.fast().gated_scan_backward(x, input_gate, decay_gate, decay, reset, pieces, dy, dfin, ctx.rate, ctx.has_state),
-                      "gated_scan")
-        return (*grads, None, None, None)
-
-
 def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tensor, decay: torch.Tensor,
                initial_state: Optional[torch.Tensor] = None, reset: Optional[torch.Tensor] = None,
                return_final_state: bool = False, rate: float = 8.0, out: Optional[torch.Tensor] = None,
@@ -119,11 +83,10 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     (``device_status`` 8).
     """
     rate = float(rate)
-    records = _records(x, input_gate, decay_gate, decay, initial_state)
-    if not records and wait_limit_ms == 0:
-        got = _lib.fast().gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, 0, False) if 0 < rate < math.inf else None
-        if got is not None:
-            return got[:2] if return_final_state else got[0]
+    got = _lib.fast().gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, 0) \
+        if 0 < rate < math.inf and wait_limit_ms == 0 else None
+    if got is not None:
+        return got if return_final_state else got[0]
     _check_gates("gated_scan", x, input_gate, decay_gate, decay, 3, rate)
     _same_device(x, initial_state=initial_state, reset=reset, out=out)
     if wait_limit_ms < 0:
@@ -134,14 +97,15 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     if reset is not None and (reset.shape != x.shape[:2] or reset.dtype != torch.bool):
         raise ValueError("reset must be bool [b,s]")
     if out is not None:
-        if records:
+        if _records(x, input_gate, decay_gate, decay, initial_state):
             raise ValueError("out cannot be given where a gradient is recorded")
         _check_out(out, x)
     x, input_gate, decay_gate, decay = _rows(x), _rows(input_gate), _rows(decay_gate), decay.float().contiguous()
-    if records:
-        y, fin = _GatedScan.apply(x, input_gate, decay_gate, decay, initial_state, reset, rate, int(wait_limit_ms))
+    if x.numel() == 0:      # no tokens: the state stays what it was
+        y = (x + input_gate + decay_gate) * decay.to(x.dtype) if out is None else out
+        fin = x.new_zeros((x.shape[0], x.shape[2]), dtype=torch.float32) if initial_state is None else initial_state.clone()
     else:
-        y, fin, _ = _gated_forward(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, int(wait_limit_ms), False)
+        y, fin = _done(_lib.fast().gated_scan(x, input_gate, decay_gate, decay, initial_state, reset, out, rate, int(wait_limit_ms)), "gated_scan")
     return (y, fin) if return_final_state else y
 
 
@@ -207,43 +171,6 @@ def _check_norm(name, x, eps, vectors, rows, groups=1):
         raise ValueError("groups must divide d")
 
 
-def _norm_forward(x, weight, residual, post_weight, scale, out, eps, keep):
-    if x.numel() == 0:
-        empty = x.new_empty((0,), dtype=torch.float32)
-        return (torch.empty_like(x) if out is None else out, None if residual is None else torch.empty_like(residual), empty,
-                empty if post_weight is not None else None)
-    return _done(_lib.fast().rms_norm(x, weight, residual, post_weight, scale, out, eps, keep), "rms_norm")
-
-
-class _RmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, residual, post_weight, scale, eps):
-        y, r, inv, invp = _norm_forward(x, weight, residual, post_weight, scale, None, eps, True)
-        # the block's output itself is needed again only behind a norm or a scale, or where it is what is normalised
-        outer = post_weight is not None or scale is not None
-        ctx.save_for_backward(x if outer or r is None else None, weight, r, post_weight, scale, inv, invp)
-        ctx.dtype = x.dtype
-        ctx.set_materialize_grads(False)
-        return y if r is None else (y, r)
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy, dr=None):
-        x, weight, r, post_weight, scale, inv, invp = ctx.saved_tensors
-        if dy is None and dr is None:
-            return (None,) * 6
-        like = x if x is not None else r
-        zero = lambda t: None if t is None else torch.zeros_like(t)
-        if like.numel() == 0:
-            return torch.zeros_like(like, dtype=ctx.dtype), zero(weight), zero(r), zero(post_weight), zero(scale), None
-        dy = torch.zeros(like.shape, dtype=ctx.dtype, device=like.device) if dy is None else _flat(dy)
-        if x is None:       # nothing is read of it but its shape and type
-            x = dy
-        dx, dres, dw, dpost, dscale = _done(
-            _lib.fast().rms_norm_backward(_flat(x), weight, r, post_weight, scale, inv, invp, dy, _flat(dr)), "rms_norm")
-        return dx, dw, dres, dpost, dscale, None
-
-
 def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None, residual: Optional[torch.Tensor] = None,
              post_weight: Optional[torch.Tensor] = None, scale: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None):
     """RMS norm ahead of a block, with what lies between two blocks in the same pass, on the current CUDA stream, and its gradient.
@@ -259,52 +186,29 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None,
     residual_out as it is stored.  ``eps`` None is float32's, as in ``nn.RMSNorm``.  ``out`` receives y where no gradient is recorded.
     """
     eps = _EPS if eps is None else float(eps)
-    records = _records(x, weight, residual, post_weight, scale)
-    if not records and (residual is not None or (post_weight is None and scale is None)) and 0 <= eps < math.inf:
-        got = _lib.fast().rms_norm(x, weight, residual, post_weight, scale, out, eps, False)
-        if got is not None:
-            return got[0] if residual is None else got[:2]
+    got = _lib.fast().rms_norm(x, weight, residual, post_weight, scale, out, eps) if 0 <= eps < math.inf else None
+    if got is not None:
+        return got[0] if residual is None else got
     _check_norm("rms_norm", x, eps, dict(weight=weight, post_weight=post_weight, scale=scale), dict(residual=residual, out=out))
     if residual is None and (post_weight is not None or scale is not None):
         raise ValueError("post_weight and scale apply to what is added to residual: give one")
     if residual is not None and residual.dtype not in (torch.float32, x.dtype):
         raise ValueError("residual must be float32 or in x's dtype")
     if out is not None:
-        if records:
+        if _records(x, weight, residual, post_weight, scale):
             raise ValueError("out cannot be given where a gradient is recorded")
         _check_out(out, x)
         if _flat(out) is not out:
             raise ValueError("out: rows must lie at one distance from each other")
-    vectors = [None if t is None else t.contiguous() for t in (weight, post_weight, scale)]
+    weight, post_weight, scale = (None if t is None else t.contiguous() for t in (weight, post_weight, scale))
     x, residual = _flat(x), _flat(residual)
-    if records:
-        return _RmsNorm.apply(x, vectors[0], residual, vectors[1], vectors[2], eps)
-    y, r, _, _ = _norm_forward(x, vectors[0], residual, vectors[1], vectors[2], out, eps, False)
-    return y if residual is None else (y, r)
-
-
-def _gated_norm_forward(x, z, weight, out, eps, groups, norm_first, keep):
     if x.numel() == 0:
-        return torch.empty_like(x) if out is None else out, x.new_empty((0,), dtype=torch.float32)
-    return _done(_lib.fast().gated_rms_norm(x, z, weight, out, eps, groups, norm_first, keep), "gated_rms_norm")
-
-
-class _GatedRmsNorm(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, z, weight, eps, groups, norm_first):
-        y, inv = _gated_norm_forward(x, z, weight, None, eps, groups, norm_first, True)
-        ctx.save_for_backward(x, z, weight, inv)
-        ctx.groups, ctx.norm_first = groups, norm_first
-        return y
-
-    @staticmethod
-    @once_differentiable
-    def backward(ctx, dy):
-        x, z, weight, inv = ctx.saved_tensors
-        if x.numel() == 0:
-            return torch.zeros_like(x), torch.zeros_like(z), torch.zeros_like(weight), None, None, None
-        grads = _done(_lib.fast().gated_rms_norm_backward(x, z, weight, inv, _flat(dy), ctx.groups, ctx.norm_first), "gated_rms_norm")
-        return (*grads, None, None, None)
+        for t in (post_weight, scale):
+            x = x if t is None else x * t.to(x.dtype)
+        y = x * weight.to(x.dtype) if out is None else out
+        return y if residual is None else (y, residual + x.to(residual.dtype))
+    y, r = _done(_lib.fast().rms_norm(x, weight, residual, post_weight, scale, out, eps), "rms_norm")
+    return y if residual is None else (y, r)
 
 
 def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None, groups: int = 1,
@@ -318,21 +222,19 @@ def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: 
     """
     eps = _EPS if eps is None else float(eps)
     groups, norm_first = int(groups), bool(norm_first)
-    records = _records(x, z, weight)
-    if not records and 0 <= eps < math.inf:
-        got = _lib.fast().gated_rms_norm(x, z, weight, out, eps, groups, norm_first, False)
-        if got is not None:
-            return got[0]
+    got = _lib.fast().gated_rms_norm(x, z, weight, out, eps, groups, norm_first) if 0 <= eps < math.inf else None
+    if got is not None:
+        return got
     _check_norm("gated_rms_norm", x, eps, dict(weight=weight), dict(z=z, out=out), groups)
     if z.dtype != x.dtype:
         raise ValueError("z must be in x's dtype")
     if out is not None:
-        if records:
+        if _records(x, z, weight):
             raise ValueError("out cannot be given where a gradient is recorded")
         _check_out(out, x)
         if _flat(out) is not out:
             raise ValueError("out: rows must lie at one distance from each other")
     x, z, weight = _flat(x), _flat(z), weight.contiguous()
-    if records:
-        return _GatedRmsNorm.apply(x, z, weight, eps, groups, norm_first)
-    return _gated_norm_forward(x, z, weight, out, eps, groups, norm_first, False)[0]
+    if x.numel() == 0:
+        return x * z * weight.to(x.dtype) if out is None else out
+    return _done(_lib.fast().gated_rms_norm(x, z, weight, out, eps, groups, norm_first), "gated_rms_norm")

@@ -293,29 +293,6 @@ def ssd_forward(
     return outs[0] if len(outs) == 1 else tuple(outs)
 
 
-class _ConvSilu(torch.autograd.Function):
-    @staticmethod
-    def forward(ctx, x, weight, bias):
-        ctx.save_for_backward(x, weight, bias)
-        with torch.no_grad():
-            return conv1d_silu(x, weight, bias)
-
-    @staticmethod
-    @torch.autograd.function.once_differentiable
-    def backward(ctx, dy):
-        x, weight, bias = ctx.saved_tensors
-        got = _lib.fast().conv1d_silu_backward(_pairs(x), weight, bias, _pairs(dy))
-        if got is None:
-            raise NotImplementedError("conv1d_silu: sizes outside what the kernels cover")
-        return got
-
-
-def _pairs(t: torch.Tensor) -> torch.Tensor:
-    """What the gradient's kernel reads two channels at a time of; other views are copied once."""
-    ok = t.stride(2) == 1 and t.stride(0) % 2 == 0 and t.stride(1) % 2 == 0 and t.data_ptr() % (2 * t.element_size()) == 0
-    return t if ok else t.contiguous()
-
-
 def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tensor] = None,
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """Causal depthwise conv1d + SiLU on the current CUDA stream: ``silu(conv1d(x^T)[..., :l])^T`` of
@@ -326,9 +303,6 @@ def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     in x's dtype (fp32 accumulation, one rounding).  Differentiable in x, weight and bias (where ``out`` is given no
     gradient is recorded).
     """
-    if out is None and torch.is_grad_enabled() and (x.requires_grad or weight.requires_grad or (bias is not None and bias.requires_grad)):
-        if x.is_cuda and x.dim() == 3 and x.dtype in _DTYPES and weight.shape[0] == x.shape[2]:
-            return _ConvSilu.apply(x, weight.to(x.dtype).contiguous(), None if bias is None else bias.to(x.dtype).contiguous())
     got = _lib.fast().conv1d_silu(x, weight, bias, out)
     if got is not None:
         return got
@@ -340,6 +314,11 @@ def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     _same_device(x, weight=weight, bias=bias, out=out)
     w = weight.reshape(d, -1).to(x.dtype).contiguous()
     taps = w.shape[1]
+    if out is None and torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)):
+        got = _lib.fast().conv1d_silu(x, w, None if bias is None else bias.to(x.dtype).contiguous(), None)
+        if got is None:
+            raise NotImplementedError("conv1d_silu: sizes outside what the kernels cover")
+        return got
     if bias is not None:
         if bias.shape != (d,):
             raise ValueError("bias must be [d]")
