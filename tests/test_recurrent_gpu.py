@@ -602,6 +602,41 @@ def test_two_blocks_together_and_their_gradients():
         assert (a.cpu().double() - r).abs().max() <= 6e-4 * r.abs().max()
 
 
+def test_the_model_adds_its_residuals_in_the_norms():
+    """The drop-in Model against its own layers called one by one with the sums and norms in PyTorch.  The sums are the same numbers bit by bit
+    and a norm's result may round the other way (half a step, 2^-11); two layers with a gain of some units pass that on: 2^-11 * 2 * 4."""
+    from workloadsuite_b200 import mamba_model as M
+
+    torch.manual_seed(5)
+    model = M.Model(128, 3, 4, 128, 64, 2, 64, 4).to(DEV).eval()
+    with torch.no_grad():
+        for n in [layer.norm for layer in model.layers] + [model.final_norm]:
+            n.weight.uniform_(0.5, 1.5)
+    x = torch.randn(2, 256, 128, dtype=torch.float16, device=DEV)
+    norm = torch.nn.functional.rms_norm
+    with torch.inference_mode():
+        got = model(x)
+        u = x
+        for layer in model.layers:
+            assert torch.equal(layer.norm(u, u)[1], u + u)
+            u = u + layer(u)
+        want = norm(u, (128,), model.final_norm.weight)
+        assert ((got - want).abs().max() <= 2.0 ** -8 * want.abs().max()).item()
+        seen = []
+        hook = model.layers[1].register_forward_hook(lambda m, a, out: seen.append((len(a), out.shape)))
+        again = model(x)                       # a layer that is watched is called as before
+        hook.remove()
+        assert seen == [(1, x.shape)] and (again - want).abs().max() <= 2.0 ** -8 * want.abs().max()
+    # gradients reach what they reached before: the residual stream and the norms
+    x = x.clone().requires_grad_(True)
+    y = model(x)
+    gx, gw = torch.autograd.grad(y.float().sum(), [x, model.final_norm.weight])
+    assert torch.isfinite(gx).all() and torch.isfinite(gw).all() and (gx != 0).any()
+    cpu = M.RMSNorm(128, dtype=torch.float32)
+    t = torch.randn(3, 128)
+    assert torch.equal(cpu(t), torch.nn.functional.rms_norm(t, (128,), cpu.weight)) and torch.equal(cpu(t, t)[1], t + t)
+
+
 def test_captured_forward_and_backward():
     """Two graphs, each with a forward and a backward of every operator, replayed in turn and beside each other on new inputs, while an eager
     graph of the same leaves is alive.  (PyTorch wants that one recorded on the stream that captures: its leaves' nodes keep the stream they were

@@ -5,8 +5,8 @@ Exports the reference's workload contract -- ``Model``, ``get_init_inputs()``,
 arguments, parameter names, shapes and dtypes (``model_ref.py:49-66,170-199``), so
 a ``state_dict`` moves between the two unchanged.  The SSD core
 (``SSDLayer._ssd_core``, ``model_ref.py:123-162``) runs in the sm_100a kernels of
-this package; the projections, the causal conv, the norms and the gate around it
-stay PyTorch host code, as in the reference (``model_ref.py:68-121``).
+this package, and so do the causal conv, dt, the gate and the norms with the residual
+sums ahead of them; the projections stay PyTorch's, as in the reference (``model_ref.py:68-121``).
 
 The file can be loaded by path (the reference harness does so,
 ``bench.py:104-115``): it locates its own package.
@@ -15,6 +15,7 @@ from __future__ import annotations
 
 import sys
 from pathlib import Path
+from typing import Optional
 
 import torch
 import torch.nn as nn
@@ -24,6 +25,7 @@ _PKG_PARENT = str(Path(__file__).resolve().parent.parent)
 if _PKG_PARENT not in sys.path:
     sys.path.insert(0, _PKG_PARENT)
 
+from workloadsuite_b200.recurrent import rms_norm  # noqa: E402
 from workloadsuite_b200.ssd import conv1d_silu, dt_prologue, ssd_forward  # noqa: E402
 
 
@@ -38,6 +40,11 @@ def _conv(x, weight, bias):
 
 
 @torch.compiler.disable
+def _norm(x, weight, eps, residual):
+    return rms_norm(x, weight, eps=eps, residual=residual)
+
+
+@torch.compiler.disable
 def _core(x, A_dt, B, C, dt, block_len, D, z):
     """The SSD core with the layer's skip and gate (``model_ref.py:116-118``) applied in the kernel's epilogue."""
     return ssd_forward(x, A_dt, B, C, block_len, dt=dt, D=D, z=z)
@@ -48,6 +55,21 @@ def _tma_friendly(t: torch.Tensor) -> torch.Tensor:
     per16 = 16 // t.element_size()
     ok = t.stride(-1) == 1 and all(st % per16 == 0 for st in t.stride()[:-1]) and t.data_ptr() % 16 == 0
     return t if ok else t.contiguous()
+
+
+class RMSNorm(nn.RMSNorm):
+    """``nn.RMSNorm`` in the package's kernel; with ``residual`` the norm of ``residual + x``, returned with that sum."""
+
+    def forward(self, x: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        w = self.weight
+        if (x.is_cuda and len(self.normalized_shape) == 1 and w is not None and w.dtype in (x.dtype, torch.float32)
+                and x.dtype in (torch.float16, torch.bfloat16, torch.float32) and x.shape[-1] <= 16384
+                and (residual is None or residual.dtype == x.dtype)):
+            return _norm(x, w, self.eps, residual)
+        if residual is None:
+            return super().forward(x)
+        residual = residual + x
+        return super().forward(residual), residual
 
 
 class SSDLayer(nn.Module):
@@ -74,13 +96,18 @@ class SSDLayer(nn.Module):
         self.D = nn.Parameter(torch.ones(self.n_heads, dtype=torch.float16))
         self.dt_bias = nn.Parameter(torch.zeros(self.n_heads, dtype=torch.float16) - 4.0)
         self.out_proj = nn.Linear(self.d_inner, self.d_model, bias=False, dtype=torch.float16)
-        self.norm = nn.RMSNorm(self.d_model, dtype=torch.float16)
+        self.norm = RMSNorm(self.d_model, dtype=torch.float16)
 
-    def forward(self, u: torch.Tensor) -> torch.Tensor:
+    def forward(self, u: torch.Tensor, residual: Optional[torch.Tensor] = None):
+        """The block's output; with ``residual`` of what ``residual + u`` is, returned with that sum (u being the output of the
+        block before): the sum costs no pass of its own."""
         batch, seq_len, _ = u.shape
         if seq_len % self.block_len != 0:
             raise ValueError(f"seq_len {seq_len} is not a multiple of block_len {self.block_len}")
-        u = self.norm(u)
+        if residual is None:
+            u = self.norm(u)
+        else:
+            u, residual = self.norm(u, residual)
         zxbcdt = self.in_proj(u)
         gn = self.n_groups * self.d_state
         x, z, B, C, dt = torch.split(zxbcdt, [self.d_inner, self.d_inner, gn, gn, self.n_heads], dim=-1)
@@ -94,7 +121,17 @@ class SSDLayer(nn.Module):
 
         z = _tma_friendly(z.unflatten(-1, (self.n_heads, self.d_head)))     # a view of the projection output
         Y = _core(x, A_dt, B, C, dt, self.block_len, self.D, z)             # (Y + x D) silu(z), model_ref.py:116-118
-        return self.out_proj(Y.view(batch, seq_len, self.d_inner))
+        Y = self.out_proj(Y.view(batch, seq_len, self.d_inner))
+        return Y if residual is None else (Y, residual)
+
+
+def _hooked(module: nn.Module) -> bool:
+    return bool(module._forward_hooks or module._forward_pre_hooks or module._backward_hooks or module._backward_pre_hooks)
+
+
+def _takes_residual(layer: nn.Module) -> bool:
+    """A layer that somebody watches, or has put in another's place, is called as the reference calls it: with one tensor, for one."""
+    return type(layer) is SSDLayer and type(layer.norm) is RMSNorm and not _hooked(layer) and not _hooked(layer.norm)
 
 
 class Model(nn.Module):
@@ -108,12 +145,23 @@ class Model(nn.Module):
         self.layers = nn.ModuleList(
             [SSDLayer(d_model, n_heads, d_state, d_head, n_groups, block_len, conv_kernel) for _ in range(n_layers)]
         )
-        self.final_norm = nn.RMSNorm(d_model, dtype=torch.float16)
+        self.final_norm = RMSNorm(d_model, dtype=torch.float16)
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
+        out = None      # of the block before, not yet added to x
         for layer in self.layers:
-            x = x + layer(x)
-        return self.final_norm(x)
+            if out is None:
+                out = layer(x)
+            elif _takes_residual(layer):
+                out, x = layer(out, x)
+            else:
+                x = x + out
+                out = layer(x)
+        if out is None:
+            return self.final_norm(x)
+        if type(self.final_norm) is RMSNorm and not _hooked(self.final_norm):
+            return self.final_norm(out, x)[0]
+        return self.final_norm(x + out)
 
 
 # production configuration of the reference (model_ref.py:211-221)
