@@ -369,7 +369,7 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     ptx::mbar_init(&sh.full[1], 1);
     ptx::fence_mbar_init();
     asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words)
-    for (int s = 0; s < 2; ++s) send_for<T, TMA, 3, kTile>(p, maps, &sh.which[s], &sh.full[s], s, stages + s * kStage, false);
+    send_for<T, TMA, 3, kTile>(p, maps, &sh.which[0], &sh.full[0], 0, stages, false);
   }
   __syncthreads();
 
@@ -388,6 +388,9 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
+    // (the second number when every CTA has its first: tiles of one sequence that are worked on at a time lie closer together)
+    if (turn == 0 && threadIdx.x == 32 * (kRuns - 1))
+      send_for<T, TMA, 3, kTile>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, false);
     const int4 which = sh.which[s];
     if (which.x < 0) break;
     const int k = which.x, unit = which.y, strip = which.z, b = which.w;
@@ -524,7 +527,7 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
     ptx::mbar_init(&sh.full[1], 1);
     ptx::fence_mbar_init();
     asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words)
-    for (int s = 0; s < 2; ++s) send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s], &sh.full[s], s, stages + s * kStage, true);
+    send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[0], &sh.full[0], 0, stages, true);
   }
   __syncthreads();
 
@@ -555,6 +558,9 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
+    // (the second number when every CTA has its first: tiles of one sequence that are worked on at a time lie closer together)
+    if (turn == 0 && threadIdx.x == 32 * (kRuns - 1))
+      send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, true);
     const int4 which = sh.which[s];
     if (which.x < 0) break;
     const int kb = which.x, k = p.tiles - 1 - kb, unit = which.y, strip = which.z, b = which.w;
