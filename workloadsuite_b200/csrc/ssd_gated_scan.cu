@@ -53,6 +53,7 @@ struct Scan {
   float rate;
   int batch, seqlen, channels, strips, tiles, npieces;
   unsigned total;                // tiles of all sequences
+  int early;                     // a forward's tile is sent for two tiles ahead, not half a one
   int64_t xs[2], is[2], rs[2], ys[2], dys[2], dxs[2], dis[2], drs[2], ms[2];
 };
 
@@ -388,8 +389,7 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
-    // (the second number when every CTA has its first: tiles of one sequence that are worked on at a time lie closer together)
-    if (turn == 0 && threadIdx.x == 32 * (kRuns - 1))
+    if (p.early && turn == 0 && threadIdx.x == 32 * (kRuns - 1))   // (when every CTA has its first)
       send_for<T, TMA, 3, kTile>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, false);
     const int4 which = sh.which[s];
     if (which.x < 0) break;
@@ -398,13 +398,9 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     const int here = min(L, p.seqlen - t0);   // tokens of this run that are there
     const Lane ln(strip, p.channels);
     const int64_t first = (int64_t)unit * p.tiles;
-    if constexpr (!TMA && kLate) {
-      asm volatile("cp.async.wait_group 0;" ::: "memory");
-      __syncthreads();
-      wait_for(p, sh, &sh.full[s ^ 1], (turn + 1) >> 1 & 1);
-      fetch(s ^ 1);
-    } else if constexpr (!TMA) {
-      fetch(s);
+    if constexpr (!TMA) {
+      if constexpr (kLate) asm volatile("cp.async.wait_group 0;" ::: "memory");
+      else fetch(s);
       __syncthreads();
     }
     const Raw* const raw = reinterpret_cast<const Raw*>(stage + w * L * kStrip) + lane;
@@ -464,8 +460,15 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     run[w][lane] = own;
     __syncthreads();
 
-    // (the tile's inputs have been read)
-    if (threadIdx.x == 32 * (kRuns - 1)) send_for<T, TMA, 3, kTile>(p, maps, &sh.which[s], &sh.full[s], turn + 2, stage, false);
+    // (the inputs of this tile and of the one before have been read)
+    if (threadIdx.x == 32 * (kRuns - 1)) {
+      const int to = p.early ? s : s ^ 1;
+      send_for<T, TMA, 3, kTile>(p, maps, &sh.which[to], &sh.full[to], p.early ? turn + 2 : turn + 1, stages + to * kStage, false);
+    }
+    if constexpr (!TMA && kLate) {
+      wait_for(p, sh, &sh.full[s ^ 1], (turn + 1) >> 1 & 1);
+      fetch(s ^ 1);
+    }
     const bool last = k == p.tiles - 1;
     Share tile = {};
     if (w == 0) {
@@ -558,9 +561,6 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
-    // (the second number when every CTA has its first: tiles of one sequence that are worked on at a time lie closer together)
-    if (turn == 0 && threadIdx.x == 32 * (kRuns - 1))
-      send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, true);
     const int4 which = sh.which[s];
     if (which.x < 0) break;
     const int kb = which.x, k = p.tiles - 1 - kb, unit = which.y, strip = which.z, b = which.w;
@@ -637,7 +637,7 @@ if (marks == 0) {
     __syncthreads();
 
     // (the inputs of the tile before have been read)
-    if (turn > 0 && threadIdx.x == 32 * (kRuns - 1))
+    if (threadIdx.x == 32 * (kRuns - 1))
       send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true);
     if constexpr (!TMA && kLate) {
       wait_for(p, sh, &sh.full[s ^ 1], (turn + 1) >> 1 & 1);
@@ -864,6 +864,10 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   using Fwd = Geometry<T, false>;
   using Bwd = Geometry<T, true>;
   const unsigned grid = std::min(p.total, 148u * (grad ? Bwd::kCtas : Fwd::kCtas));
+  // Where many tiles of one sequence are worked on at a time their numbers are taken as late as their inputs allow, so that a tile does not
+  // wait for one that is started after it: 131 072 x 2 048 bf16 (9 at a time) 494 us, taken two tiles ahead 538.  With fewer the
+  // inputs' way counts for more: 8 x 2 048 x 2 048 (1) 62 and 66, 3 x 1 021 x 1 536 fp16 (4) 16.6 and 17.6.  (Copies by threads are late ones.)
+  p.early = grid <= 6 * z.units && (tma || sizeof(T) == 2);
   auto go = [&](auto kernel, int threads, size_t smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)SSD_ERR_CUDA;
     if (!z.words && !z.rates) return launch(kernel, grid, threads, smem, stream, p, maps);
