@@ -32,12 +32,13 @@ constexpr int kStrip = 64, kPiece = 64;
 // tokens 87, with three CTAs of 8 runs of 8 72; gradient 146 us, with 16 runs of 4 244).
 template <typename T, bool GRAD> struct Geometry;
 template <typename T> struct Geometry<T, false> {
-  static constexpr int kRun = sizeof(T) == 2 ? 16 : 8, kRuns = sizeof(T) == 2 ? 8 : 16, kCtas = sizeof(T) == 2 ? 2 : 1;
+  static constexpr int kRun = sizeof(T) == 2 ? 16 : 8, kRuns = 8, kCtas = 2;
 };
 template <typename T> struct Geometry<T, true> {
   static constexpr int kRun = sizeof(T) == 2 ? 8 : 4, kRuns = sizeof(T) == 2 ? 8 : 16, kCtas = sizeof(T) == 2 ? 2 : 1;
 };
-constexpr int kTile = 128, kTileGrad = kPiece;   // tokens of a tile
+constexpr int kTileGrad = kPiece;   // tokens of a tile
+constexpr int tile_of(bool fp32) { return fp32 ? 64 : 128; }
 
 struct Scan {
   const void *x, *i, *r, *dy;
@@ -358,7 +359,7 @@ template <typename T, bool TMA>
 __global__ void __launch_bounds__(32 * Geometry<T, false>::kRuns, Geometry<T, false>::kCtas)
 gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps maps) {
   using Raw = typename Two<T>::Raw;
-  constexpr int L = Geometry<T, false>::kRun, kRuns = Geometry<T, false>::kRuns, kStage = (int)stage_numbers(3, kTile);
+  constexpr int L = Geometry<T, false>::kRun, kRuns = Geometry<T, false>::kRuns, kTile = tile_of(sizeof(T) == 4), kStage = (int)stage_numbers(3, kTile);
   static_assert(L * kRuns == kTile && kPiece % L == 0, "runs make a tile, pieces start at runs");
   extern __shared__ __align__(128) unsigned char smem[];
   T* const stages = reinterpret_cast<T*>(smem);
@@ -775,7 +776,7 @@ struct Sizes {
 };
 Sizes sizes_of(const SsdGatedScanArgs& a, bool grad) {
   Sizes z;
-  const int tile = grad ? kTileGrad : kTile;
+  const int tile = grad ? kTileGrad : tile_of(a.dtype == SSD_DTYPE_F32);
   z.tiles = (a.seqlen + (int64_t)tile - 1) / tile;
   z.units = (int64_t)a.batch * strips_of(a.channels);
   z.words = z.tiles == 1 ? 0 : 256 + z.units * z.tiles * kStrip * 12;
@@ -856,7 +857,7 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   p.total = (unsigned)(z.tiles * z.units);
   Maps maps = {};
   if (tma) {
-    const int tile = grad ? kTileGrad : kTile;
+    const int tile = grad ? kTileGrad : tile_of(sizeof(T) == 4);
     tma = operand_map<T>(&maps.at[0], a.x, a, p.xs, tile) && operand_map<T>(&maps.at[1], a.input_gate, a, p.is, tile) &&
           operand_map<T>(&maps.at[2], a.decay_gate, a, p.rs, tile) &&
           (!grad || operand_map<T>(&maps.at[3], a.dy, a, p.dys, tile));
@@ -878,7 +879,7 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
     return launch_early(kernel, grid, threads, smem, stream, p, maps);
   };
   if (!grad) {
-    const size_t smem = 2 * stage_numbers(3, kTile) * sizeof(T) + sizeof(Shared<Fwd::kRuns, 1>);
+    const size_t smem = 2 * stage_numbers(3, tile_of(sizeof(T) == 4)) * sizeof(T) + sizeof(Shared<Fwd::kRuns, 1>);
     return tma ? go(gated_scan_kernel<T, true>, 32 * Fwd::kRuns, smem) : go(gated_scan_kernel<T, false>, 32 * Fwd::kRuns, smem);
   }
   const size_t smem = 2 * stage_numbers(4, kTileGrad) * sizeof(T) + sizeof(Shared<Bwd::kRuns, 2>);
