@@ -287,10 +287,13 @@ typedef struct SsdGatedScanArgs {
   float* dinitial_state;        /* [b,d]    fp32 contiguous, or NULL */
   void* workspace;              /* ssd_b200_gated_scan_workspace_bytes() bytes, 256-byte aligned; this call's alone while it runs */
   size_t workspace_bytes;
-  int32_t* status;              /* device int32, or NULL: 8 where a wait between tiles ran out */
+  int32_t* status;              /* device int32, or NULL: 8 (1) where a wait between tiles (for a transfer) ran out */
   float rate;                   /* > 0 */
   int32_t batch, seqlen, channels, dtype;
   int32_t wait_limit_ms;        /* 0: about one second */
+  int32_t inject_lost_tile;     /* testing the give-up path: the first CTA leaves without working, so those behind it in its sequence run into the
+                                   bound of their waits, report status 8 and leave; the results are then incomplete */
+  int32_t reserved;
   int64_t x_stride[2], input_gate_stride[2], decay_gate_stride[2], reset_stride[2], y_stride[2];
   int64_t dy_stride[2], dx_stride[2], dinput_gate_stride[2], ddecay_gate_stride[2];
 } SsdGatedScanArgs;
@@ -361,12 +364,13 @@ int ssd_b200_gated_rms_norm_backward(const SsdNormArgs* args, void* stream);
 
 /* Gradient of ssd_b200_conv1d_silu(): dx [batch, seqlen, channels] (strided like x), dweight [channels, taps] and dbias [channels]
  * (NULL with bias NULL) in `dtype`, of dy.  x, weight and bias are the forward's.  workspace:
- * ssd_b200_conv1d_silu_workspace_bytes() bytes, 16-byte aligned. */
+ * ssd_b200_conv1d_silu_workspace_bytes() bytes, 16-byte aligned.  status: device int32 or NULL (1: a wait for a transfer ran out). */
 size_t ssd_b200_conv1d_silu_workspace_bytes(int32_t batch, int32_t seqlen, int32_t channels, int32_t taps);
 int ssd_b200_conv1d_silu_backward(const void* x, const void* weight, const void* bias, const void* dy, void* dx, void* dweight,
                                   void* dbias, void* workspace, size_t workspace_bytes, int32_t batch, int32_t seqlen,
                                   int32_t channels, int32_t taps, int32_t dtype, int64_t x_stride_b, int64_t x_stride_l,
-                                  int64_t dy_stride_b, int64_t dy_stride_l, int64_t dx_stride_b, int64_t dx_stride_l, void* stream);
+                                  int64_t dy_stride_b, int64_t dy_stride_l, int64_t dx_stride_b, int64_t dx_stride_l,
+                                  int32_t* status, void* stream);
 
 /* Whole forward with HOST buffers: copies X/A/B/C (and dt, initial_state when
  * given) from host memory, runs the forward and copies Y (and final_state) back,

@@ -120,7 +120,7 @@ def test_norms_refuse_on_the_host(lib):
 
 def test_conv_gradient_refuses_on_the_host(lib):
     def grad(x=P, w=P, bias=P, dy=P, dx=P, dw=P, db=P, ws=P, nbytes=1 << 40, b=2, s=10, c=16, taps=4, dtype=_lib.DTYPE_BF16, strides=(160, 16) * 3):
-        return lib.ssd_b200_conv1d_silu_backward(x, w, bias, dy, dx, dw, db, ws, nbytes, b, s, c, taps, dtype, *strides, None)
+        return lib.ssd_b200_conv1d_silu_backward(x, w, bias, dy, dx, dw, db, ws, nbytes, b, s, c, taps, dtype, *strides, None, None)
 
     for k in ("x", "w", "dy", "dx", "dw", "db"):
         assert grad(**{k: None}) == -1

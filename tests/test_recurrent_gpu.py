@@ -329,6 +329,39 @@ def test_gated_scan_offsets_past_32_bits():
     assert ((fin - fin2).abs() <= 1e-4 * fin2.abs().clamp_min(1e-2)).all()
 
 
+def test_a_wait_between_tiles_that_runs_out_is_reported_and_the_next_call_is_fine():
+    """Made on the host, without a fault: the first CTA leaves without working, so the tiles behind its own give up after 20 ms."""
+    import ctypes as C
+
+    from workloadsuite_b200 import _lib
+
+    lib, (b, s, d) = _lib.load(), (2, 3000, 128)
+    v = scan_inputs(b, s, d, torch.bfloat16, False, False, seed=8)
+    y, status = torch.zeros_like(v["x"]), torch.zeros(1, dtype=torch.int32, device=DEV)
+    pieces = torch.zeros(b, (s + 63) // 64, d, device=DEV)
+    grads, dd = [torch.zeros_like(v["x"]) for _ in range(3)], torch.zeros(d, device=DEV)
+    a = _lib.GatedScanArgs()
+    a.x, a.input_gate, a.decay_gate, a.decay = (v[k].data_ptr() for k in ("x", "i", "r", "decay"))
+    a.y, a.pieces, a.status, a.dy, a.ddecay = y.data_ptr(), pieces.data_ptr(), status.data_ptr(), v["dy"].data_ptr(), dd.data_ptr()
+    a.dx, a.dinput_gate, a.ddecay_gate = (g.data_ptr() for g in grads)
+    a.rate, a.batch, a.seqlen, a.channels, a.dtype, a.wait_limit_ms = 8.0, b, s, d, _lib.DTYPE_BF16, 20
+    for f in ("x", "input_gate", "decay_gate", "y", "dy", "dx", "dinput_gate", "ddecay_gate"):
+        setattr(a, f + "_stride", (C.c_int64 * 2)(s * d, d))
+    stream = C.c_void_p(torch.cuda.current_stream().cuda_stream)
+    for call, back in ((lib.ssd_b200_gated_scan, 0), (lib.ssd_b200_gated_scan_backward, 1)):
+        ws = torch.empty(lib.ssd_b200_gated_scan_workspace_bytes(C.byref(a), back), dtype=torch.uint8, device=DEV)
+        a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+        for inject, want in ((1, 8), (0, 0)):
+            status.zero_()
+            a.inject_lost_tile = inject
+            assert call(C.byref(a), stream) == 0
+            torch.cuda.synchronize()
+            assert status.item() == want, (back, inject)
+    ref = scan_reference(dict(v, dh=torch.zeros(b, d)))
+    check(y, ref["y"], ref["m_y"], s, "y")
+    check(grads[0], ref["dx"], ref["m_dx"], s, "dx")
+
+
 # ---- norms ----------------------------------------------------------------------------------------------
 
 def unit(v, eps):

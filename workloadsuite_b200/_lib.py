@@ -76,7 +76,7 @@ class GatedScanArgs(C.Structure):
         "x input_gate decay_gate decay initial_state reset y final_state pieces dy dfinal_state dx dinput_gate ddecay_gate ddecay "
         "dinitial_state workspace",
         [("workspace_bytes", C.c_size_t), ("status", C.c_void_p), ("rate", C.c_float),
-         *_ints("batch seqlen channels dtype wait_limit_ms"),
+         *_ints("batch seqlen channels dtype wait_limit_ms inject_lost_tile reserved"),
          *[(n + "_stride", C.c_int64 * 2) for n in "x input_gate decay_gate reset y dy dx dinput_gate ddecay_gate".split()]])
 
 
@@ -154,7 +154,7 @@ def load(build_if_missing: bool = True) -> C.CDLL:
     lib.ssd_b200_conv1d_silu_workspace_bytes.restype = C.c_size_t
     lib.ssd_b200_conv1d_silu_workspace_bytes.argtypes = [C.c_int32] * 4
     lib.ssd_b200_conv1d_silu_backward.restype = C.c_int
-    lib.ssd_b200_conv1d_silu_backward.argtypes = [C.c_void_p] * 8 + [C.c_size_t] + [C.c_int32] * 5 + [C.c_int64] * 6 + [C.c_void_p]
+    lib.ssd_b200_conv1d_silu_backward.argtypes = [C.c_void_p] * 8 + [C.c_size_t] + [C.c_int32] * 5 + [C.c_int64] * 6 + [C.c_void_p] * 2
     lib.ssd_b200_gated_scan_workspace_bytes.restype = C.c_size_t
     lib.ssd_b200_gated_scan_workspace_bytes.argtypes = [C.POINTER(GatedScanArgs), C.c_int32]
     for f in (lib.ssd_b200_gated_scan, lib.ssd_b200_gated_scan_backward):

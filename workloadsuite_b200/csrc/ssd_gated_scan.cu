@@ -54,6 +54,7 @@ struct Scan {
   float rate;
   int batch, seqlen, channels, strips, tiles, npieces;
   unsigned total;                // tiles of all sequences
+  int inject;
   int early;                     // a forward's tile is sent for two tiles ahead, not half a one
   int64_t xs[2], is[2], rs[2], ys[2], dys[2], dxs[2], dis[2], drs[2], ms[2];
 };
@@ -156,7 +157,7 @@ struct Shared {
   Share run[2][SIDES][RUNS][32];    // of the runs, tiles in turn; the gradient's other side is that of the way back
   Share seen[RUNS][32];             // of the tiles before this one, the nearest first
   int4 which[2];                    // place in its sequence (-1: there is no tile left), unit, strip, batch entry
-  int dead;                         // a wait ran out: no further one
+  int dead;                         // a wait ran out: no further one, and no further tile
   alignas(8) uint64_t full[2];
 };
 
@@ -201,6 +202,15 @@ __device__ __forceinline__ void wait_for(const Scan& p, S& sh, uint64_t* full, u
       return;
     }
   }
+}
+
+// Behind a wait that ran out the CTA leaves, once its own transfers have ended or the limit has passed again (one thread).
+template <typename S>
+__device__ __forceinline__ void drain(const Scan& p, S& sh, unsigned turn) {
+  const long long t0 = clock64();
+  for (unsigned t = turn; t < turn + 2; ++t)
+    while (!ptx::mbar_try_wait(&sh.full[t & 1], t >> 1 & 1) && clock64() - t0 < p.wait_clocks) {
+    }
 }
 
 // One operand's tile where TMA cannot read it (rows that do not start on 16 bytes), by all threads: fp32 by copies that are waited for
@@ -390,6 +400,7 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
+    if (p.inject && blockIdx.x == 0) break;   // (SsdGatedScanArgs::inject_lost_tile)
     if (p.early && turn == 0 && threadIdx.x == 32 * (kRuns - 1))   // (when every CTA has its first)
       send_for<T, TMA, 3, kTile>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, false);
     const int4 which = sh.which[s];
@@ -459,7 +470,10 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     }
     auto& run = sh.run[s][0];
     run[w][lane] = own;
-    __syncthreads();
+    if (__syncthreads_or(*(volatile int*)&sh.dead)) {
+      if (threadIdx.x == 0) drain(p, sh, turn);
+      break;
+    }
 
     // (the inputs of this tile and of the one before have been read)
     if (threadIdx.x == 32 * (kRuns - 1)) {
@@ -562,6 +576,7 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
+    if (p.inject && blockIdx.x == 0) break;   // (SsdGatedScanArgs::inject_lost_tile)
     const int4 which = sh.which[s];
     if (which.x < 0) break;
     const int kb = which.x, k = p.tiles - 1 - kb, unit = which.y, strip = which.z, b = which.w;
@@ -635,7 +650,10 @@ if (marks == 0) {
     auto &run = sh.run[s][0], &back = sh.run[s][1];
     run[w][lane] = own;
     back[w][lane] = {own.P, c};
-    __syncthreads();
+    if (__syncthreads_or(*(volatile int*)&sh.dead)) {
+      if (threadIdx.x == 0) drain(p, sh, turn);
+      break;
+    }
 
     // (the inputs of the tile before have been read)
     if (threadIdx.x == 32 * (kRuns - 1))
@@ -821,6 +839,7 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   p.status = a.status;
   p.wait_clocks = a.wait_limit_ms > 0 ? (long long)a.wait_limit_ms * 2000000LL : 2000000000LL;
   p.rate = a.rate;
+  p.inject = a.inject_lost_tile;
   p.batch = a.batch; p.seqlen = a.seqlen; p.channels = a.channels;
   p.strips = strips_of(a.channels); p.tiles = (int)z.tiles; p.npieces = (a.seqlen + kPiece - 1) / kPiece;
   char* ws = static_cast<char*>(a.workspace);

@@ -746,7 +746,8 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
     const size_t need = f_conv_workspace(b, l, d, taps);
     const Tensor ws = scratch(x, need);
     must(true, f_conv_backward(x.data_ptr(), w.data_ptr(), ptr(bias), dy.data_ptr(), dx.data_ptr(), dw.data_ptr(), ptr(db), ptr(ws), need, b, l, d,
-                               taps, dtype_of(x), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1), dx.stride(0), dx.stride(1), q.stream()),
+                               taps, dtype_of(x), x.stride(0), x.stride(1), dy.stride(0), dy.stride(1), dx.stride(0), dx.stride(1),
+                               ptr<int32_t>(status_word(q.dev.index())), q.stream()),
          "conv1d_silu");
     return once({dx, dw, db, Tensor()}, "conv1d_silu");
   }
