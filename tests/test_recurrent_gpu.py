@@ -262,6 +262,50 @@ def test_gated_scan_step(dtype, b, d):
     assert (wide[:, 0] == 0).all() and (wide[:, d + 1:] == 0).all()
 
 
+def test_views_of_any_layout_are_taken():
+    """Channels that do not lie side by side, one channel of any stride, expanded batches, rows that do not lie at one distance."""
+    v = scan_inputs(3, 70, 16, torch.float16, True, False, seed=6)
+    want = W().gated_scan(v["x"], v["i"], v["r"], v["decay"], reset=v["reset"])
+    turned = [v[k].transpose(1, 2).contiguous().transpose(1, 2) for k in ("x", "i", "r")]
+    assert turned[0].stride(-1) != 1
+    assert torch.equal(W().gated_scan(*turned, v["decay"].double().float(), reset=v["reset"].t().contiguous().t()), want)
+    assert torch.equal(W().gated_scan_step(*(t[:, 5] for t in turned), v["decay"], torch.zeros(3, 16, device=DEV)),
+                       W().gated_scan_step(*(v[k][:, 5] for k in ("x", "i", "r")), v["decay"], torch.zeros(3, 16, device=DEV)))
+    one = [t[..., :1] for t in turned]
+    assert one[0].stride(-1) != 1
+    got = W().gated_scan(*one, v["decay"][:1], reset=v["reset"])
+    assert ((got - want[..., :1]).abs() <= 2.0 ** -10 * want[..., :1].abs()).all()
+    wide = [t[:1].expand(3, 70, 16) for t in (v["x"], v["i"], v["r"])]
+    assert torch.equal(W().gated_scan(*wide, v["decay"])[2], W().gated_scan(*(t[:1] for t in wide), v["decay"])[0])
+    x, w = torch.randn(4, 6, 24, device=DEV), torch.randn(24, device=DEV)
+    n = W().rms_norm(x, w)
+    assert torch.equal(W().rms_norm(x.transpose(0, 1), w), n.transpose(0, 1)) and torch.equal(W().rms_norm(x[:, ::2], w), n[:, ::2])
+    assert torch.equal(W().rms_norm(x.transpose(1, 2).contiguous().transpose(1, 2), w), n)
+    assert torch.equal(W().gated_rms_norm(x[:1].expand(4, 6, 24), x[1:2].expand(4, 6, 24), w)[3], W().gated_rms_norm(x[0], x[1], w))
+    x = x.requires_grad_(True)
+    a, = torch.autograd.grad(W().rms_norm(x.transpose(0, 1), w).sum(), [x])
+    b, = torch.autograd.grad(W().rms_norm(x, w), [x], [torch.ones_like(n)])
+    assert torch.equal(a, b)
+
+
+def test_gradients_are_not_differentiable_and_say_so():
+    v = scan_inputs(1, 8, 16, torch.float32, False, False, seed=2)
+    x = v["x"].requires_grad_(True)
+    w, cw = torch.ones(16, device=DEV, requires_grad=True), torch.ones(16, 1, 2, device=DEV)
+    for y in (W().gated_scan(x, v["i"], v["r"], v["decay"]), W().rms_norm(x, w), W().rms_norm(x, w, residual=x)[0], W().gated_rms_norm(x, v["i"], w),
+              W().conv1d_silu(x, cw)):
+        g, = torch.autograd.grad(y.square().sum(), [x], create_graph=True)
+        with pytest.raises(RuntimeError, match="not twice differentiable"):
+            g.sum().backward()
+    # an operand that is changed after the call is noticed
+    a = x.detach().clone().requires_grad_(True)
+    b = a * 1
+    y = W().rms_norm(b, w)
+    b.mul_(2)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        y.sum().backward()
+
+
 def test_gated_scan_of_no_tokens():
     x = torch.zeros(2, 0, 8, device=DEV)
     decay = torch.zeros(8, device=DEV)

@@ -264,7 +264,7 @@ bool fits(int64_t n) { return n > 0 && n <= 0x7fffffff; }
 bool plain32(const Tensor& t, std::initializer_list<int64_t> s) {
   return !t.defined() || (t.scalar_type() == at::kFloat && shaped(t, s) && t.is_contiguous());
 }
-bool like3(const Tensor& t, const Tensor& x) { return t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && t.stride(2) == 1; }
+bool like3(const Tensor& t, const Tensor& x) { return t.scalar_type() == x.scalar_type() && t.sizes() == x.sizes() && inner(t); }
 void two(const Tensor& t, int64_t* st) {
   if (!t.defined()) return;
   st[0] = t.stride(0);
@@ -296,7 +296,7 @@ variable_list once(variable_list grads, const char* what) {
   if (!at::GradMode::is_enabled()) return grads;
   variable_list there;
   for (Tensor& g : grads)
-    if (g.defined()) there.push_back(g.detach());
+    if (g.defined()) there.push_back(g.detach().requires_grad_(true));
   auto error = std::make_shared<torch::autograd::DelayedError>(std::string(what) + " is not twice differentiable", (int)there.size());
   there = (*error)(std::move(there));
   size_t n = 0;
@@ -311,7 +311,7 @@ variable_list once(variable_list grads, const char* what) {
 bool gated_args(const Tensor& x, const Tensor& i, const Tensor& r, const Tensor& decay, const Tensor& init, const Tensor& reset, float rate,
                 const Where& w, SsdGatedScanArgs* a) {
   const int64_t b = x.size(0), s = x.size(1), d = x.size(2);
-  if (!fits(b) || !fits(s) || !fits(d) || x.stride(2) != 1 || !like3(i, x) || !like3(r, x) || decay.scalar_type() != at::kFloat ||
+  if (!fits(b) || !fits(s) || !fits(d) || !inner(x) || !like3(i, x) || !like3(r, x) || decay.scalar_type() != at::kFloat ||
       !shaped(decay, {d}) || !decay.is_contiguous() || !plain32(init, {b, d}) ||
       (reset.defined() && (reset.scalar_type() != at::kBool || !shaped(reset, {b, s}))) || !w.here(i) || !w.here(r) || !w.here(decay) ||
       !w.here(init) || !w.here(reset))
@@ -434,7 +434,7 @@ PyObject* py_gated_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
       r->dim() != 2 || dtype_of(*x) < 0)
     Py_RETURN_NONE;
   const int64_t b = x->size(0), d = x->size(1);
-  auto like = [&](const Tensor& t) { return t.scalar_type() == x->scalar_type() && t.sizes() == x->sizes() && t.stride(1) == 1; };
+  auto like = [&](const Tensor& t) { return t.scalar_type() == x->scalar_type() && t.sizes() == x->sizes() && inner(t); };
   if (!fits(b) || !fits(d) || !like(*x) || !like(*i) || !like(*r) || decay->scalar_type() != at::kFloat || !shaped(*decay, {d}) ||
       !decay->is_contiguous() || !plain32(*state, {b, d}) || !plain32(*state_out, {b, d}) || (out->defined() && (out->dim() != 2 || !like(*out))))
     Py_RETURN_NONE;

@@ -27,7 +27,7 @@ def _need_cuda(name: str, x: torch.Tensor):
 
 def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """A tensor whose channels do not lie side by side is copied once; anything else stays the view it is."""
-    return t if t is None or t.stride(-1) == 1 else t.contiguous()
+    return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
 def _done(got, name: str):
@@ -144,7 +144,7 @@ _EPS = torch.finfo(torch.float32).eps     # what nn.RMSNorm takes where none is 
 def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """[..., d] whose rows do not lie at one distance is copied once."""
     if t is None or t.dim() < 2:
-        return t if t is None or t.stride(-1) == 1 else t.contiguous()
+        return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
     try:
         t.view(-1, t.shape[-1])
     except RuntimeError:
