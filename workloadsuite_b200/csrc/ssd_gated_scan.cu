@@ -54,7 +54,7 @@ struct Scan {
   float rate;
   int batch, seqlen, channels, strips, tiles, npieces;
   unsigned total;                // tiles of all sequences
-  int inject;
+  int inject, enter_ahead;       // enter_ahead: a gradient's entering states come with the inputs
   int early;                     // a forward's tile is sent for two tiles ahead, not half a one
   int64_t xs[2], is[2], rs[2], ys[2], dys[2], dxs[2], dis[2], drs[2], ms[2];
 };
@@ -159,6 +159,7 @@ struct Shared {
   int4 which[2];                    // place in its sequence (-1: there is no tile left), unit, strip, batch entry
   int dead;                         // a wait ran out: no further one, and no further tile
   alignas(8) uint64_t full[2];
+  alignas(16) float rate[2][kStrip], enter[2][kStrip];   // of the tiles' channels: rates, and (gradient) the states entering them
 };
 
 struct Maps {
@@ -167,7 +168,8 @@ struct Maps {
 
 // Takes the next tile's number and sends for its inputs (one thread).
 template <typename T, bool TMA, int N, int TILE>
-__device__ __forceinline__ void send_for(const Scan& p, const Maps& maps, int4* which, uint64_t* full, unsigned turn, T* stage, bool backwards) {
+__device__ __forceinline__ void send_for(const Scan& p, const Maps& maps, int4* which, uint64_t* full, unsigned turn, T* stage, bool backwards,
+                                         float* rate, float* enter) {
   const unsigned t = p.tiles == 1 ? blockIdx.x + turn * gridDim.x : atomicAdd(p.counter, 1u) + 1u;
   if (t >= p.total) {
     which->x = -1;
@@ -181,12 +183,20 @@ __device__ __forceinline__ void send_for(const Scan& p, const Maps& maps, int4* 
     ptx::mbar_arrive(full);
     return;
   }
-  ptx::mbar_expect_tx(full, N * TILE * kStrip * sizeof(T));
+  const int k = backwards ? p.tiles - 1 - place : place;
+  const uint32_t rates = p.rates ? kStrip * 4 : 0, states = p.enter_ahead ? (uint32_t)min(kStrip, p.channels - strip * kStrip) * 4 : 0;
+  ptx::mbar_expect_tx(full, N * TILE * kStrip * (uint32_t)sizeof(T) + rates + states);
+  auto numbers = [&](float* to, const float* from, uint32_t bytes) {
+    asm volatile("cp.async.bulk.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1], %2, [%3];" ::"r"(ptx::smem_u32(to)), "l"(from), "r"(bytes),
+                 "r"(ptx::smem_u32(full)) : "memory");
+  };
+  if (rates) numbers(rate, p.rates + strip * kStrip, rates);
+  if (states) numbers(enter, p.pieces + ((int64_t)b * p.npieces + k) * p.channels + strip * kStrip, states);
 #pragma unroll
   for (int n = 0; n < N; ++n)
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.mbarrier::complete_tx::bytes [%0], [%1, {%3, %4, %5}], [%2];" ::"r"(
                      ptx::smem_u32(stage + n * TILE * kStrip)),
-                 "l"(&maps.at[n]), "r"(ptx::smem_u32(full)), "r"(strip * kStrip), "r"((backwards ? p.tiles - 1 - place : place) * TILE), "r"(b)
+                 "l"(&maps.at[n]), "r"(ptx::smem_u32(full)), "r"(strip * kStrip), "r"(k * TILE), "r"(b)
                  : "memory");
 }
 
@@ -328,6 +338,11 @@ __device__ __forceinline__ Pair fold_seen(const Shared<RUNS, SIDES>& sh, int k) 
 
 constexpr size_t stage_numbers(int n, int tile) { return (size_t)n * tile * kStrip; }
 
+__device__ __forceinline__ Pair own_pair(const float* strip) {   // of a strip's numbers this lane's two
+  const float2 f = *reinterpret_cast<const float2*>(strip + 2 * (threadIdx.x % 32));
+  return pair(f.x, f.y);
+}
+
 // Lane l of a warp works on channels 2 l and 2 l + 1 of the strip.
 struct Lane {
   int c;
@@ -380,8 +395,9 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     ptx::mbar_init(&sh.full[0], 1);
     ptx::mbar_init(&sh.full[1], 1);
     ptx::fence_mbar_init();
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words)
-    send_for<T, TMA, 3, kTile>(p, maps, &sh.which[0], &sh.full[0], 0, stages, false);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words and rates)
+    asm volatile("fence.proxy.async;" ::: "memory");
+    send_for<T, TMA, 3, kTile>(p, maps, &sh.which[0], &sh.full[0], 0, stages, false, sh.rate[0], nullptr);
   }
   __syncthreads();
 
@@ -402,7 +418,7 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
     if (p.inject && blockIdx.x == 0) break;   // (SsdGatedScanArgs::inject_lost_tile)
     if (p.early && turn == 0 && threadIdx.x == 32 * (kRuns - 1))   // (when every CTA has its first)
-      send_for<T, TMA, 3, kTile>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, false);
+      send_for<T, TMA, 3, kTile>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, false, sh.rate[1], nullptr);
     const int4 which = sh.which[s];
     if (which.x < 0) break;
     const int k = which.x, unit = which.y, strip = which.z, b = which.w;
@@ -420,7 +436,7 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     auto ri = [&](int t) { return raw[t * 32 + kTile * 32]; };
     auto rr = [&](int t) { return raw[t * 32 + 2 * kTile * 32]; };
     const unsigned marks = marks_of<L>(p, b, t0, here);
-    const Pair rate = ln.rates(p);
+    const Pair rate = TMA && p.rates ? own_pair(sh.rate[s]) : ln.rates(p);
 
     Pair a[L], u[L];
     Share own = {both(1.f), both(0.f)};
@@ -478,7 +494,8 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     // (the inputs of this tile and of the one before have been read)
     if (threadIdx.x == 32 * (kRuns - 1)) {
       const int to = p.early ? s : s ^ 1;
-      send_for<T, TMA, 3, kTile>(p, maps, &sh.which[to], &sh.full[to], p.early ? turn + 2 : turn + 1, stages + to * kStage, false);
+      send_for<T, TMA, 3, kTile>(p, maps, &sh.which[to], &sh.full[to], p.early ? turn + 2 : turn + 1, stages + to * kStage, false, sh.rate[to],
+                                      nullptr);
     }
     if constexpr (!TMA && kLate) {
       wait_for(p, sh, &sh.full[s ^ 1], (turn + 1) >> 1 & 1);
@@ -544,8 +561,9 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
     ptx::mbar_init(&sh.full[0], 1);
     ptx::mbar_init(&sh.full[1], 1);
     ptx::fence_mbar_init();
-    asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words)
-    send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[0], &sh.full[0], 0, stages, true);
+    asm volatile("griddepcontrol.wait;" ::: "memory");   // (prepare_kernel's words and rates)
+    asm volatile("fence.proxy.async;" ::: "memory");
+    send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[0], &sh.full[0], 0, stages, true, sh.rate[0], sh.enter[0]);
   }
   __syncthreads();
 
@@ -596,8 +614,9 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
     auto rr = [&](int t) { return pair_of<T>(raw[t * 32 + 2 * kNext]); };
     auto dy = [&](int t) { return pair_of<T>(raw[t * 32 + 3 * kNext]); };
     const unsigned marks = marks_of<L>(p, b, t0, here);
-    Pair h = ln.get(p.pieces + ((int64_t)b * p.npieces + k) * p.channels);   // the state entering the tile
-    const Pair rate = ln.rates(p), minus = both(-1.f), one = both(1.f);
+    // the state entering the tile
+    Pair h = TMA && p.enter_ahead ? own_pair(sh.enter[s]) : ln.get(p.pieces + ((int64_t)b * p.npieces + k) * p.channels);
+    const Pair rate = TMA && p.rates ? own_pair(sh.rate[s]) : ln.rates(p), minus = both(-1.f), one = both(1.f);
 
     Pair a[L], sr[L], si[L], wt[L], m[L];
     Share own = {both(1.f), both(0.f)};
@@ -657,7 +676,7 @@ if (marks == 0) {
 
     // (the inputs of the tile before have been read)
     if (threadIdx.x == 32 * (kRuns - 1))
-      send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true);
+      send_for<T, TMA, 4, kTileGrad>(p, maps, &sh.which[s ^ 1], &sh.full[s ^ 1], turn + 1, stages + (s ^ 1) * kStage, true, sh.rate[s ^ 1], sh.enter[s ^ 1]);
     if constexpr (!TMA && kLate) {
       wait_for(p, sh, &sh.full[s ^ 1], (turn + 1) >> 1 & 1);
       fetch(s ^ 1);
@@ -888,6 +907,7 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   // wait for one that is started after it: 131 072 x 2 048 bf16 (9 at a time) 494 us, taken two tiles ahead 538.  With fewer the
   // inputs' way counts for more: 8 x 2 048 x 2 048 (1) 62 and 66, 3 x 1 021 x 1 536 fp16 (4) 16.6 and 17.6.  (Copies by threads are late ones.)
   p.early = grid <= 6 * z.units && (tma || sizeof(T) == 2);
+  p.enter_ahead = grad && tma && reinterpret_cast<uintptr_t>(a.pieces) % 16 == 0 && a.channels % 4 == 0;
   auto go = [&](auto kernel, int threads, size_t smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)SSD_ERR_CUDA;
     if (!z.words && !z.rates) return launch(kernel, grid, threads, smem, stream, p, maps);
