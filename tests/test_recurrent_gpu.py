@@ -197,6 +197,24 @@ def test_gated_scan_at_the_edges_of_its_gates(dtype):
     assert (dx[shut] == 0).all() and (di[shut] == 0).all() and (dr[v["r"].float().abs() == inf] == 0).all()
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_rows_off_16_bytes_through_many_tiles(dtype):
+    """Rows that TMA cannot read, several tiles for every CTA: what the same numbers give where it can, bit by bit, and every time."""
+    b, s, d = 54, 853, 151
+    wide = scan_inputs(b, s, 152, dtype, True, True, seed=12)
+    odd = {k: t[..., :d].contiguous() if k in ("x", "i", "r", "dy", "h", "dh", "decay") else t for k, t in wide.items()}
+
+    def run(v):
+        ins = [v[k].detach().requires_grad_(True) for k in ("x", "i", "r", "decay", "h")]
+        y, fin = W().gated_scan(*ins[:4], initial_state=ins[4], reset=v["reset"], return_final_state=True)
+        return [y.detach(), fin.detach(), *torch.autograd.grad([y, fin], ins, [v["dy"], v["dh"]])]
+
+    want = run(wide)
+    for _ in range(5):
+        for g, w in zip(run(odd), want):
+            assert torch.equal(g, w[..., :d])
+
+
 def test_gated_scan_keeps_bad_numbers_where_they_are():
     """An infinity or a NaN reaches the tokens behind it in its own channel and row, up to a reset; everything else is as without it, and so
     are the gradients of what does not depend on it."""
