@@ -236,6 +236,13 @@ def test_gated_scan_keeps_bad_numbers_where_they_are():
         dx, di = torch.autograd.grad([y], ins, [torch.ones_like(y)])
         assert torch.isfinite(dx).all()
         assert torch.isfinite(di[~hit]).all()
+    for name in ("i", "r"):
+        bad = {k: v[k].clone() for k in ("x", "i", "r")}
+        bad[name][0, 130, 7] = math.nan
+        y = W().gated_scan(bad["x"], bad["i"], bad["r"], v["decay"], initial_state=v["h"], reset=reset)
+        assert torch.isnan(y[hit]).all() and torch.equal(y[~hit], good[~hit])
+        step = W().gated_scan_step(bad["x"][:, 130], bad["i"][:, 130], bad["r"][:, 130], v["decay"], v["h"].clone())
+        assert torch.isnan(step[0, 7]) and torch.isfinite(step).sum() == step.numel() - 1
     h = v["h"].clone()
     h[1, 3] = math.inf          # a state that is not finite, dropped at once
     reset[1, 0] = True

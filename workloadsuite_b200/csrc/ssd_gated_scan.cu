@@ -103,6 +103,13 @@ __device__ __forceinline__ float decay_rate(float rate, float decay) {
 // MILD: v stays below 1/2 however far the gate opens (rate * softplus(decay) does), as it does where layers are initialised.
 constexpr float kMild = 0.5f;
 __device__ __forceinline__ Pair sigmoid(Pair v) { return each(each(v * both(-kLog2E), exp2_approx) + both(1.f), rcp_approx); }
+// 1 / sqrt(v), of the smallest normal number where v is less; of a NaN a NaN
+__device__ __forceinline__ float inv_root(float v) {
+  float r;
+  asm("max.NaN.f32 %0, %1, 0f00800000;" : "=f"(r) : "f"(v));
+  return rsqrt_approx(r);
+}
+
 template <bool MILD>
 struct Gates {
   Pair sr, v, a, om;
@@ -126,7 +133,7 @@ struct Gates {
     om = q * (a + one);
   }
   // 1 / sqrt(1 - a^2); where a is 1 a large number, which comes with factors that are zero
-  __device__ __forceinline__ Pair inv() const { return each(om, [](float f) { return rsqrt_approx(fmaxf(f, 1.17549435e-38f)); }); }
+  __device__ __forceinline__ Pair inv() const { return each(om, inv_root); }
 };
 
 // Pairs of a run or a tile, of a lane's two channels.
@@ -455,7 +462,7 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
         for (int t = 0; t < L; ++t) {
           const Gates<true> g(rate, pair_of<T>(rr(t)));
           const Pair d = each(pair_of<T>(ri(t)) * both(-kLog2E), exp2_approx) + both(1.f);
-          const Pair m = each(g.om * (d * d), [](float f) { return rsqrt_approx(fmaxf(f, 1.17549435e-38f)); });
+          const Pair m = each(g.om * (d * d), inv_root);
           a[t] = g.a;
           u[t] = (pair_of<T>(rx(t)) * g.om) * m;
         }
