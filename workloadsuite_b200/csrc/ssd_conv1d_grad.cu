@@ -6,7 +6,8 @@
 // are on their way (TMA, a ring of its own for each warp) while one is worked on: registers do not hold enough of them to cover the memory's latency
 // (4 x 8 192 x 5 120 bf16: a block ahead in registers 239 us).  A CTA's runs follow one another; it leaves
 // its sums for dw and dbias to column_sum_kernel, in a fixed order.
-// 4 x 8 192 x 5 120 bf16: 215 us (4.7 TB/s, 72 % of the copy bandwidth).  Bound: latency with sixteen warps an SM and 27 instructions an element.
+// 4 x 8 192 x 5 120 bf16: 197 us (5.1 TB/s, 79 % of the copy bandwidth).  Bound: latency with sixteen warps an SM and 25 instructions an element.
+// Sixteen warps are four CTAs of four: a CTA's last warp holds up fewer of them (two of eight 216 us; eight of two 199, but 8 x 2 048 x 2 048 53 for 50).
 #include <algorithm>
 #include <type_traits>
 
@@ -17,7 +18,7 @@
 namespace ssd {
 namespace {
 
-constexpr int kWarps = 8, kAhead = 8, kCtas = 2;
+constexpr int kWarps = 4, kAhead = 8, kCtas = 4;
 constexpr int stages_of(int bytes) { return bytes == 2 ? 4 : 3; }   // blocks of a warp's ring
 
 struct ConvGrad {
@@ -208,7 +209,7 @@ struct Cut {
 Cut cut_of(int batch, int seqlen, int channels) {
   Cut c;
   const int64_t strips = (int64_t)batch * ((channels + 63) / 64);
-  for (c.run = 128; c.run > 8; c.run /= 2) {
+  for (c.run = 256; c.run > 8; c.run /= 2) {
     if (strips * ((seqlen + (int64_t)kWarps * c.run - 1) / (kWarps * c.run)) >= 148 * 4) break;
   }
   c.ctas = (int)(((int64_t)seqlen + kWarps * c.run - 1) / (kWarps * c.run));
