@@ -12,6 +12,7 @@
 
 #include "ssd_b200.h"
 #include "ssd_common.cuh"
+#include "vec_io.cuh"
 
 namespace ssd {
 namespace {
@@ -123,14 +124,8 @@ conv1d_silu_kernel(const T* __restrict__ x, const T* __restrict__ w, const T* __
       float acc = bs[e];
 #pragma unroll
       for (int k = 0; k < K; ++k) acc = fmaf(wk[k][e], win[k][e], acc);
-      if (sizeof(T) == 2) {
-        // silu(a) = a * (0.5 + 0.5 tanh(a / 2)): one MUFU operation; its 2^-11 error is below the 16-bit rounding
-        float th;
-        asm("tanh.approx.f32 %0, %1;" : "=f"(th) : "f"(0.5f * acc));
-        out[e] = acc * fmaf(0.5f, th, 0.5f);
-      } else {
-        out[e] = __fdividef(acc, 1.f + __expf(-acc));
-      }
+      // (not by tanh.approx, which is one operation less: what it leaves of 1 + tanh(a / 2) is off by 6 half steps of fp16 at -8, by all of it below -12)
+      out[e] = sizeof(T) == 2 ? acc * rcp_approx(1.f + exp2_approx(-kLog2E * acc)) : __fdividef(acc, 1.f + __expf(-acc));
     }
     store8<T>(y + b * ysb + (int64_t)t * ysl + c0, out, vec);
   };
@@ -269,13 +264,17 @@ conv1d_silu_staged_kernel(const T* __restrict__ x, const T* __restrict__ w, cons
 #pragma unroll
   for (int p = 0; p < kStages - 1; ++p) issue(p);
 
+  // Taps and bias times -log2 e, so that with v = -log2(e) a the sums are exponents as they are: silu(a) = v / (-log2(e) (1 + 2^v)).
+  // Two special functions an element and a row's issue slots cost 8 % (b4 s8192 h80: 122 us) beside one tanh.approx (112), which is no
+  // function to round once to 16 bits below -4; a polynomial in 2^-|v| in place of the reciprocal 137; scaling behind the sums 124.5.
+  const f32x2 scale2 = pack_f2(-kLog2E, -kLog2E);
   f32x2 wk[K][4], bs[4];
 #pragma unroll
   for (int j = 0; j < 4; ++j) {
-    bs[j] = bias ? pack_f2(Cvt<T>::to_f(bias[c0 + 2 * j]), Cvt<T>::to_f(bias[c0 + 2 * j + 1])) : pack_f2(0.f, 0.f);
+    bs[j] = bias ? mul_f2(scale2, pack_f2(Cvt<T>::to_f(bias[c0 + 2 * j]), Cvt<T>::to_f(bias[c0 + 2 * j + 1]))) : pack_f2(0.f, 0.f);
 #pragma unroll
     for (int k = 0; k < K; ++k)
-      wk[k][j] = pack_f2(Cvt<T>::to_f(w[(int64_t)(c0 + 2 * j) * K + k]), Cvt<T>::to_f(w[(int64_t)(c0 + 2 * j + 1) * K + k]));
+      wk[k][j] = mul_f2(scale2, pack_f2(Cvt<T>::to_f(w[(int64_t)(c0 + 2 * j) * K + k]), Cvt<T>::to_f(w[(int64_t)(c0 + 2 * j + 1) * K + k])));
   }
   auto widen = [&](const uint4& q, f32x2 (&row)[4]) {
     const float2 a = up2(xcol, q.x), bq = up2(xcol, q.y), c = up2(xcol, q.z), d = up2(xcol, q.w);
@@ -289,7 +288,6 @@ conv1d_silu_staged_kernel(const T* __restrict__ x, const T* __restrict__ w, cons
     const uint4 q = t >= 0 ? *reinterpret_cast<const uint4*>(xcol + (int64_t)t * xsl) : make_uint4(0, 0, 0, 0);
     widen(q, win[(4 - k) & 7]);
   }
-  const f32x2 half2 = pack_f2(0.5f, 0.5f);
   for (int piece = 0; piece < npieces; ++piece) {
     issue(piece + kStages - 1);
     cp_async_wait<kStages - 1>();   // this thread's copies of `piece` have landed (it is their only reader)
@@ -307,12 +305,10 @@ conv1d_silu_staged_kernel(const T* __restrict__ x, const T* __restrict__ w, cons
           f32x2 acc = bs[j];
 #pragma unroll
           for (int k = 0; k < K; ++k) acc = fma_f2(wk[k][j], win[(s + 8 - (K - 1) + k) & 7][j], acc);
-          // silu(a) = a * (0.5 + 0.5 tanh(a / 2)): one MUFU operation per element; its 2^-11 error is below the 16-bit rounding
-          float h0, h1, a0, a1;
-          unpack_f2(mul_f2(acc, half2), h0, h1);
-          asm("tanh.approx.f32 %0, %1;" : "=f"(h0) : "f"(h0));
-          asm("tanh.approx.f32 %0, %1;" : "=f"(h1) : "f"(h1));
-          unpack_f2(mul_f2(acc, fma_f2(pack_f2(h0, h1), half2, half2)), a0, a1);
+          float a0, a1;
+          unpack_f2(acc, a0, a1);
+          unpack_f2(fma_f2(pack_f2(exp2_approx(a0), exp2_approx(a1)), scale2, scale2), a0, a1);
+          unpack_f2(mul_f2(acc, pack_f2(rcp_approx(a0), rcp_approx(a1))), a0, a1);
           o[j] = pk2(xcol, a0, a1);
         }
         *reinterpret_cast<uint4*>(ycol + (int64_t)(t0 + u) * ysl) = make_uint4(o[0], o[1], o[2], o[3]);
@@ -326,7 +322,7 @@ conv1d_silu_staged_kernel(const T* __restrict__ x, const T* __restrict__ w, cons
 // tokens and some ten for the rows before and the start, and with what it shares the SM with (two 1.4, three 2.0 times that of one alone, from
 // b1 s4096 h32: 64 tokens, one block an SM, 12.8 us, 32 10.0, 24 11.0; b1 s8192 h24: 64 13.6, 32 11.1; b2 s4096 h48: 64 23.8, 56 22.4; b4 s333
 // h80: 32 8.2, 16 7.2).  Otherwise the longest: what is read at a time lies closer together than with longer ones (b4 s8192 h80: 56
-// 115 us, 64 113, 96 114, 192 121, 376, which is a single round, 133).
+// 115 us, 64 113, 96 114, 192 121, 376, which is a single round, 133).  (Measured with one special function an element; with two all are up to a tenth longer.)
 int staged_run(int64_t columns, int seqlen) {
   constexpr int kShare[3] = {5, 7, 10};
   int best = kLongestRun, cost = 1 << 30;
