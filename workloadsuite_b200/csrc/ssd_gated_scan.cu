@@ -15,8 +15,8 @@
 // A state is only ever folded through whole tiles' pairs, h <- P h + q, one tile after the other, wherever the look back begins:
 // results do not depend on what was published when.
 // Entering states of 64-token pieces are kept for the gradient, which makes every h again in fp32 instead of reading y.
-// 8 x 2 048 x 2 048 bf16: forward 62 us (4.3 TB/s of algorithmic traffic, 67 % of the copy bandwidth), gradient 137 (53 %); 131 072 x 2 048:
-// 497 us.  Bound: latency with sixteen warps an SM, whose registers the tokens' a and u fill; issue slots are half used, the
+// 8 x 2 048 x 2 048 bf16: forward 62 us (4.3 TB/s of algorithmic traffic, 67 % of the copy bandwidth), gradient 135 (53 %); 131 072 x 2 048:
+// 494 us; where a strip's gates are not all MILD (below) 79, 142 and 618.  Bound: latency with sixteen warps an SM, whose registers the tokens' a and u fill; issue slots are half used, the
 // special-function unit too (four functions a number, five in the gradient).
 #include <algorithm>
 #include <cmath>
@@ -108,6 +108,12 @@ __device__ __forceinline__ float inv_root(float v) {
   float r;
   asm("max.NaN.f32 %0, %1, 0f00800000;" : "=f"(r) : "f"(v));
   return rsqrt_approx(r);
+}
+
+__device__ __forceinline__ float not_above_zero(float v) {   // (a NaN stays one)
+  float r;
+  asm("min.NaN.f32 %0, %1, 0f00000000;" : "=f"(r) : "f"(v));
+  return r;
 }
 
 template <bool MILD>
@@ -456,22 +462,27 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
 #pragma unroll
       for (int t = 1; t < L; ++t) least = Two<T>::least(least, ri(t));
       const float2 kk = halves(rate), ll = Two<T>::up(least);
-      // u = x om / (sqrt(om) (1 + e^-i)): one reciprocal square root of om (1 + e^-i)^2 where that is no overflow
-      if (__all_sync(~0u, kk.x < kMild && kk.y < kMild && ll.x > -40.f && ll.y > -40.f)) {
+      // u = x om / (sqrt(om) (1 + e^-i)), one reciprocal square root of om (1 + e^-i)^2.  Where a run holds a gate that is all but shut that
+      // would overflow: its gates are taken at kShut at least, times e^(i - kShut), which is 1 for the others (and in the general loop, as a loop
+      // more costs the first one 2 %).  So a number is rounded in one way, whatever its neighbours are.
+      constexpr float kShut = -40.f;
+      const bool open = ll.x > kShut && ll.y > kShut;
+      if (__all_sync(~0u, open && kk.x < kMild && kk.y < kMild)) {
 #pragma unroll
         for (int t = 0; t < L; ++t) {
           const Gates<true> g(rate, pair_of<T>(rr(t)));
           const Pair d = each(pair_of<T>(ri(t)) * both(-kLog2E), exp2_approx) + both(1.f);
-          const Pair m = each(g.om * (d * d), inv_root);
           a[t] = g.a;
-          u[t] = (pair_of<T>(rx(t)) * g.om) * m;
+          u[t] = (pair_of<T>(rx(t)) * g.om) * each(g.om * (d * d), inv_root);
         }
       } else {
 #pragma unroll
         for (int t = 0; t < L; ++t) {
           const Gates<false> g(rate, pair_of<T>(rr(t)));
+          const Pair i = pair_of<T>(ri(t)), less = each(each(i + both(-kShut), not_above_zero) * both(kLog2E), exp2_approx);
+          const Pair d = each(each(i, [](float v) { return fmaxf(v, kShut); }) * both(-kLog2E), exp2_approx) + both(1.f);
           a[t] = g.a;
-          u[t] = (g.om * g.inv()) * (sigmoid(pair_of<T>(ri(t))) * pair_of<T>(rx(t)));
+          u[t] = ((pair_of<T>(rx(t)) * less) * g.om) * each(g.om * (d * d), inv_root);
         }
       }
       if (here < L) {
@@ -654,7 +665,7 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
         for (int t = 0; t < L; ++t)
           if (t >= here) a[t] = one, sr[t] = si[t] = wt[t] = m[t] = both(0.f);
       }
-if (marks == 0) {
+      if (marks == 0) {
 #pragma unroll
         for (int t = 0; t < L; ++t) {
           own.P = own.P * a[t];
