@@ -330,7 +330,7 @@ int ssd_b200_gated_step(const SsdGatedStepArgs* args, void* stream);
  * The backwards write every result whole; sums over rows are in a fixed order. */
 typedef struct SsdNormArgs {
   const void* x;                /* [rows,d] dtype */
-  const void* z;                /* [rows,d] dtype  (gated) */
+  const void* z;                /* [rows,d] dtype  (gated; NULL for ssd_b200_rms_norm and its backward) */
   const void* weight;
   const void* residual;         /* [rows,d] residual_dtype, or NULL */
   const void* post_weight;      /* or NULL */
@@ -356,7 +356,7 @@ typedef struct SsdNormArgs {
   int64_t x_stride, z_stride, residual_stride, y_stride, residual_out_stride;
   int64_t dy_stride, dresidual_out_stride, dx_stride, dz_stride, dresidual_stride;
 } SsdNormArgs;
-size_t ssd_b200_norm_workspace_bytes(const SsdNormArgs* args);
+size_t ssd_b200_norm_workspace_bytes(const SsdNormArgs* args);   /* of the gated backward where z is given, of the other one where not */
 int ssd_b200_rms_norm(const SsdNormArgs* args, void* stream);
 int ssd_b200_rms_norm_backward(const SsdNormArgs* args, void* stream);
 int ssd_b200_gated_rms_norm(const SsdNormArgs* args, void* stream);

@@ -630,6 +630,7 @@ Shape shape_of(int64_t rows, int d, int groups, bool grad) {
 
 int check(const SsdNormArgs* a, bool gated, bool grad) {
   if (!a) return SSD_ERR_NULL_POINTER;
+  if (!gated && a->z) return SSD_ERR_UNSUPPORTED;   // (the workspace's size is asked for by it)
   const int groups = gated ? a->groups : 1;
   if (a->rows <= 0 || a->d <= 0 || groups <= 0 || a->d % groups != 0 || !(a->eps >= 0.f && a->eps < INFINITY)) return SSD_ERR_BAD_SHAPE;
   if (a->d / groups > 16384 || groups > 65535) return SSD_ERR_TOO_LARGE;
