@@ -36,3 +36,24 @@ def test_a_norm_without_a_gate_takes_none(lib):
         assert lib.ssd_b200_rms_norm_backward(norm(z=P, dz=P, workspace_bytes=nbytes, **shape), None) == -4
         assert lib.ssd_b200_rms_norm(norm(z=P, workspace_bytes=nbytes, **shape), None) == -4
     assert lib.ssd_b200_rms_norm_backward(norm(workspace_bytes=gated, **shape), None) == -5
+
+
+def test_sizes_next_to_the_end_of_32_bits(lib):
+    """Channels that rounding up to strips of 64 takes past 2^31, tokens that a run's rim does: too large, not a negative number of strips."""
+    def scan(**kw):
+        a = _lib.GatedScanArgs()
+        for f in ("x", "input_gate", "decay_gate", "decay", "y", "pieces", "dy", "dx", "dinput_gate", "ddecay_gate", "ddecay", "workspace"):
+            setattr(a, f, P)
+        a.workspace_bytes, a.rate, a.batch, a.seqlen, a.channels, a.dtype = 1 << 62, 8.0, 1, 1, 64, _lib.DTYPE_BF16
+        for k, v in kw.items():
+            setattr(a, k, v)
+        return C.byref(a)
+
+    for channels in (0x7fffffff, 0x7fffffff - 60, 0x7fffff80):
+        for call, back in ((lib.ssd_b200_gated_scan, 0), (lib.ssd_b200_gated_scan_backward, 1)):
+            assert call(scan(channels=channels), None) == -8
+            assert lib.ssd_b200_gated_scan_workspace_bytes(scan(channels=channels), back) == 0
+    conv = lambda s, c: lib.ssd_b200_conv1d_silu_backward(P, P, P, P, P, P, P, P, 1 << 62, 1, s, c, 4, _lib.DTYPE_BF16, *(8, 8) * 3, None, None)
+    assert conv(1, 0x7fffffff - 7) == -8 and conv(1, 64 * 65535 + 8) == -8
+    assert conv(0x7fffffff, 8) == -8 and conv(0x7fffffff - 3, 8) == -8
+    assert lib.ssd_b200_conv1d_silu(P, P, P, P, 1, 0x7fffffff - 3, 8, 4, _lib.DTYPE_BF16, *(8, 8) * 2, None) == -8

@@ -389,6 +389,7 @@ extern "C" int ssd_b200_conv1d_silu(const void* x, const void* weight, const voi
   if (!x || !weight || !y) return SSD_ERR_NULL_POINTER;
   if (batch <= 0 || seqlen <= 0 || channels <= 0 || taps <= 0 || taps > ssd::kMaxTaps) return SSD_ERR_BAD_SHAPE;
   if (channels % 8 != 0) return SSD_ERR_UNSUPPORTED;
+  if (seqlen > 0x7fffff00) return SSD_ERR_TOO_LARGE;   // (runs round it up)
   cudaStream_t s = static_cast<cudaStream_t>(stream);
   switch (dtype) {
     case SSD_DTYPE_F32:

@@ -202,6 +202,9 @@ struct FinishConv {
   }
 };
 
+// Strips of channels are a grid's second axis, and a run goes a few tokens past its end.
+bool covered(int seqlen, int channels) { return channels <= 64 * 65535 && seqlen <= 0x7fffff00; }
+
 struct Cut {
   int run, ctas;   // tokens of a warp, CTAs of a sequence
 };
@@ -259,7 +262,7 @@ int run_grad(ConvGrad p, void* dw, void* db, int batch, int taps, int dtype, cud
 }  // namespace ssd
 
 extern "C" size_t ssd_b200_conv1d_silu_workspace_bytes(int32_t batch, int32_t seqlen, int32_t channels, int32_t taps) {
-  if (batch <= 0 || seqlen <= 0 || channels <= 0 || taps < 2 || taps > 4) return 0;
+  if (batch <= 0 || seqlen <= 0 || channels <= 0 || taps < 2 || taps > 4 || !ssd::covered(seqlen, channels)) return 0;
   return (size_t)batch * ssd::cut_of(batch, seqlen, channels).ctas * (taps + 1) * channels * sizeof(float);
 }
 
@@ -271,11 +274,12 @@ extern "C" int ssd_b200_conv1d_silu_backward(const void* x, const void* weight, 
   if (!x || !weight || !dy || !dx || !dweight || (bias && !dbias)) return SSD_ERR_NULL_POINTER;
   if (batch <= 0 || seqlen <= 0 || channels <= 0 || taps <= 0) return SSD_ERR_BAD_SHAPE;
   if (channels % 8 != 0 || taps < 2 || taps > 4) return SSD_ERR_UNSUPPORTED;
+  if (!ssd::covered(seqlen, channels)) return SSD_ERR_TOO_LARGE;
   if (!workspace || reinterpret_cast<uintptr_t>(workspace) % 16 ||
       workspace_bytes < ssd_b200_conv1d_silu_workspace_bytes(batch, seqlen, channels, taps))
     return SSD_ERR_WORKSPACE;
   const ssd::Cut cut = ssd::cut_of(batch, seqlen, channels);
-  if ((int64_t)batch * cut.ctas > 0x7fffffff || (channels + 63) / 64 > 65535) return SSD_ERR_TOO_LARGE;
+  if ((int64_t)batch * cut.ctas > 0x7fffffff) return SSD_ERR_TOO_LARGE;
   // two channels at once: rows start on their boundary
   for (int64_t stride : {x_stride_b, x_stride_l, dy_stride_b, dy_stride_l, dx_stride_b, dx_stride_l})
     if (stride % 2) return SSD_ERR_MISALIGNED;

@@ -849,8 +849,9 @@ int check(const SsdGatedScanArgs* a, bool grad) {
   if (!a) return SSD_ERR_NULL_POINTER;
   if (a->batch <= 0 || a->seqlen <= 0 || a->channels <= 0 || a->wait_limit_ms < 0 || !(a->rate > 0.f && a->rate < INFINITY)) return SSD_ERR_BAD_SHAPE;
   if (a->dtype != SSD_DTYPE_F32 && a->dtype != SSD_DTYPE_F16 && a->dtype != SSD_DTYPE_BF16) return SSD_ERR_UNSUPPORTED;
+  if (a->seqlen > 0x7fffff00 || a->channels > 0x7fffff00) return SSD_ERR_TOO_LARGE;   // (tiles and strips round them up)
   const Sizes z = sizes_of(*a, grad);
-  if (a->seqlen > 0x7fffff00 || z.tiles * z.units > 0x7fffffff) return SSD_ERR_TOO_LARGE;
+  if (z.tiles * z.units > 0x7fffffff) return SSD_ERR_TOO_LARGE;
   return SSD_OK;
 }
 
