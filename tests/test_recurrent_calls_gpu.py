@@ -1,6 +1,9 @@
 """Calls of the recurrent block's operators that the documentation allows and that once went wrong, each by itself.
 Tolerances as in test_recurrent_gpu.py."""
 import math
+import subprocess
+import sys
+from pathlib import Path
 
 import pytest
 import torch
@@ -48,3 +51,60 @@ def test_gated_scan_rounds_a_channel_whatever_its_neighbours_are(dtype, d):
         changed[at] = value
         for n, (g, w) in enumerate(zip(run(**{name: changed}), want)):
             assert torch.equal(g[..., others], w[..., others]), (name, value, n)
+
+
+_FIRST_IN_A_CAPTURE = """
+import torch
+import workloadsuite_b200 as W
+from workloadsuite_b200 import _lib
+
+x = torch.randn(2, 40, 16, device="cuda", requires_grad=True)
+w = torch.randn(16, 1, 4, device="cuda", requires_grad=True)
+graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+torch.cuda.synchronize()
+with torch.inference_mode(), torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+    {first}
+with torch.cuda.graph(graph, stream=side):
+    y = W.conv1d_silu(x, w)
+    torch.autograd.grad([y], [x, w], [torch.ones_like(y)])
+word = _lib.fast().status_word(0)
+assert (word == 0).all()
+word[0] = 5
+torch.cuda.synchronize()
+graph.replay()
+assert W.device_status() == 5 and W.device_status() == 0
+"""
+
+_FIRST_FROM_MANY_THREADS = """
+import threading
+import torch
+import workloadsuite_b200 as W
+from workloadsuite_b200 import _lib
+
+_lib.fast()
+x, w = torch.randn(2, 40, 16, device="cuda"), torch.randn(16, 1, 4, device="cuda")
+gate, seen = threading.Barrier(8), []
+
+def work(n):
+    leaf = x.clone().requires_grad_(True)
+    y = W.conv1d_silu(leaf, w).sum()
+    torch.cuda.synchronize()
+    gate.wait()
+    if n % 2:
+        y.backward()
+    seen.append(_lib.fast().status_word(0).data_ptr())
+
+threads = [threading.Thread(target=work, args=(n,)) for n in range(8)]
+[t.start() for t in threads]
+[t.join() for t in threads]
+assert len(seen) == 8 and len(set(seen)) == 1, seen
+"""
+
+
+@pytest.mark.parametrize("program", [_FIRST_IN_A_CAPTURE.format(first="pass"), _FIRST_IN_A_CAPTURE.format(first="W.gated_scan(x, x, x, w[:, 0, 0])"),
+                                     _FIRST_FROM_MANY_THREADS], ids=["a capture's backward", "a capture's forward", "threads"])
+def test_the_status_word_is_made_once_and_outside_of_captures(program):
+    """In processes that have not used it: its first use in a capture (of a backward pass, which another thread runs), or by many threads.  A
+    status that nobody has read is there after a replay."""
+    r = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stderr[-2000:]

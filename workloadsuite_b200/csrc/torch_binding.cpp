@@ -7,7 +7,12 @@
 // here: work may have been enqueued by then, and a step made again would advance the state twice.
 #include <Python.h>
 
+#include <atomic>
+#include <mutex>
+
 #include <ATen/ATen.h>
+#include <c10/core/InferenceMode.h>
+#include <c10/cuda/CUDAGraphsC10Utils.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/csrc/Exceptions.h>
@@ -46,7 +51,7 @@ PyObject* f_raise;   // raises the Python exception of an error code
 
 constexpr int kMaxDevices = 64;
 Tensor* g_workspace[kMaxDevices];   // scratch of the runs that leave results for a later one (never shrinks)
-Tensor* g_status[kMaxDevices];      // the kernels' status word
+std::atomic<Tensor*> g_status[kMaxDevices];   // the kernels' status word
 
 int dtype_of(const Tensor& t) {
   switch (t.scalar_type()) {
@@ -87,9 +92,28 @@ struct Where {
   void* stream() const { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
 };
 
+// Made once, by whichever thread asks first: autograd's threads do too, which do not hold the interpreter.  Zeroed before anybody has it, on a
+// stream of its own, in memory of no pool, so that a capture that is under way records none of it and no replay clears it.
 Tensor& status_word(int dev) {
-  if (!g_status[dev]) g_status[dev] = new Tensor(at::zeros({1024}, at::TensorOptions().dtype(at::kInt).device(at::kCUDA, dev)));
-  return *g_status[dev];
+  if (Tensor* t = g_status[dev].load(std::memory_order_acquire)) return *t;
+  static std::mutex making;
+  const std::lock_guard<std::mutex> lock(making);
+  if (Tensor* t = g_status[dev].load(std::memory_order_acquire)) return *t;
+  constexpr int kWords = 1024;
+  const c10::cuda::CUDAGuard guard((c10::DeviceIndex)dev);
+  const c10::cuda::CUDAStreamCaptureModeGuard relaxed(cudaStreamCaptureModeRelaxed);
+  const c10::InferenceMode plain(false);   // (it is cleared outside of such a mode)
+  void* at = nullptr;
+  cudaStream_t stream = nullptr;
+  C10_CUDA_CHECK(cudaMalloc(&at, kWords * sizeof(int32_t)));
+  C10_CUDA_CHECK(cudaStreamCreateWithFlags(&stream, cudaStreamNonBlocking));
+  C10_CUDA_CHECK(cudaMemsetAsync(at, 0, kWords * sizeof(int32_t), stream));
+  C10_CUDA_CHECK(cudaStreamSynchronize(stream));
+  C10_CUDA_CHECK(cudaStreamDestroy(stream));
+  const c10::Device device(c10::kCUDA, (c10::DeviceIndex)dev);
+  Tensor* t = new Tensor(at::for_blob(at, {kWords}).options(at::TensorOptions().dtype(at::kInt).device(device)).target_device(device).make_tensor());
+  g_status[dev].store(t, std::memory_order_release);
+  return *t;
 }
 Tensor& workspace(int dev, int64_t bytes) {
   if (!g_workspace[dev] || g_workspace[dev]->numel() < bytes) {
