@@ -108,3 +108,43 @@ def test_the_status_word_is_made_once_and_outside_of_captures(program):
     status that nobody has read is there after a replay."""
     r = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0, r.stderr[-2000:]
+
+
+def test_the_model_calls_layers_that_are_not_as_built_with_one_tensor():
+    """A forward that is replaced on a layer or a norm (for offloading, recomputation, logging), or on their class, takes one tensor and gives
+    one, as in the reference; so does what hooks on every module see.  Results: the sums are the same numbers, a norm in another place
+    may round the other way (half a step, 2^-11, through two layers with a gain of some units)."""
+    import torch.nn.modules.module as every
+    from torch.utils.checkpoint import checkpoint
+
+    from workloadsuite_b200 import mamba_model as M
+
+    torch.manual_seed(6)
+    model = M.Model(128, 3, 4, 128, 64, 2, 64, 4).to(DEV).eval()
+    x = torch.randn(1, 128, 128, dtype=torch.float16, device=DEV)
+    with torch.no_grad():
+        want = model(x)
+        same = lambda got: ((got - want).abs().max() <= 2.0 ** -8 * want.abs().max()).item()
+        for module in (model.layers[1], model.layers[2].norm, model.final_norm):
+            seen, old = [], module.forward
+            module.forward = lambda u: (seen.append(u.shape), old(u))[1]
+            assert same(model(x)) and seen == [x.shape]
+            del module.forward
+            module.forward = lambda u: checkpoint(old, u, use_reentrant=False)
+            assert same(model(x))
+            del module.forward
+        for cls, calls in ((M.SSDLayer, 3), (M.RMSNorm, 4)):
+            seen, old = [], cls.forward
+            cls.forward = lambda self, u: (seen.append(u.shape), old(self, u))[1]
+            try:
+                assert same(model(x)) and len(seen) == calls
+            finally:
+                cls.forward = old
+        seen = []
+        hook = every.register_module_forward_hook(lambda m, a, out: seen.append((type(m).__name__, len(a), isinstance(out, torch.Tensor))))
+        try:
+            assert same(model(x))
+        finally:
+            hook.remove()
+        assert all(n == 1 and one for _, n, one in seen) and [n for n, _, _ in seen].count("RMSNorm") == 4
+        assert torch.equal(model(x), want)
