@@ -148,3 +148,48 @@ def test_the_model_calls_layers_that_are_not_as_built_with_one_tensor():
             hook.remove()
         assert all(n == 1 and one for _, n, one in seen) and [n for n, _, _ in seen].count("RMSNorm") == 4
         assert torch.equal(model(x), want)
+
+
+def test_a_tangent_is_refused_and_not_dropped():
+    """Whichever operand carries it, recorded for a backward gradient or not; outside of dual numbers the same call is made."""
+    import torch.autograd.forward_ad as forward_ad
+
+    v = scan_inputs(1, 9, 16, torch.float32, False, True, seed=3)
+    x, w, cw, cb = v["x"], torch.ones(16, device=DEV), torch.randn(16, 1, 4, device=DEV), torch.zeros(16, device=DEV)
+    calls = [("gated_scan", lambda *a: W().gated_scan(*a[:4], initial_state=a[4]), (x, v["i"], v["r"], v["decay"], v["h"])),
+             ("rms_norm", lambda *a: W().rms_norm(a[0], a[1], residual=a[2], post_weight=a[3], scale=a[4]), (x, w, v["dy"], w, w)),
+             ("rms_norm", W().rms_norm, (x, w)), ("gated_rms_norm", W().gated_rms_norm, (x, v["i"], w)), ("conv1d_silu", W().conv1d_silu, (x, cw, cb))]
+    for name, call, args in calls:
+        for records in (False, True):
+            for n in range(len(args)):
+                with forward_ad.dual_level():
+                    other = [a.clone().requires_grad_(records and m != n) for m, a in enumerate(args)]
+                    call(*other)
+                    other[n] = forward_ad.make_dual(other[n], torch.ones_like(other[n]))
+                    with pytest.raises(NotImplementedError, match=f"{name} has no forward-mode gradient"):
+                        call(*other)
+
+
+def test_the_model_s_norm_carries_what_pytorch_s_does():
+    """Forward-mode tangents, function transforms and tensor subclasses go through PyTorch's operators, as with nn.RMSNorm."""
+    import torch.autograd.forward_ad as forward_ad
+
+    from workloadsuite_b200 import mamba_model as M
+
+    class Sub(torch.Tensor):
+        pass
+
+    own, plain = M.RMSNorm(64).to(DEV), torch.nn.RMSNorm(64).to(DEV)
+    with torch.no_grad():
+        own.weight.uniform_(0.5, 1.5)
+        plain.weight.copy_(own.weight)
+    x, t = torch.randn(4, 5, 64, device=DEV), torch.randn(4, 5, 64, device=DEV)
+    with forward_ad.dual_level():
+        a, b = (forward_ad.unpack_dual(n(forward_ad.make_dual(x, t))) for n in (own, plain))
+        assert torch.equal(a.primal, b.primal) and torch.equal(a.tangent, b.tangent)
+        y, r = own(x, forward_ad.make_dual(x, t))
+        assert torch.equal(forward_ad.unpack_dual(r).tangent, t) and forward_ad.unpack_dual(y).tangent is not None
+    for transform in (torch.func.vmap, lambda f: torch.func.grad(lambda u: f(u).sum()), lambda f: lambda u: torch.func.jvp(f, (u,), (t,))[1]):
+        assert torch.equal(transform(own)(x), transform(plain)(x))
+    y = own(x.as_subclass(Sub))
+    assert type(y) is Sub and torch.equal(y.as_subclass(torch.Tensor), plain(x))

@@ -306,6 +306,12 @@ bool records(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
+// Forward-mode gradients have no kernels: what carries one goes the long way, which says so.
+bool tangents(std::initializer_list<const Tensor*> ts) {
+  for (const Tensor* t : ts)
+    if (t->defined() && t->_fw_grad(0).defined()) return true;
+  return false;
+}
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
 // A gradient whose innermost axis is not contiguous (a sum's is expanded) is copied once.
@@ -435,6 +441,7 @@ PyObject* py_gated(PyObject*, PyObject* const* o, Py_ssize_t n) {
       !get(o[5], &reset, true) || !get(o[6], &out, true) || !real(o[7], &rate) || !PyLong_CheckExact(o[8]) || !x->is_cuda() ||
       x->dim() != 3 || i->dim() != 3 || r->dim() != 3 || dtype_of(*x) < 0)
     Py_RETURN_NONE;
+  if (tangents({x, i, r, decay, init})) Py_RETURN_NONE;
   const int wait_ms = (int)PyLong_AsLong(o[8]);
   int rc = 0;
   if (records({x, i, r, decay, init})) {
@@ -641,7 +648,7 @@ PyObject* py_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const Tensor *x, *wt, *res, *post, *scale, *out;
   float eps;
   if (n != 7 || !get(o[0], &x) || !get(o[1], &wt) || !get(o[2], &res, true) || !get(o[3], &post, true) || !get(o[4], &scale, true) ||
-      !get(o[5], &out, true) || !real(o[6], &eps) || !norm_operand(*x))
+      !get(o[5], &out, true) || !real(o[6], &eps) || !norm_operand(*x) || tangents({x, wt, res, post, scale}))
     Py_RETURN_NONE;
   int rc = 0;
   if (records({x, wt, res, post, scale})) {
@@ -709,7 +716,7 @@ PyObject* py_gated_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
   const Tensor *x, *z, *wt, *out;
   float eps;
   if (n != 7 || !get(o[0], &x) || !get(o[1], &z) || !get(o[2], &wt) || !get(o[3], &out, true) || !real(o[4], &eps) ||
-      !PyLong_CheckExact(o[5]) || !norm_operand(*x))
+      !PyLong_CheckExact(o[5]) || !norm_operand(*x) || tangents({x, z, wt}))
     Py_RETURN_NONE;
   const long groups = PyLong_AsLong(o[5]);
   const bool first = o[6] == Py_True;
@@ -781,7 +788,9 @@ struct ConvNode : torch::autograd::Function<ConvNode> {
 PyObject* py_conv(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Tensor *x, *w, *bias, *out;
-  if (n != 4 || !get(o[0], &x) || !get(o[1], &w) || !get(o[2], &bias, true) || !get(o[3], &out, true) || !x->is_cuda()) Py_RETURN_NONE;
+  if (n != 4 || !get(o[0], &x) || !get(o[1], &w) || !get(o[2], &bias, true) || !get(o[3], &out, true) || !x->is_cuda() ||
+      tangents({x, w, bias}))
+    Py_RETURN_NONE;
   int rc = 0;
   Tensor y;
   if (!out->defined() && records({x, w, bias})) {

@@ -19,6 +19,7 @@ from typing import Optional
 
 import torch
 import torch.nn as nn
+from torch.autograd import forward_ad
 from torch.nn.modules.module import _has_any_global_hook
 import torch.nn.functional as F
 
@@ -42,7 +43,14 @@ def _conv(x, weight, bias):
 
 @torch.compiler.disable
 def _norm(x, weight, eps, residual):
-    return rms_norm(x, weight, eps=eps, residual=residual)
+    given = [t for t in (x, weight, residual) if t is not None]
+    if all(type(t) in (torch.Tensor, nn.Parameter) and not torch._C._functorch.is_functorch_wrapped_tensor(t)
+           and (forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None) for t in given):
+        return rms_norm(x, weight, eps=eps, residual=residual)
+    # transforms, tangents and tensor subclasses: PyTorch's operators carry them
+    r = x if residual is None else residual + x
+    y = nn.functional.rms_norm(r, (r.shape[-1],), weight, eps)
+    return y if residual is None else (y, r)
 
 
 @torch.compiler.disable

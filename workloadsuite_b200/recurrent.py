@@ -3,7 +3,8 @@
 
 The reference has the norms as ``nn.RMSNorm`` with a residual sum of its own (``model_ref.py:49-66, 165-204``) and no
 counterpart of the recurrence.  All run in the kernels of ``csrc/ssd_gated_scan.cu`` and ``csrc/ssd_norm.cu`` on the current
-CUDA stream, without a CPU path, and never synchronise the host.
+CUDA stream, without a CPU path, and never synchronise the host.  Gradients are backward ones; an operand with a forward-mode tangent is
+refused (NotImplementedError).
 """
 from __future__ import annotations
 
@@ -13,7 +14,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ssd import _DTYPES, _check_out, _same_device
+from .ssd import _DTYPES, _check_out, _no_tangents, _same_device
 
 
 def _records(*tensors) -> bool:
@@ -88,6 +89,7 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     if got is not None:
         return got if return_final_state else got[0]
     _check_gates("gated_scan", x, input_gate, decay_gate, decay, 3, rate)
+    _no_tangents("gated_scan", x, input_gate, decay_gate, decay, initial_state)
     _same_device(x, initial_state=initial_state, reset=reset, out=out)
     if wait_limit_ms < 0:
         raise ValueError("wait_limit_ms must not be negative")
@@ -190,6 +192,7 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None,
     if got is not None:
         return got[0] if residual is None else got
     _check_norm("rms_norm", x, eps, dict(weight=weight, post_weight=post_weight, scale=scale), dict(residual=residual, out=out))
+    _no_tangents("rms_norm", x, weight, residual, post_weight, scale)
     if residual is None and (post_weight is not None or scale is not None):
         raise ValueError("post_weight and scale apply to what is added to residual: give one")
     if residual is not None and residual.dtype not in (torch.float32, x.dtype):
@@ -226,6 +229,7 @@ def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: 
     if got is not None:
         return got
     _check_norm("gated_rms_norm", x, eps, dict(weight=weight), dict(z=z, out=out), groups)
+    _no_tangents("gated_rms_norm", x, z, weight)
     if z.dtype != x.dtype:
         raise ValueError("z must be in x's dtype")
     if out is not None:

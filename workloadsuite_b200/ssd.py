@@ -10,6 +10,7 @@ import ctypes as C
 from typing import Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 
@@ -92,6 +93,12 @@ def _check_out(out: torch.Tensor, like: torch.Tensor, name: str = "out"):
         raise ValueError(f"{name} must have the shape {tuple(like.shape)}, dtype {like.dtype} and device of X")
     if out.dim() and out.stride(-1) != 1 and out.shape[-1] != 1:
         raise ValueError(f"{name}: innermost axis must be contiguous")
+
+
+def _no_tangents(name: str, *tensors):
+    """The gradients that the kernels have are backward ones: a tangent would be dropped without a word."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError(f"{name} has no forward-mode gradient")
 
 
 def _check(X, A, B, Cm, dt, initial_states):
@@ -301,13 +308,14 @@ def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     x [b,l,d] with a contiguous channel axis (a column slice of the projection output is fine); weight the
     ``nn.Conv1d(d, d, k, groups=d)`` parameter [d,1,k] (or [d,k]); bias [d] or None.  Returns [b,l,d] contiguous
     in x's dtype (fp32 accumulation, one rounding).  Differentiable in x, weight and bias (where ``out`` is given no
-    gradient is recorded).
+    gradient is recorded), backward only: an operand with a forward-mode tangent is refused.
     """
     got = _lib.fast().conv1d_silu(x, weight, bias, out)
     if got is not None:
         return got
     if not x.is_cuda:
         raise RuntimeError("conv1d_silu needs CUDA tensors (there is no CPU path)")
+    _no_tangents("conv1d_silu", x, weight, bias)
     if x.dim() != 3 or x.stride(2) != 1 or x.dtype not in _DTYPES:
         raise ValueError("x must be [b,l,d] float32/float16/bfloat16 with a contiguous channel axis")
     b, l, d = x.shape
