@@ -193,3 +193,32 @@ def test_the_model_s_norm_carries_what_pytorch_s_does():
         assert torch.equal(transform(own)(x), transform(plain)(x))
     y = own(x.as_subclass(Sub))
     assert type(y) is Sub and torch.equal(y.as_subclass(torch.Tensor), plain(x))
+
+
+@pytest.mark.parametrize("records", [False, True])
+def test_conv1d_silu_says_the_same_whether_it_records_or_not(records):
+    x = torch.randn(2, 30, 8, device=DEV).requires_grad_(records)
+    w = torch.randn(8, 1, 4, device=DEV)
+    for error, args in ((ValueError, (x, w, torch.zeros(7, device=DEV))), (ValueError, (x, w[:4])), (ValueError, (x, w.reshape(8, 2, 2))),
+                        (ValueError, (x, w.cpu())), (ValueError, (x.transpose(1, 2), w)), (NotImplementedError, (x, w[..., :1])),
+                        (NotImplementedError, (x[..., :7], w[:7])), (NotImplementedError, (x, w.repeat(1, 1, 2))), (W().SsdError, (x[:, :0], w))):
+        with pytest.raises(error):
+            W().conv1d_silu(*args)
+
+
+@pytest.mark.parametrize("of", ["x", "w", "bias"])
+def test_conv1d_silu_takes_tensor_subclasses(of):
+    """The kernels read them, and gradients arrive at them."""
+    class Sub(torch.Tensor):
+        pass
+
+    v = {"x": torch.randn(2, 30, 8, device=DEV), "w": torch.randn(8, 1, 4, device=DEV), "bias": torch.randn(8, device=DEV)}
+    plain = {k: t.clone().requires_grad_(True) for k, t in v.items()}
+    sub = {k: (t.clone().as_subclass(Sub) if k == of else t.clone()).requires_grad_(True) for k, t in v.items()}
+    y, want = (W().conv1d_silu(*d.values()) for d in (sub, plain))
+    assert torch.equal(y, want)
+    dy = torch.randn_like(want)
+    for a, b in zip(torch.autograd.grad([y], list(sub.values()), [dy]), torch.autograd.grad([want], list(plain.values()), [dy])):
+        assert torch.equal(a.as_subclass(torch.Tensor), b)
+    with torch.no_grad():
+        assert torch.equal(W().conv1d_silu(*sub.values()), want)

@@ -88,6 +88,19 @@ def _rows_contiguous(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t.contiguous()
 
 
+def _plain(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
+    """A tensor of a subclass as the plain one that it is, for the kernels and for autograd (one without memory of its own stays what it is,
+    and is refused)."""
+    if t is None or type(t) in (torch.Tensor, torch.nn.Parameter):
+        return t
+    with torch._C.DisableTorchFunctionSubclass():
+        plain = t.as_subclass(torch.Tensor)
+        try:
+            return plain if plain.numel() == 0 or plain.data_ptr() else t
+        except RuntimeError:
+            return t
+
+
 def _check_out(out: torch.Tensor, like: torch.Tensor, name: str = "out"):
     if out.shape != like.shape or out.dtype != like.dtype or out.device != like.device:
         raise ValueError(f"{name} must have the shape {tuple(like.shape)}, dtype {like.dtype} and device of X")
@@ -320,17 +333,19 @@ def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
         raise ValueError("x must be [b,l,d] float32/float16/bfloat16 with a contiguous channel axis")
     b, l, d = x.shape
     _same_device(x, weight=weight, bias=bias, out=out)
-    w = weight.reshape(d, -1).to(x.dtype).contiguous()
+    if weight.dim() > 1 and (weight.shape[0] != d or weight.numel() != d * weight.shape[-1]):
+        raise ValueError("weight must be [d,1,k] or [d,k]")
+    if bias is not None and bias.shape != (d,):
+        raise ValueError("bias must be [d]")
+    x, w = _plain(x), _plain(weight).reshape(d, -1).to(x.dtype).contiguous()
     taps = w.shape[1]
-    if out is None and torch.is_grad_enabled() and (x.requires_grad or w.requires_grad or (bias is not None and bias.requires_grad)):
-        got = _lib.fast().conv1d_silu(x, w, None if bias is None else bias.to(x.dtype).contiguous(), None)
-        if got is None:
-            raise NotImplementedError("conv1d_silu: sizes outside what the kernels cover")
-        return got
     if bias is not None:
-        if bias.shape != (d,):
-            raise ValueError("bias must be [d]")
-        bias = bias.to(x.dtype).contiguous()
+        bias = _plain(bias).to(x.dtype).contiguous()
+    if out is None and torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, w, bias)):
+        got = _lib.fast().conv1d_silu(x, w, bias, None)
+        if got is None:
+            _raise(-1 if x.numel() == 0 else -4)     # (what the call without a gradient says)
+        return got
     if out is None:
         out = torch.empty((b, l, d), dtype=x.dtype, device=x.device)
     else:
