@@ -222,3 +222,20 @@ def test_conv1d_silu_takes_tensor_subclasses(of):
         assert torch.equal(a.as_subclass(torch.Tensor), b)
     with torch.no_grad():
         assert torch.equal(W().conv1d_silu(*sub.values()), want)
+
+
+def test_numbers_that_32_bits_do_not_hold_are_refused():
+    """A limit of 2^32 milliseconds was taken as none, one of 2^70 and as many groups were a SystemError."""
+    x, d, h = torch.randn(2, 300, 8, device=DEV), torch.zeros(8, device=DEV), torch.zeros(2, 8, device=DEV)
+    for bad in (dict(wait_limit_ms=2 ** 31), dict(wait_limit_ms=2 ** 32), dict(wait_limit_ms=2 ** 70), dict(rate=1e39), dict(rate=1e-50)):
+        with pytest.raises(ValueError):
+            W().gated_scan(x, x, x, d, **bad)
+    with pytest.raises(ValueError):
+        W().gated_scan_step(x[:, 0], x[:, 0], x[:, 0], d, h, rate=1e39)
+    for bad in (dict(groups=2 ** 33), dict(groups=2 ** 70), dict(groups=2 ** 32 + 1), dict(groups=0), dict(eps=1e39), dict(eps=-1e-60)):
+        with pytest.raises(ValueError):
+            W().gated_rms_norm(x, x, d, **bad)
+    with pytest.raises(ValueError):
+        W().rms_norm(x, d, eps=1e39)
+    a, b = W().gated_scan(x, x, x, d, wait_limit_ms=2 ** 31 - 1), W().gated_scan(x, x, x, d)
+    assert torch.equal(a, b) and torch.equal(W().rms_norm(x, d + 1, eps=1e-60), W().rms_norm(x, d + 1, eps=0.0))

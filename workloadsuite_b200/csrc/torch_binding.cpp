@@ -284,6 +284,13 @@ bool real(PyObject* o, float* v) {
   return true;
 }
 bool fits(int64_t n) { return n > 0 && n <= 0x7fffffff; }
+bool whole(PyObject* o, int* v) {   // a number of 32 bits
+  if (!PyLong_CheckExact(o)) return false;
+  int over = 0;
+  const long n = PyLong_AsLongAndOverflow(o, &over);
+  *v = (int)n;
+  return over == 0 && n == (long)*v;
+}
 // fp32, whole and contiguous, or not given
 bool plain32(const Tensor& t, std::initializer_list<int64_t> s) {
   return !t.defined() || (t.scalar_type() == at::kFloat && shaped(t, s) && t.is_contiguous());
@@ -437,12 +444,12 @@ PyObject* py_gated(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Tensor *x, *i, *r, *decay, *init, *reset, *out;
   float rate;
+  int wait_ms;
   if (n != 9 || !get(o[0], &x) || !get(o[1], &i) || !get(o[2], &r) || !get(o[3], &decay) || !get(o[4], &init, true) ||
-      !get(o[5], &reset, true) || !get(o[6], &out, true) || !real(o[7], &rate) || !PyLong_CheckExact(o[8]) || !x->is_cuda() ||
+      !get(o[5], &reset, true) || !get(o[6], &out, true) || !real(o[7], &rate) || !whole(o[8], &wait_ms) || !x->is_cuda() ||
       x->dim() != 3 || i->dim() != 3 || r->dim() != 3 || dtype_of(*x) < 0)
     Py_RETURN_NONE;
   if (tangents({x, i, r, decay, init})) Py_RETURN_NONE;
-  const int wait_ms = (int)PyLong_AsLong(o[8]);
   int rc = 0;
   if (records({x, i, r, decay, init})) {
     if (out->defined()) Py_RETURN_NONE;
@@ -715,10 +722,10 @@ PyObject* py_gated_norm(PyObject*, PyObject* const* o, Py_ssize_t n) {
   HANDLE_TH_ERRORS
   const Tensor *x, *z, *wt, *out;
   float eps;
+  int groups;
   if (n != 7 || !get(o[0], &x) || !get(o[1], &z) || !get(o[2], &wt) || !get(o[3], &out, true) || !real(o[4], &eps) ||
-      !PyLong_CheckExact(o[5]) || !norm_operand(*x) || tangents({x, z, wt}))
+      !whole(o[5], &groups) || !norm_operand(*x) || tangents({x, z, wt}))
     Py_RETURN_NONE;
-  const long groups = PyLong_AsLong(o[5]);
   const bool first = o[6] == Py_True;
   int rc = 0;
   if (records({x, z, wt})) {

@@ -8,6 +8,7 @@ refused (NotImplementedError).
 """
 from __future__ import annotations
 
+import ctypes
 import math
 from typing import Optional
 
@@ -31,6 +32,11 @@ def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
+def _real(v: float) -> float:
+    """As the kernels get it, in 32 bits."""
+    return ctypes.c_float(v).value
+
+
 def _done(got, name: str):
     if got is None:
         raise NotImplementedError(f"{name}: sizes or strides outside what the kernels cover")
@@ -51,8 +57,8 @@ def _check_gates(name, x, input_gate, decay_gate, decay, dims, rate):
             raise ValueError(f"{what} must have the shape and dtype of x")
     if decay.shape != x.shape[-1:] or decay.dtype not in _DTYPES:
         raise ValueError("decay must be a floating point [d]")
-    if not 0 < rate < math.inf:
-        raise ValueError("rate must be positive and finite")
+    if not 0 < _real(rate) < math.inf:
+        raise ValueError("rate must be positive and finite in float32")
 
 
 def _check_state(name, t, x):
@@ -91,8 +97,8 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     _check_gates("gated_scan", x, input_gate, decay_gate, decay, 3, rate)
     _no_tangents("gated_scan", x, input_gate, decay_gate, decay, initial_state)
     _same_device(x, initial_state=initial_state, reset=reset, out=out)
-    if wait_limit_ms < 0:
-        raise ValueError("wait_limit_ms must not be negative")
+    if not 0 <= wait_limit_ms < 1 << 31:
+        raise ValueError("wait_limit_ms must not be negative, nor 2^31 and more")
     if initial_state is not None:
         _check_state("initial_state", initial_state, x)
         initial_state = initial_state.contiguous()
@@ -167,8 +173,8 @@ def _check_norm(name, x, eps, vectors, rows, groups=1):
             raise ValueError(f"{what} must have the shape of x")
     if x.shape[-1] == 0:
         raise ValueError("rows must not be empty")
-    if not 0 <= eps < math.inf:
-        raise ValueError("eps must be finite and not negative")
+    if not 0 <= _real(eps) < math.inf or eps < 0:
+        raise ValueError("eps must be finite in float32 and not negative")
     if groups <= 0 or x.shape[-1] % groups != 0:
         raise ValueError("groups must divide d")
 
