@@ -239,3 +239,29 @@ def test_numbers_that_32_bits_do_not_hold_are_refused():
         W().rms_norm(x, d, eps=1e39)
     a, b = W().gated_scan(x, x, x, d, wait_limit_ms=2 ** 31 - 1), W().gated_scan(x, x, x, d)
     assert torch.equal(a, b) and torch.equal(W().rms_norm(x, d + 1, eps=1e-60), W().rms_norm(x, d + 1, eps=0.0))
+
+
+def test_the_block_s_operators_take_tensor_subclasses():
+    class Sub(torch.Tensor):
+        pass
+
+    sub = lambda t: t.detach().clone().as_subclass(Sub)
+    same = lambda a, b: torch.equal(a.as_subclass(torch.Tensor), b)
+    v = scan_inputs(2, 70, 16, torch.float16, True, True, seed=3)
+    args, w = (v["x"], v["i"], v["r"], v["decay"]), torch.randn(16, device=DEV)
+    want = W().gated_scan(*args, initial_state=v["h"], reset=v["reset"])
+    for n in range(6):
+        given = [sub(t) if m == n else t for m, t in enumerate((*args, v["h"], v["reset"]))]
+        assert torch.equal(W().gated_scan(*given[:4], initial_state=given[4], reset=given[5]), want)
+    out = sub(want)
+    assert same(W().gated_scan(*args, initial_state=v["h"], reset=v["reset"], out=out.zero_()), want) and same(out, want)
+    state, other = v["h"].clone(), sub(v["h"])
+    y = W().gated_scan_step(*(t[:, 0] for t in args[:3]), args[3], state)
+    assert torch.equal(W().gated_scan_step(*(sub(t[:, 0]) for t in args[:3]), sub(args[3]), other), y) and same(other, state)
+    for call, ops in ((W().rms_norm, (v["x"], w)), (lambda x, w, r: W().rms_norm(x, w, residual=r)[0], (v["x"], w, v["dy"])),
+                      (W().gated_rms_norm, (v["x"], v["i"], w))):
+        plain, given = ([t.clone().requires_grad_(True) for t in ops], [sub(t).requires_grad_(True) for t in ops])
+        want, got = call(*plain), call(*given)
+        assert same(got, want)
+        for a, b in zip(torch.autograd.grad([got], given, [v["dy"]]), torch.autograd.grad([want], plain, [v["dy"]])):
+            assert same(a, b)

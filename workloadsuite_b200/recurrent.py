@@ -15,7 +15,7 @@ from typing import Optional
 import torch
 
 from . import _lib
-from .ssd import _DTYPES, _check_out, _no_tangents, _same_device
+from .ssd import _DTYPES, _check_out, _no_tangents, _plain, _same_device
 
 
 def _records(*tensors) -> bool:
@@ -29,6 +29,7 @@ def _need_cuda(name: str, x: torch.Tensor):
 
 def _rows(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """A tensor whose channels do not lie side by side is copied once; anything else stays the view it is."""
+    t = _plain(t)
     return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
 
 
@@ -101,14 +102,15 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
         raise ValueError("wait_limit_ms must not be negative, nor 2^31 and more")
     if initial_state is not None:
         _check_state("initial_state", initial_state, x)
-        initial_state = initial_state.contiguous()
+        initial_state = _plain(initial_state).contiguous()
     if reset is not None and (reset.shape != x.shape[:2] or reset.dtype != torch.bool):
         raise ValueError("reset must be bool [b,s]")
     if out is not None:
         if _records(x, input_gate, decay_gate, decay, initial_state):
             raise ValueError("out cannot be given where a gradient is recorded")
         _check_out(out, x)
-    x, input_gate, decay_gate, decay = _rows(x), _rows(input_gate), _rows(decay_gate), decay.float().contiguous()
+    x, input_gate, decay_gate, decay = _rows(x), _rows(input_gate), _rows(decay_gate), _plain(decay).float().contiguous()
+    reset, out = _plain(reset), _plain(out)
     if x.numel() == 0:      # no tokens: the state stays what it was
         y = (x + input_gate + decay_gate) * decay.to(x.dtype) if out is None else out
         fin = x.new_zeros((x.shape[0], x.shape[2]), dtype=torch.float32) if initial_state is None else initial_state.clone()
@@ -140,8 +142,8 @@ def gated_scan_step(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch
         _check_out(out, x)
     if x.numel() == 0:
         return torch.empty_like(x) if out is None else out
-    return _done(_lib.fast().gated_step(_rows(x), _rows(input_gate), _rows(decay_gate), decay.detach().float().contiguous(), state,
-                                        out_state, out, rate), "gated_scan_step")
+    return _done(_lib.fast().gated_step(_rows(x), _rows(input_gate), _rows(decay_gate), _plain(decay).detach().float().contiguous(), _plain(state),
+                                        _plain(out_state), _plain(out), rate), "gated_scan_step")
 
 
 # ---- norms ----------------------------------------------------------------------------------------------
@@ -151,6 +153,7 @@ _EPS = torch.finfo(torch.float32).eps     # what nn.RMSNorm takes where none is 
 
 def _flat(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     """[..., d] whose rows do not lie at one distance is copied once."""
+    t = _plain(t)
     if t is None or t.dim() < 2:
         return t if t is None or t.stride(-1) == 1 or t.shape[-1] == 1 else t.contiguous()
     try:
@@ -207,9 +210,10 @@ def rms_norm(x: torch.Tensor, weight: torch.Tensor, eps: Optional[float] = None,
         if _records(x, weight, residual, post_weight, scale):
             raise ValueError("out cannot be given where a gradient is recorded")
         _check_out(out, x)
+        out = _plain(out)
         if _flat(out) is not out:
             raise ValueError("out: rows must lie at one distance from each other")
-    weight, post_weight, scale = (None if t is None else t.contiguous() for t in (weight, post_weight, scale))
+    weight, post_weight, scale = (None if t is None else _plain(t).contiguous() for t in (weight, post_weight, scale))
     x, residual = _flat(x), _flat(residual)
     if x.numel() == 0:
         for t in (post_weight, scale):
@@ -242,9 +246,10 @@ def gated_rms_norm(x: torch.Tensor, z: torch.Tensor, weight: torch.Tensor, eps: 
         if _records(x, z, weight):
             raise ValueError("out cannot be given where a gradient is recorded")
         _check_out(out, x)
+        out = _plain(out)
         if _flat(out) is not out:
             raise ValueError("out: rows must lie at one distance from each other")
-    x, z, weight = _flat(x), _flat(z), weight.contiguous()
+    x, z, weight = _flat(x), _flat(z), _plain(weight).contiguous()
     if x.numel() == 0:
         return x * z * weight.to(x.dtype) if out is None else out
     return _done(_lib.fast().gated_rms_norm(x, z, weight, out, eps, groups, norm_first), "gated_rms_norm")
