@@ -265,3 +265,22 @@ def test_the_block_s_operators_take_tensor_subclasses():
         assert same(got, want)
         for a, b in zip(torch.autograd.grad([got], given, [v["dy"]]), torch.autograd.grad([want], plain, [v["dy"]])):
             assert same(a, b)
+
+
+def test_a_backward_pass_notices_that_what_it_saved_was_written_over():
+    """By `out`, or by a step's state: an error as for any operator that works in place, not a gradient of other numbers."""
+    x, w, h = torch.randn(2, 16, device=DEV), torch.randn(16, device=DEV), torch.zeros(2, 16, device=DEV)
+    cw = torch.randn(16, 1, 2, device=DEV)
+    calls = {"gated_scan": lambda o: W().gated_scan(x[None], x[None], x[None], w, out=o[None]),
+             "step's y": lambda o: W().gated_scan_step(x, x, x, w, h, out=o), "step's state": lambda o: W().gated_scan_step(x, x, x, w, o),
+             "step's new state": lambda o: W().gated_scan_step(x, x, x, w, h, out_state=o), "rms_norm": lambda o: W().rms_norm(x, w, out=o),
+             "gated_rms_norm": lambda o: W().gated_rms_norm(x, x, w, out=o), "conv1d_silu": lambda o: W().conv1d_silu(x[None], cw, out=o[None]),
+             "conv1d_silu, the long way": lambda o: W().conv1d_silu(x[None], cw.double(), out=o[None])}
+    for name, call in calls.items():
+        leaf, saved = torch.ones(2, 16, device=DEV, requires_grad=True), torch.randn(2, 16, device=DEV)
+        y = leaf * saved
+        call(saved)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            y.sum().backward()
+        with torch.inference_mode():
+            call(torch.randn(2, 16, device=DEV))

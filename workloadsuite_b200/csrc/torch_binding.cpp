@@ -319,6 +319,10 @@ bool tangents(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->_fw_grad(0).defined()) return true;
   return false;
 }
+// A tensor that a kernel has written over: a backward pass that saved it is to notice.
+void written(const Tensor& t) {
+  if (t.defined() && !t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
 Maybe maybe(const Tensor& t) { return t.defined() ? Maybe(t) : std::nullopt; }
 Tensor given(const Maybe& t) { return t ? *t : Tensor(); }
 // A gradient whose innermost axis is not contiguous (a sum's is expanded) is copied once.
@@ -385,6 +389,7 @@ bool gated_forward(const Tensor& x, const Tensor& i, const Tensor& r, const Tens
   a.workspace = ptr(ws);
   a.workspace_bytes = need;
   *rc = f_gated(&a, w.stream());
+  written(out);
   return true;
 }
 bool gated_backward(const Tensor& x, const Tensor& i, const Tensor& r, const Tensor& decay, const Tensor& reset, const Tensor& pieces,
@@ -488,6 +493,8 @@ PyObject* py_gated_step(PyObject*, PyObject* const* o, Py_ssize_t n) {
   a.batch = (int)b; a.channels = (int)d; a.dtype = dtype_of(*x);
   a.x_stride = x->stride(0); a.input_gate_stride = i->stride(0); a.decay_gate_stride = r->stride(0); a.y_stride = y.stride(0);
   if (const int rc = f_gated_step(&a, w.stream())) return declined(rc);
+  written(state_out->defined() ? *state_out : *state);
+  written(*out);
   return THPVariable_Wrap(std::move(y));
   END_HANDLE_TH_ERRORS
 }
@@ -582,6 +589,7 @@ bool norm_forward(const Tensor& x, const Tensor& wt, const Tensor& res, const Te
   c.a.inv_rms_post = ptr<float>(v->invp);
   c.a.eps = eps;
   *rc = f_norm(&c.a, c.w.stream());
+  written(out);
   return true;
 }
 // like: x, or where nothing of it is read a tensor of its shape and type
@@ -684,6 +692,7 @@ bool gated_norm_forward(const Tensor& x, const Tensor& z, const Tensor& wt, cons
   c.a.inv_rms = ptr<float>(v->inv);
   c.a.eps = eps;
   *rc = f_gated_norm(&c.a, c.w.stream());
+  written(out);
   return true;
 }
 
@@ -756,6 +765,7 @@ bool conv_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Te
   *y = out.defined() ? out : at::empty(x.sizes(), x.options());
   *rc = f_conv(x.data_ptr(), w.data_ptr(), ptr(bias), y->data_ptr(), (int)x.size(0), (int)x.size(1), (int)x.size(2), (int)w.size(-1), dtype_of(x),
                x.stride(0), x.stride(1), y->stride(0), y->stride(1), q.stream());
+  written(out);
   return true;
 }
 // What the gradient reads two channels at a time of; other views are copied once.

@@ -358,6 +358,8 @@ def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
                                       C.c_void_p(torch.cuda.current_stream(x.device).cuda_stream))
     if rc != _lib.SSD_OK:
         _raise(rc)
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
     return out
 
 
