@@ -291,8 +291,8 @@ typedef struct SsdGatedScanArgs {
   float rate;                   /* > 0 */
   int32_t batch, seqlen, channels, dtype;
   int32_t wait_limit_ms;        /* 0: about one second */
-  int32_t inject_lost_tile;     /* testing the give-up path: the first CTA leaves without working, so those behind it in its sequence run into the
-                                   bound of their waits, report status 8 and leave; the results are then incomplete */
+  int32_t inject_lost_tile;     /* testing the give-up path: the CTA that has the first tile leaves without working, so those behind it in its sequence run
+                                   into the bound of their waits, report status 8 and leave; the results are then incomplete */
   int32_t reserved;
   int64_t x_stride[2], input_gate_stride[2], decay_gate_stride[2], reset_stride[2], y_stride[2];
   int64_t dy_stride[2], dx_stride[2], dinput_gate_stride[2], ddecay_gate_stride[2];

@@ -284,3 +284,31 @@ def test_a_backward_pass_notices_that_what_it_saved_was_written_over():
             y.sum().backward()
         with torch.inference_mode():
             call(torch.randn(2, 16, device=DEV))
+
+
+def test_a_tile_that_is_lost_on_purpose_is_the_first_one():
+    """Whichever CTA takes it: every such launch reports its waits (the first CTA may find no tile left, or one that nobody waits for)."""
+    import ctypes as C
+
+    from workloadsuite_b200 import _lib
+
+    lib, (b, s, d) = _lib.load(), (1, 300, 64)
+    v = scan_inputs(b, s, d, torch.bfloat16, False, False, seed=8)
+    y, status = torch.zeros_like(v["x"]), torch.zeros(1, dtype=torch.int32, device=DEV)
+    a = _lib.GatedScanArgs()
+    a.x, a.input_gate, a.decay_gate, a.decay = (v[k].data_ptr() for k in ("x", "i", "r", "decay"))
+    a.y, a.status = y.data_ptr(), status.data_ptr()
+    a.rate, a.batch, a.seqlen, a.channels, a.dtype, a.wait_limit_ms, a.inject_lost_tile = 8.0, b, s, d, _lib.DTYPE_BF16, 5, 1
+    for f in ("x", "input_gate", "decay_gate", "y"):
+        setattr(a, f + "_stride", (C.c_int64 * 2)(s * d, d))
+    ws = torch.empty(lib.ssd_b200_gated_scan_workspace_bytes(C.byref(a), 0), dtype=torch.uint8, device=DEV)
+    a.workspace, a.workspace_bytes = ws.data_ptr(), ws.numel()
+    side = torch.cuda.Stream()
+    m = torch.randn(2048, 2048, device=DEV)
+    for n in range(100):
+        status.zero_()
+        with torch.cuda.stream(side):
+            m @ m
+        assert lib.ssd_b200_gated_scan(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
+        torch.cuda.synchronize()
+        assert status.item() == 8, n

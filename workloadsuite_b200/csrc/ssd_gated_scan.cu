@@ -433,7 +433,7 @@ gated_scan_kernel(const __grid_constant__ Scan p, const __grid_constant__ Maps m
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
-    if (p.inject && blockIdx.x == 0) break;   // (SsdGatedScanArgs::inject_lost_tile)
+    if (p.inject && sh.which[s].x == 0 && sh.which[s].y == 0) break;   // (SsdGatedScanArgs::inject_lost_tile)
     if (p.early && turn == 0 && threadIdx.x == 32 * (kRuns - 1))   // (when every CTA has its first)
       send_for<T, TMA, 3, kTile>(p, maps, &sh.which[1], &sh.full[1], 1, stages + kStage, false, sh.rate[1], nullptr);
     const int4 which = sh.which[s];
@@ -616,7 +616,7 @@ gated_scan_grad_kernel(const __grid_constant__ Scan p, const __grid_constant__ M
     const int s = turn & 1;
     T* const stage = stages + s * kStage;
     wait_for(p, sh, &sh.full[s], turn >> 1 & 1);
-    if (p.inject && blockIdx.x == 0) break;   // (SsdGatedScanArgs::inject_lost_tile)
+    if (p.inject && sh.which[s].x == 0 && sh.which[s].y == 0) break;   // (SsdGatedScanArgs::inject_lost_tile)
     const int4 which = sh.which[s];
     if (which.x < 0) break;
     const int kb = which.x, k = p.tiles - 1 - kb, unit = which.y, strip = which.z, b = which.w;
