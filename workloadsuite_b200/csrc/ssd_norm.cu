@@ -31,17 +31,14 @@ __device__ __forceinline__ void four(F f) {
 #pragma unroll
   for (int e = 0; e < 4; ++e) f(e);
 }
-__device__ __forceinline__ Pair words_to_pair(const float*, const uint4& q, int e) {
-  return e == 0 ? pair(__uint_as_float(q.x), __uint_as_float(q.y)) : pair(__uint_as_float(q.z), __uint_as_float(q.w));
-}
+__device__ __forceinline__ Pair words_to_pair(uint32_t lo, uint32_t hi) { return pair(__uint_as_float(lo), __uint_as_float(hi)); }
 template <typename T>
 __device__ __forceinline__ Eight widen(const uint4& a, const uint4& b) {
   Eight r;
   if constexpr (sizeof(T) == 2) {
     r[0] = pair_of<T>(a.x); r[1] = pair_of<T>(a.y); r[2] = pair_of<T>(a.z); r[3] = pair_of<T>(a.w);
   } else {
-    const float* t = nullptr;
-    r[0] = words_to_pair(t, a, 0); r[1] = words_to_pair(t, a, 1); r[2] = words_to_pair(t, b, 0); r[3] = words_to_pair(t, b, 1);
+    r[0] = words_to_pair(a.x, a.y); r[1] = words_to_pair(a.z, a.w); r[2] = words_to_pair(b.x, b.y); r[3] = words_to_pair(b.z, b.w);
   }
   return r;
 }
@@ -247,7 +244,7 @@ struct Forward {
   // residual: 50 us for 8 192 rows without, 56 with).  One sum: 52 and 52 at 2 048, 91 and 98 at 8 192.
   static constexpr int kPieces = I * (int)(sizeof(T) + sizeof(R)) / 2, kStages = OUTER ? 0 : stages_of(kPieces);
   static constexpr bool kAhead = VEC && kStages > 0;
-  static constexpr bool kKeep = I <= 2 && !OUTER;   // vectors stay in registers
+  static constexpr bool kKeep = I <= 2 && !OUTER;   // the weight stays in registers
 };
 template <typename T, typename R, int I, bool VEC, bool OUTER>
 __global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_kernel(const Norm p) {
@@ -257,13 +254,10 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_kernel(const Norm
   clear(sums);
   RowSum row_sum{sums, 0};
   const Ahead<F::kPieces, F::kStages> ahead;
-  Eight w[I], ps[I];
+  Eight w[I];
   if constexpr (F::kKeep) {
 #pragma unroll
-    for (int it = 0; it < I; ++it) {
-      w[it] = p.w.get<T, VEC>(0, it, p.d);
-      if constexpr (OUTER) ps[it] = p.outer<T, VEC>(it);
-    }
+    for (int it = 0; it < I; ++it) w[it] = p.w.get<T, VEC>(0, it, p.d);
   }
   auto x = rows_in<T>(p.x, p.xs);
   auto res = rows_in<R>(p.res, p.rs);
@@ -291,8 +285,8 @@ __global__ void __launch_bounds__(I == 1 ? 128 : 512) rms_norm_kernel(const Norm
           }
 #pragma unroll
           for (int it = 0; it < I; ++it) {
-            if constexpr (!F::kKeep) ps[it] = p.outer<T, VEC>(it);
-            four([&](int e) { v[it][e] = v[it][e] * both(inv) * ps[it][e]; });
+            const Eight ps = p.outer<T, VEC>(it);
+            four([&](int e) { v[it][e] = v[it][e] * both(inv) * ps[e]; });
           }
         }
         if (p.res) {
