@@ -927,9 +927,11 @@ int run_scan(const SsdGatedScanArgs& a, bool grad, cudaStream_t stream) {
   using Bwd = Geometry<T, true>;
   const unsigned grid = std::min(p.total, 148u * (grad ? Bwd::kCtas : Fwd::kCtas));
   // Where many tiles of one sequence are worked on at a time their numbers are taken as late as their inputs allow, so that a tile does not
-  // wait for one that is started after it: 131 072 x 2 048 bf16 (9 at a time) 494 us, taken two tiles ahead 538.  With fewer the
-  // inputs' way counts for more: 8 x 2 048 x 2 048 (1) 62 and 66, 3 x 1 021 x 1 536 fp16 (4) 16.6 and 17.6.  (Copies by threads are late ones.)
-  p.early = grid <= 6 * z.units && (tma || sizeof(T) == 2);
+  // wait for one that is started after it; with fewer the inputs' way counts for more.  One sequence of 2^26 numbers bf16 (2^25 fp32), us, taken
+  // two tiles ahead and late: 9.25 tiles at a time 138.5 131.7 (109.7 104.4), 7 132.0 130.0 (104.7 101.7), 6 129.9 128.5 (103.0 100.8), 5 127.4 126.7
+  // (100.3 100.1), 4.6 125.8 125.3 (99.6 100.1), 4 124.8 125.0 (98.2 100.2), 3 122.4 124.0 (95.8 100.2), 2 119.9 121.5 (92.4 98.6).
+  // (Copies by threads are late ones.)
+  p.early = 2 * (int64_t)grid <= 9 * z.units && (tma || sizeof(T) == 2);
   p.enter_ahead = grad && tma && reinterpret_cast<uintptr_t>(a.pieces) % 16 == 0 && a.channels % 4 == 0;
   auto go = [&](auto kernel, int threads, size_t smem) {
     if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem) != cudaSuccess) return (int)SSD_ERR_CUDA;
