@@ -265,8 +265,8 @@ conv1d_silu_staged_kernel(const T* __restrict__ x, const T* __restrict__ w, cons
   for (int p = 0; p < kStages - 1; ++p) issue(p);
 
   // Taps and bias times -log2 e, so that with v = -log2(e) a the sums are exponents as they are: silu(a) = v / (-log2(e) (1 + 2^v)).
-  // Two special functions an element and a row's issue slots cost 8 % (b4 s8192 h80: 122 us) beside one tanh.approx (112), which is no
-  // function to round once to 16 bits below -4; a polynomial in 2^-|v| in place of the reciprocal 137; scaling behind the sums 124.5.
+  // Two special functions an element (tanh.approx, a single one, is no function to round once to 16 bits below -4): b4 s8192 h80 114 us,
+  // 113 with that one; 122 with a branch ahead of every row, 137 with a polynomial in 2^-|v| in place of the reciprocal.
   const f32x2 scale2 = pack_f2(-kLog2E, -kLog2E);
   f32x2 wk[K][4], bs[4];
 #pragma unroll
@@ -292,27 +292,32 @@ conv1d_silu_staged_kernel(const T* __restrict__ x, const T* __restrict__ w, cons
     issue(piece + kStages - 1);
     cp_async_wait<kStages - 1>();   // this thread's copies of `piece` have landed (it is their only reader)
     const int t0 = t_begin + piece * kPiece, st = piece % kStages;
+    auto row = [&](int u) {
+      const int s = (4 + u) & 7;
+      uint4 q;
+      asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(slot_addr(st, u)));
+      widen(q, win[s]);
+      uint32_t o[4];
 #pragma unroll
-    for (int u = 0; u < kPiece; ++u) {
-      if (t0 + u < t_end) {
-        const int s = (4 + u) & 7;
-        uint4 q;
-        asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(q.x), "=r"(q.y), "=r"(q.z), "=r"(q.w) : "r"(slot_addr(st, u)));
-        widen(q, win[s]);
-        uint32_t o[4];
+      for (int j = 0; j < 4; ++j) {
+        f32x2 acc = bs[j];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-          f32x2 acc = bs[j];
-#pragma unroll
-          for (int k = 0; k < K; ++k) acc = fma_f2(wk[k][j], win[(s + 8 - (K - 1) + k) & 7][j], acc);
-          float a0, a1;
-          unpack_f2(acc, a0, a1);
-          unpack_f2(fma_f2(pack_f2(exp2_approx(a0), exp2_approx(a1)), scale2, scale2), a0, a1);
-          unpack_f2(mul_f2(acc, pack_f2(rcp_approx(a0), rcp_approx(a1))), a0, a1);
-          o[j] = pk2(xcol, a0, a1);
-        }
-        *reinterpret_cast<uint4*>(ycol + (int64_t)(t0 + u) * ysl) = make_uint4(o[0], o[1], o[2], o[3]);
+        for (int k = 0; k < K; ++k) acc = fma_f2(wk[k][j], win[(s + 8 - (K - 1) + k) & 7][j], acc);
+        float a0, a1;
+        unpack_f2(acc, a0, a1);
+        unpack_f2(fma_f2(pack_f2(exp2_approx(a0), exp2_approx(a1)), scale2, scale2), a0, a1);
+        unpack_f2(mul_f2(acc, pack_f2(rcp_approx(a0), rcp_approx(a1))), a0, a1);
+        o[j] = pk2(xcol, a0, a1);
       }
+      *reinterpret_cast<uint4*>(ycol + (int64_t)(t0 + u) * ysl) = make_uint4(o[0], o[1], o[2], o[3]);
+    };
+    if (t0 + kPiece <= t_end) {   // (rows beside each other, no branch between them: their functions' latency is what the kernel waits for)
+#pragma unroll
+      for (int u = 0; u < kPiece; ++u) row(u);
+    } else {
+#pragma unroll
+      for (int u = 0; u < kPiece; ++u)
+        if (t0 + u < t_end) row(u);
     }
   }
   cp_async_wait<0>();
@@ -322,7 +327,7 @@ conv1d_silu_staged_kernel(const T* __restrict__ x, const T* __restrict__ w, cons
 // tokens and some ten for the rows before and the start, and with what it shares the SM with (two 1.4, three 2.0 times that of one alone, from
 // b1 s4096 h32: 64 tokens, one block an SM, 12.8 us, 32 10.0, 24 11.0; b1 s8192 h24: 64 13.6, 32 11.1; b2 s4096 h48: 64 23.8, 56 22.4; b4 s333
 // h80: 32 8.2, 16 7.2).  Otherwise the longest: what is read at a time lies closer together than with longer ones (b4 s8192 h80: 56
-// 115 us, 64 113, 96 114, 192 121, 376, which is a single round, 133).  (Measured with one special function an element; with two all are up to a tenth longer.)
+// 115 us, 64 113, 96 114, 192 121, 376, which is a single round, 133).  (Measured with one special function an element.)
 int staged_run(int64_t columns, int seqlen) {
   constexpr int kShare[3] = {5, 7, 10};
   int best = kLongestRun, cost = 1 << 30;
