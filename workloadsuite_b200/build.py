@@ -76,9 +76,14 @@ def _torch_flags(torch):
     return ["-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
 
 
+# PyTorch's C++ runtime by its name: a compiler that has the archive alone links it in, and with two of them in one process a message
+# that is put together from a number ends it.
+TORCH_LIBRARIES = ["-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda", "-l:libstdc++.so.6"]
+
+
 def _torch_fingerprint(torch) -> str:
     """What the binding was built from and against: it holds inline code of one PyTorch's C++ headers and one Python's."""
-    return _hash([BINDING, HEADER], " ".join(_torch_flags(torch)), torch.__version__, str(sysconfig.get_config_var("EXT_SUFFIX")))
+    return _hash([BINDING, HEADER], " ".join(_torch_flags(torch) + TORCH_LIBRARIES), torch.__version__, str(sysconfig.get_config_var("EXT_SUFFIX")))
 
 
 def source_fingerprint() -> str:
@@ -103,14 +108,14 @@ def is_current() -> bool:
         torch is None or _stamped(TORCH_LIB, TORCH_STAMP, _torch_fingerprint(torch)))
 
 
-def _start_torch_binding(torch):
+def _start_torch_binding(torch, source: Path = BINDING):
     """Compiles ``csrc/torch_binding.cpp`` (a CPython module on PyTorch's C++ API) in the background."""
     root = Path(torch.__file__).resolve().parent
     cuda = Path(_nvcc()).resolve().parent.parent
     cmd = [os.environ.get("CXX") or shutil.which("g++") or "c++", *_torch_flags(torch),
            "-I", str(HEADER.parent), "-I", str(root / "include"), "-I", str(root / "include/torch/csrc/api/include"),
-           "-I", str(cuda / "include"), "-I", sysconfig.get_paths()["include"], str(BINDING), "-o", str(TORCH_LIB),
-           "-L", str(root / "lib"), f"-Wl,-rpath,{root / 'lib'}", "-ltorch_python", "-ltorch_cpu", "-lc10", "-lc10_cuda"]
+           "-I", str(cuda / "include"), "-I", sysconfig.get_paths()["include"], str(source), "-o", str(TORCH_LIB),
+           "-L", str(root / "lib"), f"-Wl,-rpath,{root / 'lib'}", *TORCH_LIBRARIES]
     return subprocess.Popen(cmd, stdout=subprocess.PIPE, stderr=subprocess.STDOUT, text=True)
 
 
