@@ -8,7 +8,7 @@ from pathlib import Path
 import pytest
 import torch
 
-from test_recurrent_gpu import DEV, DTYPES, W, _no_wait_ran_out, check, leaves, scan_inputs, scan_reference  # noqa: F401
+from test_recurrent_gpu import DELTA, DEV, DTYPES, W, _no_wait_ran_out, check, leaves, scan_inputs, scan_reference  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -312,3 +312,30 @@ def test_a_tile_that_is_lost_on_purpose_is_the_first_one():
         assert lib.ssd_b200_gated_scan(C.byref(a), C.c_void_p(torch.cuda.current_stream().cuda_stream)) == 0
         torch.cuda.synchronize()
         assert status.item() == 8, n
+
+
+@pytest.mark.parametrize("b,s", [(1, 1), (1, 5), (3, 1)])
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_conv1d_silu_gradient_of_rows_that_start_anywhere(dtype, b, s):
+    """x and dy one number off the boundary of two, single rows among them: strides of one row may be anything, and it counts as contiguous."""
+    d, taps = 24, 3
+    gen = torch.Generator(device=DEV).manual_seed(b + s)
+    rnd = lambda *n: torch.randn(*n, generator=gen, device=DEV).to(dtype)
+    x, dy, w = rnd(b, s, d), rnd(b, s, d), rnd(d, 1, taps)
+
+    def off(t, width):
+        buf = torch.zeros(b, s, width, dtype=dtype, device=DEV)
+        buf[..., 5:5 + d] = t
+        return buf[..., 5:5 + d]
+
+    def run(x, dy):
+        ins = [x.detach().requires_grad_(True), w.detach().requires_grad_(True)]
+        y = W().conv1d_silu(*ins)
+        return [y.detach(), *torch.autograd.grad([y], ins, [dy])]
+
+    want = run(x, dy)
+    for width in (36, 37):
+        for a, c in ((off(x, width), dy), (x, off(dy, width)), (off(x, width), off(dy, width))):
+            for g, r in zip(run(a, c), want):
+                near = 2 * torch.finfo(dtype).eps * r.abs() + 2 * DELTA * r.abs().max()
+                assert ((g - r).abs() <= near).all()

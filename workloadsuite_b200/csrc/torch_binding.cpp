@@ -772,7 +772,7 @@ bool conv_forward(const Tensor& x, const Tensor& w, const Tensor& bias, const Te
 Tensor usable_pairs(const Tensor& t) {
   const bool ok = t.stride(2) == 1 && t.stride(0) % 2 == 0 && t.stride(1) % 2 == 0 &&
                   reinterpret_cast<uintptr_t>(t.data_ptr()) % (2 * t.element_size()) == 0;
-  return ok ? t : t.contiguous();
+  return ok ? t : t.clone(at::MemoryFormat::Contiguous);   // (a single row counts as contiguous wherever it starts)
 }
 
 struct ConvNode : torch::autograd::Function<ConvNode> {
