@@ -264,7 +264,8 @@ int ssd_b200_step_strided(const SsdStepArgs* args, void* stream);
  *   log a[t] = -rate * softplus(decay[c]) * sigmoid(decay_gate[t]),  b[t] = sqrt(1 - a[t]^2),
  *   h[t] = a[t] * h[t-1] + b[t] * sigmoid(input_gate[t]) * x[t],     y[t] = h[t]
  * (the carry of model_ref.py:152-157 with a state of one number per channel).  Strides in elements (batch, sequence; reset's
- * in bytes); channels contiguous.  A token whose reset byte is not 0 starts anew: h[t-1] is left out, whatever it is.
+ * in bytes); channels contiguous.  A token whose reset byte is not 0 starts anew: h[t-1] is left out, whatever it is
+ * (b[t] stays, which published blocks of this kind leave out there).  Gates that open less than 2^-126 count as shut.
  * The states entering every 64th token go to `pieces` when given: what ssd_b200_gated_scan_backward() starts from.
  * Results do not vary from run to run. */
 typedef struct SsdGatedScanArgs {

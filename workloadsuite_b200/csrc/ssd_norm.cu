@@ -1,11 +1,11 @@
 // RMS norms between blocks and their gradients (formulas: ssd_b200.h).
-// A row (of a group) is one warp's or one CTA's, eight numbers a thread and step, worked on in registers: every input is read once, every
-// output written once.  CTAs stay and take rows in turn; the inputs of the next rows are on their way (cp.async) while one is worked on, each
+// A row (of a group) is one warp's or one CTA's, eight numbers a thread and step, worked on in registers (but for what ptxas spills of the
+// gradients' sixteen and thirty-two numbers a thread, up to 1.1 KB): every input is read once, every output written once.  CTAs stay and take rows in turn; the inputs of the next rows are on their way (cp.async) while one is worked on, each
 // thread's into places that nobody else reads, so that waiting for its own copies is all the synchronisation they need.
 // The gradients against vectors are sums over rows: a CTA adds those of its rows up in registers and leaves
 // them to column_sum_kernel, so that their order is fixed.
-// Bound: HBM and, between a row's halves, its sums.  16 384 rows of 2 048 fp16 with residual: 51 us (5.3 TB/s, 81 % of the copy bandwidth), gradient 50;
-// gated, 8 192 rows of 8 x 1 024 bf16: 70 (89 %) and 122 (85 %).
+// Bound: HBM and, between a row's halves, its sums.  16 384 rows of 2 048 fp16 with residual: 52 us (5.2 TB/s, 80 % of the copy bandwidth), gradient 51;
+// gated, 8 192 rows of 8 x 1 024 bf16: 68 (91 %) and 124 (84 %).
 #include <algorithm>
 #include <cmath>
 #include <type_traits>

@@ -80,7 +80,8 @@ def gated_scan(x: torch.Tensor, input_gate: torch.Tensor, decay_gate: torch.Tens
     x, input_gate, decay_gate [b,s,d] in one dtype of float32/float16/bfloat16 (views with contiguous channels, such as columns of
     a projection's output, are read where they lie); decay [d], one number per channel, float32 or any of those;
     initial_state float32 [b,d] or None for zeros; reset bool [b,s]: a token that is marked starts anew, as if the state
-    before it were zero, whatever it was (documents packed into one row).  Gates, decays and the state are float32
+    before it were zero, whatever it was (documents packed into one row); the factor sqrt(1 - a^2) stays, which published blocks of this
+    kind drop at a document's first token.  Gates, decays and the state are float32
     throughout; y is rounded once, to x's dtype.  Sequences of no tokens are allowed.
 
     Returns y [b,s,d], with ``return_final_state`` also the float32 state [b,d] behind the last token (the

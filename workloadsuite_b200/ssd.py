@@ -321,7 +321,8 @@ def conv1d_silu(x: torch.Tensor, weight: torch.Tensor, bias: Optional[torch.Tens
     x [b,l,d] with a contiguous channel axis (a column slice of the projection output is fine); weight the
     ``nn.Conv1d(d, d, k, groups=d)`` parameter [d,1,k] (or [d,k]); bias [d] or None.  Returns [b,l,d] contiguous
     in x's dtype (fp32 accumulation, one rounding).  Differentiable in x, weight and bias (where ``out`` is given no
-    gradient is recorded), backward only: an operand with a forward-mode tangent is refused.
+    gradient is recorded), backward only: an operand with a forward-mode tangent is refused.  A row is one sequence: of documents packed
+    into one, the last k - 1 tokens reach into the next.
     """
     got = _lib.fast().conv1d_silu(x, weight, bias, out)
     if got is not None:
