@@ -214,3 +214,32 @@ def test_gated_scan_of_many_tiles(dtype, d, kind):
         check(a, ref[name], ref["m_" + name], s, name)
     for _ in range(3):
         assert all(torch.equal(a, c) for a, c in zip(got, call()))
+
+
+def test_gradients_past_32_bits():
+    """2.25e9 numbers a tensor (33 GB in all): the last rows, tokens and tiles are what the same numbers give by themselves."""
+    s, d, n = 1_100_032, 2048, 30_080         # whole tiles ahead of the last ones, so that sums are in the same order
+    gen = torch.Generator(device=DEV).manual_seed(1)
+    base = lambda: torch.randn(50_000, d, generator=gen, device=DEV).bfloat16().repeat(23, 1)[:s]
+    x, dy, w = base(), base(), (1 + 0.1 * torch.randn(d, generator=gen, device=DEV)).bfloat16()
+
+    def of(call, outs, *ops):
+        ins = [t.detach().requires_grad_(True) for t in ops]
+        y = call(*ins)
+        y = y if isinstance(y, tuple) else (y,)
+        return [t.detach() for t in y] + list(torch.autograd.grad([y[k] for k in outs], ins, [dy[-y[0].shape[-2]:].view_as(y[k]) for k in outs]))
+
+    def same(call, outs, *ops, skip=0):
+        full, tail = of(call, outs, *ops), of(call, outs, *(t[-n:] if t.shape[0] == s else t for t in ops))
+        for a, b in zip(full, tail):
+            if a.numel() == s * d:
+                assert torch.equal(a.view(s, d)[s - n + skip:], b.view(n, d)[skip:])
+            assert torch.isfinite(a.flatten()[-d:]).all()
+
+    same(lambda a, r, p: W().rms_norm(a, p, residual=r, post_weight=w, scale=w), (0, 1), x, x.flip(1), w)
+    same(lambda a, z, p: W().gated_rms_norm(a, z, p, groups=4), (0,), x, x.flip(1), w)
+    same(lambda a, c: W().conv1d_silu(a[None], c), (0,), x, (0.5 * torch.randn(d, 4, generator=gen, device=DEV)).bfloat16(), skip=3)
+    decay = torch.rand(d, generator=gen, device=DEV) - 6
+    with torch.no_grad():
+        _, h = W().gated_scan(*[x[None, :-n]] * 3, decay, return_final_state=True)
+    same(lambda a, i, r: W().gated_scan(a[None], i[None], r[None], decay, initial_state=h if a.shape[0] == n else None), (0,), x, x, x)
