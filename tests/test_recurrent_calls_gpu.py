@@ -339,3 +339,13 @@ def test_conv1d_silu_gradient_of_rows_that_start_anywhere(dtype, b, s):
             for g, r in zip(run(a, c), want):
                 near = 2 * torch.finfo(dtype).eps * r.abs() + 2 * DELTA * r.abs().max()
                 assert ((g - r).abs() <= near).all()
+
+
+@pytest.mark.parametrize("transform", [torch.func.vmap, lambda f: torch.func.grad(lambda t: f(t).sum()), lambda f: lambda t: torch.func.jvp(f, (t,), (t,))])
+def test_function_transforms_are_refused_by_name(transform):
+    w, decay = torch.ones(16, device=DEV), torch.zeros(16, device=DEV)
+    x = torch.randn(3, 2, 9, 16, device=DEV)
+    for name, call in (("gated_scan", lambda t: W().gated_scan(t, t, t, decay)), ("rms_norm", lambda t: W().rms_norm(t, w)),
+                       ("gated_rms_norm", lambda t: W().gated_rms_norm(t, t, w)), ("conv1d_silu", lambda t: W().conv1d_silu(t, torch.ones(16, 1, 2, device=DEV)))):
+        with pytest.raises(NotImplementedError, match=name):
+            transform(call)(x if transform is torch.func.vmap else x[0])

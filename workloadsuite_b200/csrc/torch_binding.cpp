@@ -313,10 +313,12 @@ bool records(std::initializer_list<const Tensor*> ts) {
     if (t->defined() && t->requires_grad()) return true;
   return false;
 }
-// Forward-mode gradients have no kernels: what carries one goes the long way, which says so.
+// Forward-mode gradients and function transforms have no kernels: what carries one goes the long way, which says so.
 bool tangents(std::initializer_list<const Tensor*> ts) {
   for (const Tensor* t : ts)
-    if (t->defined() && t->_fw_grad(0).defined()) return true;
+    if (t->defined() && (t->_fw_grad(0).defined() || t->key_set().has(c10::DispatchKey::FuncTorchBatched) ||
+                         t->key_set().has(c10::DispatchKey::FuncTorchGradWrapper)))
+      return true;
   return false;
 }
 // A tensor that a kernel has written over: a backward pass that saved it is to notice.

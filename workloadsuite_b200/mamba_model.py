@@ -27,7 +27,8 @@ _PKG_PARENT = str(Path(__file__).resolve().parent.parent)
 if _PKG_PARENT not in sys.path:
     sys.path.insert(0, _PKG_PARENT)
 
-from workloadsuite_b200.recurrent import rms_norm  # noqa: E402
+from workloadsuite_b200 import _lib  # noqa: E402
+from workloadsuite_b200.recurrent import _EPS, rms_norm  # noqa: E402
 from workloadsuite_b200.ssd import conv1d_silu, dt_prologue, ssd_forward  # noqa: E402
 
 
@@ -41,13 +42,22 @@ def _conv(x, weight, bias):
     return conv1d_silu(x, weight, bias)
 
 
+def _carries_more(*tensors) -> bool:
+    """Transforms, tangents and tensor subclasses, which PyTorch's operators carry and the kernels do not."""
+    plain, wrapped, dual = (torch.Tensor, nn.Parameter), torch._C._functorch.is_functorch_wrapped_tensor, forward_ad._current_level >= 0
+    for t in tensors:
+        if t is not None and (type(t) not in plain or wrapped(t) or (dual and forward_ad.unpack_dual(t).tangent is not None)):
+            return True
+    return False
+
+
 @torch.compiler.disable
 def _norm(x, weight, eps, residual):
-    given = [t for t in (x, weight, residual) if t is not None]
-    if all(type(t) in (torch.Tensor, nn.Parameter) and not torch._C._functorch.is_functorch_wrapped_tensor(t)
-           and (forward_ad._current_level < 0 or forward_ad.unpack_dual(t).tangent is None) for t in given):
+    got = _lib.fast().rms_norm(x, weight, residual, None, None, None, _EPS if eps is None else eps)     # (declines what has to be looked at)
+    if got is not None:
+        return got[0] if residual is None else got
+    if not _carries_more(x, weight, residual):
         return rms_norm(x, weight, eps=eps, residual=residual)
-    # transforms, tangents and tensor subclasses: PyTorch's operators carry them
     r = x if residual is None else residual + x
     y = nn.functional.rms_norm(r, (r.shape[-1],), weight, eps)
     return y if residual is None else (y, r)

@@ -109,7 +109,9 @@ def _check_out(out: torch.Tensor, like: torch.Tensor, name: str = "out"):
 
 
 def _no_tangents(name: str, *tensors):
-    """The gradients that the kernels have are backward ones: a tangent would be dropped without a word."""
+    """The gradients that the kernels have are backward ones, recorded by autograd: a tangent would be dropped without a word."""
+    if any(t is not None and torch._C._functorch.is_functorch_wrapped_tensor(t) for t in tensors):
+        raise NotImplementedError(f"{name} knows no function transforms (torch.func)")
     if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
         raise NotImplementedError(f"{name} has no forward-mode gradient")
 
