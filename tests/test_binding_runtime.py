@@ -61,3 +61,28 @@ def test_an_error_with_a_number_in_it_is_raised(tmp_path):
     assert job.returncode == 0, log
     r = subprocess.run([sys.executable, "-c", PROGRAM.format(path=str(out))], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "raised" in r.stdout, (r.returncode, r.stderr[-2000:])
+
+
+def test_a_subclass_without_memory_stays_what_it_is():
+    """One that wraps another tensor has no numbers of its own that a kernel could read: nothing is made of it that looks as if it had."""
+    from workloadsuite_b200.ssd import _plain
+
+    class Wrapper(torch.Tensor):
+        @staticmethod
+        def __new__(cls, inner):
+            return torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+
+        @classmethod
+        def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+            return cls(torch.ones(3))
+
+    class Sub(torch.Tensor):
+        pass
+
+    w = Wrapper(torch.ones(3))
+    assert _plain(w) is w and _plain(None) is None
+    t = torch.ones(3, requires_grad=True)
+    assert _plain(t) is t
+    s = torch.ones(3).as_subclass(Sub).requires_grad_(True)
+    p = _plain(s)
+    assert type(p) is torch.Tensor and p.data_ptr() == s.data_ptr() and type(torch.autograd.grad(p.sum(), [s])[0]) in (torch.Tensor, Sub)

@@ -3,8 +3,8 @@
 
 The reference has the norms as ``nn.RMSNorm`` with a residual sum of its own (``model_ref.py:49-66, 165-204``) and no
 counterpart of the recurrence.  All run in the kernels of ``csrc/ssd_gated_scan.cu`` and ``csrc/ssd_norm.cu`` on the current
-CUDA stream, without a CPU path, and never synchronise the host.  Gradients are backward ones; an operand with a forward-mode tangent is
-refused (NotImplementedError).
+CUDA stream, without a CPU path, and never synchronise the host.  Gradients are backward ones, recorded by autograd; an operand with a
+forward-mode tangent or under a function transform (``torch.func``) is refused (NotImplementedError).
 """
 from __future__ import annotations
 

@@ -94,8 +94,8 @@ def _plain(t: Optional[torch.Tensor]) -> Optional[torch.Tensor]:
     if t is None or type(t) in (torch.Tensor, torch.nn.Parameter):
         return t
     with torch._C.DisableTorchFunctionSubclass():
-        plain = t.as_subclass(torch.Tensor)
         try:
+            plain = t.as_subclass(torch.Tensor)
             return plain if plain.numel() == 0 or plain.data_ptr() else t
         except RuntimeError:
             return t
