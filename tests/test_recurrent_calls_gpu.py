@@ -349,3 +349,57 @@ def test_function_transforms_are_refused_by_name(transform):
                        ("gated_rms_norm", lambda t: W().gated_rms_norm(t, t, w)), ("conv1d_silu", lambda t: W().conv1d_silu(t, torch.ones(16, 1, 2, device=DEV)))):
         with pytest.raises(NotImplementedError, match=name):
             transform(call)(x if transform is torch.func.vmap else x[0])
+
+
+_CAPTURE_BESIDE_AN_EAGER_GRAPH = """
+import torch
+import workloadsuite_b200 as W
+
+x = torch.randn(2, 40, 16, device="cuda", requires_grad=True)
+w = torch.ones(16, device="cuda", requires_grad=True)
+alive, side = W.gated_scan(x, x, x, w), torch.cuda.Stream()      # recorded on another stream than the one that captures
+torch.cuda.synchronize()
+try:
+    with torch.cuda.graph(torch.cuda.CUDAGraph(), stream=side):
+        torch.autograd.grad([W.gated_scan(x, x, x, w)], [x, w], [torch.ones_like(x)])
+except RuntimeError as e:
+    print("raised", e)
+"""
+
+_BACKWARD_WITHOUT_MEMORY = """
+import torch
+import workloadsuite_b200 as W
+
+x = torch.randn(4096, 4096, device="cuda", requires_grad=True)
+w = torch.ones(4096, device="cuda", requires_grad=True)
+calls = [W.rms_norm(x, w), W.gated_rms_norm(x, x, w), W.gated_scan(x[None], x[None], x[None], w)[0], W.conv1d_silu(x[None], torch.ones(4096, 1, 2, device="cuda"))[0]]
+dy = torch.ones_like(x)
+free = torch.cuda.memory_reserved()
+torch.cuda.set_per_process_memory_fraction(free / torch.cuda.get_device_properties(0).total_memory)
+keep = []
+try:
+    while True:
+        keep.append(torch.empty(1 << 20, device="cuda"))
+except torch.OutOfMemoryError:
+    pass
+raised = 0
+for y in calls:
+    try:
+        torch.autograd.grad([y], [x], [dy])
+    except torch.OutOfMemoryError:
+        raised += 1
+assert raised == len(calls), raised
+del keep
+torch.cuda.empty_cache()
+torch.cuda.set_per_process_memory_fraction(1.0)
+for y in (W.rms_norm(x, w),):
+    torch.autograd.grad([y], [x], [dy])
+print("raised")
+"""
+
+
+@pytest.mark.parametrize("program", [_CAPTURE_BESIDE_AN_EAGER_GRAPH, _BACKWARD_WITHOUT_MEMORY], ids=["capture", "memory"])
+def test_what_a_backward_pass_runs_into_is_raised(program):
+    """In processes of their own: a capture that PyTorch cannot make, an allocation that fails in autograd's thread."""
+    r = subprocess.run([sys.executable, "-c", program], cwd=Path(__file__).resolve().parent.parent, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "raised" in r.stdout, (r.returncode, r.stdout[-500:], r.stderr[-2000:])
